@@ -16,8 +16,8 @@ _lock = threading.Lock()
 _gpu = None
 _synth = None
 
-c_u32, c_i32, c_u64, c_f32, c_vp, c_int = (ctypes.c_uint32, ctypes.c_int32, ctypes.c_uint64, ctypes.c_float,
-                                           ctypes.c_void_p, ctypes.c_int)
+c_u32, c_i32, c_u64, c_f32, c_vp, c_int, c_sz = (ctypes.c_uint32, ctypes.c_int32, ctypes.c_uint64, ctypes.c_float,
+                                                 ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t)
 
 
 class Stats(ctypes.Structure):
@@ -76,6 +76,34 @@ GPU_API = [
     ("lfm_gpu_moe_profile_read", c_int, [c_vp, ctypes.POINTER(KernelTime), c_u32, ctypes.POINTER(c_u32)]),
 ]
 
+class Kv(ctypes.Structure):
+    _fields_ = [("pages", c_vp), ("n_pages", c_u32), ("page_tokens", c_u32), ("n_kv_heads", c_u32),
+                ("head_dim", c_u32)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", c_u32), ("n_tokens", c_u32), ("table_stride", c_u32), ("max_kv_len", c_u32),
+                ("q_start", c_vp), ("kv_len", c_vp), ("page_table", c_vp)]
+
+
+class Rope(ctypes.Structure):
+    _fields_ = [("cos", c_vp), ("sin", c_vp), ("n_pos", c_u32), ("rot_dim", c_u32), ("pairs", c_int), ("eps", c_f32),
+                ("q_norm", c_vp), ("k_norm", c_vp)]
+
+
+# every entry point of include/lfm_gpu_attn.h
+ATTN_API = [
+    ("lfm_gpu_kv_page_bytes", c_sz, [c_u32, c_u32, c_u32]),
+    ("lfm_gpu_add_rmsnorm", c_int, [c_vp, c_vp, c_vp, c_u32, c_u32, c_u32, c_vp, c_f32, c_vp, c_vp, c_u32, c_vp, c_vp]),
+    ("lfm_gpu_q8k_read", c_int, [c_vp, c_vp, c_u32, c_u32, c_u32, c_vp, c_vp]),
+    ("lfm_gpu_kv_append", c_int, [c_vp, ctypes.POINTER(Kv), ctypes.POINTER(KvBatch), ctypes.POINTER(Rope), c_u32, c_u32,
+                                  c_vp, c_sz, c_vp, c_sz, c_vp, c_sz, c_vp, c_sz, c_vp]),
+    ("lfm_gpu_kv_read", c_int, [c_vp, ctypes.POINTER(Kv), ctypes.POINTER(KvBatch), c_u32, c_vp, c_vp, c_vp]),
+    ("lfm_gpu_attn_forward", c_int, [c_vp, ctypes.POINTER(Kv), ctypes.POINTER(KvBatch), c_u32, c_f32, c_int, c_u32,
+                                     c_f32, c_u32, c_vp, c_sz, c_vp, c_sz, c_vp]),
+    ("lfm_gpu_attn_reserve", c_int, [c_vp]),
+]
+
 SYNTH_API = [
     ("lfm_synth_u64", c_u64, [c_u64, c_u64]),
     ("lfm_synth_normal", ctypes.c_double, [c_u64, c_u64]),
@@ -89,12 +117,12 @@ SYNTH_API = [
 ]
 
 
-def header_functions() -> list:
-    """Names of the functions include/lfm_gpu_moe.h declares."""
-    path = os.path.join(_build.ROOT, "include", "lfm_gpu_moe.h")
+def header_functions(header: str = "lfm_gpu_moe.h", prefix: str = "lfm_gpu_moe_") -> list:
+    """Names of the functions include/<header> declares."""
+    path = os.path.join(_build.ROOT, "include", header)
     text = open(path).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
-    return sorted(set(re.findall(r"\b(lfm_gpu_moe_\w+)\s*\(", text)))
+    return sorted(set(re.findall(r"\b(" + prefix + r"\w+)\s*\(", text)))
 
 
 def _bind(lib, api):
@@ -114,7 +142,7 @@ def load_gpu(build_if_missing: bool = True):
                 _build.build_gpu()
             if not os.path.exists(_build.GPU_SO):
                 raise RuntimeError(f"CUDA library missing: {_build.GPU_SO} (run python -m laii_b200.build)")
-            _gpu = _bind(ctypes.CDLL(_build.GPU_SO), GPU_API)
+            _gpu = _bind(ctypes.CDLL(_build.GPU_SO), GPU_API + ATTN_API)
         return _gpu
 
 

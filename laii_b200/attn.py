@@ -1,0 +1,223 @@
+"""Python host API over include/lfm_gpu_attn.h on torch tensors of the handle's device.
+
+What an lfm2moe layer does before its MoE FFN (``laii_b200.moe``): the residual's addition with RMSNorm and
+Q8_K rows, q/k normalisation and rotation with keys and values into a paged 4-bit cache, and grouped-query
+attention over it.  Calls run on torch's current stream, asynchronously; errors come back as ``MoEError`` with
+the library's status code, wrong tensors as ``ValueError``; there is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native
+from .moe import GpuMoE, MoEError
+from .synth import Q8K_BYTES
+
+GGML_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+def _type(dtype: torch.dtype, what: str) -> int:
+    t = GGML_TYPE.get(dtype)
+    if t is None:
+        raise ValueError(f"{what}: {dtype} (float32, float16 or bfloat16)")
+    return t
+
+
+def _dense(t: Optional[torch.Tensor], what: str, dtype: torch.dtype, device: torch.device, ndim: int) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or t.dim() != ndim or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {ndim}-d {dtype} tensor on {device}")
+    return t.data_ptr()
+
+
+class KVPages:
+    """One layer's pool of 4-bit cache pages over a uint8 tensor that the caller owns (layout: lfm_gpu_kv_t)."""
+
+    def __init__(self, pages: torch.Tensor, page_tokens: int, n_kv_heads: int, head_dim: int):
+        size = self.page_bytes(page_tokens, n_kv_heads, head_dim)
+        if size == 0:
+            raise ValueError(f"no cache of {page_tokens}-token pages and {n_kv_heads} heads of {head_dim}")
+        if pages.dtype != torch.uint8 or not pages.is_cuda or not pages.is_contiguous() or pages.numel() % size:
+            raise ValueError(f"pages must be a contiguous uint8 CUDA tensor of whole {size}-byte pages")
+        self.pages, self.page_tokens, self.n_kv_heads, self.head_dim = pages, page_tokens, n_kv_heads, head_dim
+        self.n_pages = pages.numel() // size
+        self._c = _native.Kv(pages.data_ptr(), self.n_pages, page_tokens, n_kv_heads, head_dim)
+
+    @staticmethod
+    def page_bytes(page_tokens: int, n_kv_heads: int, head_dim: int) -> int:
+        """Bytes of a page, 0 for a shape that is not supported."""
+        return _native.load_gpu().lfm_gpu_kv_page_bytes(page_tokens, n_kv_heads, head_dim)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, device="cuda") -> "KVPages":
+        size = cls.page_bytes(page_tokens, n_kv_heads, head_dim)
+        return cls(torch.empty(n_pages, size, dtype=torch.uint8, device=device), page_tokens, n_kv_heads, head_dim)
+
+
+class KVBatch:
+    """A ragged batch: int32 device tensors q_start [n + 1], kv_len [n] and page_table [n, pages], read when a call
+    runs (lfm_gpu_kv_batch_t).  max_kv_len plans the work; any value is safe."""
+
+    def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, max_kv_len: int = 0):
+        n, dev = kv_len.numel(), kv_len.device
+        if not kv_len.is_cuda or q_start.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
+            raise ValueError("q_start [n + 1], kv_len [n] and page_table [n, pages] on one CUDA device")
+        self.device = dev
+        self._keep = (q_start, kv_len, page_table)
+        self._c = _native.KvBatch(n, 0, page_table.shape[1], max_kv_len, _dense(q_start, "q_start", torch.int32, dev, 1),
+                                  _dense(kv_len, "kv_len", torch.int32, dev, 1),
+                                  _dense(page_table, "page_table", torch.int32, dev, 2))
+
+    def rows(self, n_tokens: int) -> "ctypes.Structure":
+        self._c.n_tokens = n_tokens
+        return self._c
+
+
+class Rope:
+    """Per-head norms and the rotation that append applies (lfm_gpu_rope_t): cos and sin fp32 [positions, rot_dim / 2]."""
+
+    def __init__(self, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, pairs: bool = False,
+                 q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-5):
+        if (cos is None) != (sin is None) or (cos is not None and cos.shape != sin.shape):
+            raise ValueError("cos and sin come together, of one shape")
+        given = [t for t in (cos, q_norm, k_norm) if t is not None]
+        dev = given[0].device if given else None
+        self._keep = (cos, sin, q_norm, k_norm)
+        self.norm_dim = {t.numel() for t in (q_norm, k_norm) if t is not None}
+        self._c = _native.Rope(_dense(cos, "cos", torch.float32, dev, 2), _dense(sin, "sin", torch.float32, dev, 2),
+                               0 if cos is None else cos.shape[0], 0 if cos is None else 2 * cos.shape[1], int(pairs), eps,
+                               _dense(q_norm, "q_norm", torch.float32, dev, 1), _dense(k_norm, "k_norm", torch.float32, dev, 1))
+
+
+class GpuAttn:
+    """The attention-side operators of a handle."""
+
+    def __init__(self, moe: GpuMoE):
+        self.moe = moe
+        self.device = torch.device("cuda", moe.device)
+        self._lib = _native.load_gpu()
+
+    def _check(self, st: int):
+        if st != 0:
+            raise MoEError(st, self._lib.lfm_gpu_moe_last_error(self.moe._h).decode(errors="replace"))
+
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _rows(self, t: torch.Tensor, what: str, heads: Optional[int], dim: int, dtype=None) -> Tuple[int, int]:
+        """Pointer and token stride of rows [tokens, heads, dim]."""
+        if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads) or t.device != self.device:
+            raise ValueError(f"{what} must be [tokens, {heads or 'heads'}, {dim}] on {self.device}")
+        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
+            raise ValueError(f"{what}: the heads of a token must lie one behind the other")
+        if dtype is not None and t.dtype != dtype:
+            raise ValueError(f"{what} is {t.dtype}, not {dtype}")
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
+
+    def _same_device(self, cache: KVPages, batch: KVBatch):
+        if cache.pages.device != self.device or batch.device != self.device:
+            raise ValueError(f"cache and batch must be on {self.device}")
+
+    # -- residual addition, RMSNorm, Q8_K ---------------------------------
+    def add_rmsnorm(self, x: torch.Tensor, delta: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float = 1e-5,
+                    x_out: Optional[torch.Tensor] = None, xb_dtype: Optional[torch.dtype] = None, q8: bool = True
+                    ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """(x + delta, its RMSNorm as xb_dtype or None, its RMSNorm as block_q8_K bytes [T, D / 256, 292] or None).
+        x fp32 [T, D]; x_out may be x (in place)."""
+        xp = _dense(x, "x", torch.float32, self.device, 2)
+        T, D = x.shape
+        dt = 0
+        if delta is not None:
+            dt = _type(delta.dtype, "delta")
+            if delta.shape != x.shape:
+                raise ValueError("delta must have the shape of x")
+        if weight is not None and weight.numel() != D:
+            raise ValueError(f"weight must have {D} values")
+        if x_out is None:
+            x_out = torch.empty_like(x)
+        elif x_out.shape != x.shape:
+            raise ValueError("x_out must have the shape of x")
+        xb = torch.empty(T, D, dtype=xb_dtype, device=self.device) if xb_dtype is not None else None
+        qb = torch.empty(T, D // 256, Q8K_BYTES, dtype=torch.uint8, device=self.device) if q8 else None
+        self._check(self._lib.lfm_gpu_add_rmsnorm(
+            self.moe._h, xp, _dense(delta, "delta", delta.dtype if delta is not None else None, self.device, 2), dt, T, D,
+            _dense(weight, "weight", torch.float32, self.device, 1), eps, _dense(x_out, "x_out", torch.float32, self.device, 2),
+            None if xb is None else xb.data_ptr(), 0 if xb is None else _type(xb_dtype, "xb_dtype"),
+            None if qb is None else qb.data_ptr(), self._stream()))
+        return x_out, xb, qb
+
+    def read_q8(self, q8: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+        """The values of block_q8_K rows [T, D / 256, 292] as [T, D]."""
+        p = _dense(q8, "q8", torch.uint8, self.device, 3)
+        if q8.shape[2] != Q8K_BYTES:
+            raise ValueError(f"q8 must be [T, D / 256, {Q8K_BYTES}]")
+        out = torch.empty(q8.shape[0], q8.shape[1] * 256, dtype=dtype, device=self.device)
+        self._check(self._lib.lfm_gpu_q8k_read(self.moe._h, p, q8.shape[0], out.shape[1], _type(dtype, "dtype"), out.data_ptr(),
+                                               self._stream()))
+        return out
+
+    # -- the cache ----------------------------------------------------------
+    def append(self, cache: KVPages, batch: KVBatch, q: Optional[torch.Tensor], k: Optional[torch.Tensor],
+               v: Optional[torch.Tensor], rope: Optional[Rope] = None, q_out: Optional[torch.Tensor] = None
+               ) -> Optional[torch.Tensor]:
+        """k and v [tokens, kv heads, dim] into the cache; returns q [tokens, heads, dim] normalised and rotated
+        (into q_out, which may be q).  Either of q and (k, v) may be None."""
+        self._same_device(cache, batch)
+        first = q if q is not None else k
+        if first is None or (k is None) != (v is None):
+            raise ValueError("q, or k and v, or all three")
+        T, dt, d = first.shape[0], first.dtype, cache.head_dim
+        qa = oa = ka = va = (None, 0)
+        if q is not None:
+            qa = self._rows(q, "q", None, d, dt)
+            if q_out is None:
+                q_out = torch.empty(T, q.shape[1], d, dtype=dt, device=self.device)
+            elif q_out.shape != q.shape:
+                raise ValueError("q_out must have the shape of q")
+            oa = self._rows(q_out, "q_out", q.shape[1], d, dt)
+        if k is not None:
+            if k.shape[0] != T or v.shape[0] != T:
+                raise ValueError("q, k and v must have the same number of tokens")
+            ka, va = self._rows(k, "k", cache.n_kv_heads, d, dt), self._rows(v, "v", cache.n_kv_heads, d, dt)
+        if rope is not None and rope.norm_dim - {d}:
+            raise ValueError(f"q_norm and k_norm must have {d} values")
+        self._check(self._lib.lfm_gpu_kv_append(
+            self.moe._h, ctypes.byref(cache._c), ctypes.byref(batch.rows(T)), None if rope is None else ctypes.byref(rope._c),
+            _type(dt, "q"), 0 if q is None else q.shape[1], qa[0], qa[1], oa[0], oa[1], ka[0], ka[1], va[0], va[1],
+            self._stream()))
+        return q_out
+
+    def read(self, cache: KVPages, batch: KVBatch, n_tokens: int, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The keys and values that the cache holds for the batch's n_tokens rows, [n_tokens, kv heads, dim] each."""
+        self._same_device(cache, batch)
+        k = torch.empty(n_tokens, cache.n_kv_heads, cache.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        self._check(self._lib.lfm_gpu_kv_read(self.moe._h, ctypes.byref(cache._c), ctypes.byref(batch.rows(n_tokens)),
+                                              _type(dtype, "dtype"), k.data_ptr(), v.data_ptr(), self._stream()))
+        return k, v
+
+    # -- attention ------------------------------------------------------------
+    def attend(self, cache: KVPages, batch: KVBatch, q: torch.Tensor, scale: Optional[float] = None, causal: bool = True,
+               window: int = 0, softcap: float = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """softmax(scale q k) v over the cache, [tokens, heads, dim] like q (scale None: dim ** -0.5)."""
+        self._same_device(cache, batch)
+        d = cache.head_dim
+        qp, qs = self._rows(q, "q", None, d)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        elif out.shape != q.shape:
+            raise ValueError("out must have the shape of q")
+        op, os_ = self._rows(out, "out", q.shape[1], d, q.dtype)
+        self._check(self._lib.lfm_gpu_attn_forward(
+            self.moe._h, ctypes.byref(cache._c), ctypes.byref(batch.rows(q.shape[0])), q.shape[1],
+            d ** -0.5 if scale is None else scale, int(causal), window, softcap, _type(q.dtype, "q"), qp, qs, op, os_,
+            self._stream()))
+        return out
+
+    def reserve(self):
+        """Allocate attend's scratch now (needed before a stream capture)."""
+        self._check(self._lib.lfm_gpu_attn_reserve(self.moe._h))

@@ -1,6 +1,6 @@
 """Build the native libraries in-tree (laii_b200/_lib/).
 
-  liblfm_gpu_moe.so  CUDA kernels + C-ABI (include/lfm_gpu_moe.h), sm_100a only
+  liblfm_gpu_moe.so  CUDA kernels + C-ABI (include/lfm_gpu_moe.h, lfm_gpu_attn.h), sm_100a only
   liblfm_synth.so    host seeded-input generator (C)
 
 nvcc flags: -gencode arch=compute_100a,code=sm_100a; -fmad=false and
@@ -26,8 +26,9 @@ BUILD = os.path.join(PKG, "_build")
 GPU_SO = os.path.join(LIB, "liblfm_gpu_moe.so")
 SYNTH_SO = os.path.join(LIB, "liblfm_synth.so")
 
-CU_SOURCES = ["lfm_gpu_moe.cu", "k_route.cu", "k_gemv.cu", "k_layer.cu", "k_gemm.cu", "k_umma.cu", "k_expert.cu", "k_ep.cu", "k_q6k.cu", "k_synth.cu", "lfm_gguf.cpp"]
-HEADERS = ["lfm_formats.h", "lfm_synth_core.h", "moe_internal.h", "moe_device.cuh"]
+CU_SOURCES = ["lfm_gpu_moe.cu", "k_route.cu", "k_gemv.cu", "k_layer.cu", "k_gemm.cu", "k_umma.cu", "k_expert.cu", "k_ep.cu", "k_q6k.cu", "k_synth.cu", "lfm_gguf.cpp",
+              "lfm_gpu_attn.cu", "k_norm.cu", "k_kv.cu", "k_attn.cu"]
+HEADERS = ["lfm_formats.h", "lfm_synth_core.h", "moe_internal.h", "moe_device.cuh", "attn_internal.h", "attn_device.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -95,6 +96,7 @@ def build_synth(force: bool = False) -> str:
 def build_gpu(force: bool = False, verbose_ptxas: bool = False) -> str:
     srcs = [os.path.join(CSRC, s) for s in CU_SOURCES]
     deps = srcs + [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(ROOT, "include", "lfm_gpu_moe.h"),
+                                                              os.path.join(ROOT, "include", "lfm_gpu_attn.h"),
                                                               os.path.abspath(__file__)]
     if not (force or _stale(GPU_SO, deps)):
         return GPU_SO

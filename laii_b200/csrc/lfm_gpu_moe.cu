@@ -16,6 +16,7 @@
 #include <mutex>
 #include <vector>
 
+#include "attn_internal.h"
 #include "lfm_gpu_moe.h"
 #include "moe_internal.h"
 
@@ -63,10 +64,11 @@ struct Workspace {
 
 namespace {
 enum KernelId { K_ROUTE, K_GATEUP, K_QUANT_H, K_DOWN, K_COMBINE, K_LAYER, K_PLAN, K_GEMM_G, K_GEMM_U, K_SWIGLU, K_GEMM_D,
-                K_XT, K_GEMM_GU, K_EP_PUBLISH, K_EP_PLAN, K_COUNT };
+                K_XT, K_GEMM_GU, K_EP_PUBLISH, K_EP_PLAN, K_ATTN_SIDE, K_COUNT = K_ATTN_SIDE + 5 };
 const char *const kKernelNames[K_COUNT] = {"route", "gateup", "quant_h", "down", "combine", "moe_layer",
                                            "gemm_plan", "gemm_gate", "gemm_up", "swiglu_q8", "gemm_down",
-                                           "xt_gather", "gemm_gateup", "ep_publish", "ep_plan"};
+                                           "xt_gather", "gemm_gateup", "ep_publish", "ep_plan",
+                                           "add_rmsnorm", "q8k_read", "kv_append", "kv_read", "attn"};
 struct ProfRec {
     int kid;
     cudaEvent_t a, b;
@@ -444,6 +446,23 @@ lfm_gpu_status_t read_device_error(lfm_gpu_moe_t *h) {
 }
 
 }  // namespace
+
+/* ---- what the attention side (lfm_gpu_attn.cu) uses of a handle ---- */
+HostView lfm_host_view(lfm_gpu_moe_t *h) { return HostView{h->device, h->sm_count, !h->prof && h->use_pdl, h->dev_err}; }
+
+lfm_gpu_status_t lfm_host_fail(lfm_gpu_moe_t *h, lfm_gpu_status_t st, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(h->err, sizeof h->err, fmt, ap);
+    va_end(ap);
+    return st;
+}
+
+lfm_gpu_status_t lfm_host_cuda_fail(lfm_gpu_moe_t *h, cudaError_t e, const char *what) { return cuda_fail(h, e, what); }
+
+cudaError_t lfm_host_timed(lfm_gpu_moe_t *h, AttnKernelId id, cudaStream_t s, cudaError_t (*fn)(void *), void *ctx) {
+    return timed(h, K_ATTN_SIDE + (int)id, s, [&] { return fn(ctx); }, 0);
+}
 
 LFM_API lfm_gpu_status_t lfm_gpu_moe_create(lfm_gpu_moe_t **out, int device_id) {
     if (!out) return LFM_GPU_ERR_INVALID_ARG;

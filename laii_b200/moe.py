@@ -263,10 +263,10 @@ class GpuMoE:
 
     def profile_read(self) -> dict:
         """{kernel name: (launches, total ms)} since the last read; clears the records."""
-        buf = (_native.KernelTime * 16)()
+        buf = (_native.KernelTime * 32)()
         n = ctypes.c_uint32()
-        self._check(self._lib.lfm_gpu_moe_profile_read(self._h, buf, 16, ctypes.byref(n)))
-        return {buf[i].name.decode(): (buf[i].launches, buf[i].total_ms) for i in range(min(n.value, 16))}
+        self._check(self._lib.lfm_gpu_moe_profile_read(self._h, buf, 32, ctypes.byref(n)))
+        return {buf[i].name.decode(): (buf[i].launches, buf[i].total_ms) for i in range(min(n.value, 32))}
 
     def last_stats(self) -> dict:
         s = _native.Stats()
