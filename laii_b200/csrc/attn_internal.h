@@ -72,7 +72,13 @@ cudaError_t lfm_launch_q8k_read(const uint8_t *q8, uint32_t rows, uint32_t D, ui
                                 bool pdl);
 cudaError_t lfm_launch_kv_append(const AppendArgs &a, uint32_t head_dim, uint32_t type, cudaStream_t s, bool pdl);
 cudaError_t lfm_launch_kv_read(const ReadArgs &a, uint32_t head_dim, uint32_t type, cudaStream_t s, bool pdl);
-cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, cudaStream_t s, bool pdl);
+/* max_kv_len plans the splits of long sequences, scratch holds their parts (LFM_ATTN_SCRATCH_BYTES, the leading
+ * LFM_ATTN_COUNTS words zero; the kernels leave them zero). */
+cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
+                            cudaStream_t s, bool pdl);
+#define LFM_ATTN_COUNTS 16384u
+#define LFM_ATTN_PARTS_BYTES ((size_t)32 << 20)
+#define LFM_ATTN_SCRATCH_BYTES (LFM_ATTN_PARTS_BYTES + LFM_ATTN_COUNTS * sizeof(uint32_t))
 
 /* ---- the handle, as lfm_gpu_moe.cu keeps it ------------------------------ */
 enum AttnKernelId { AK_NORM, AK_Q8K_READ, AK_APPEND, AK_KV_READ, AK_ATTN };
@@ -87,5 +93,11 @@ lfm_gpu_status_t lfm_host_cuda_fail(lfm_gpu_moe_t *h, cudaError_t e, const char 
 /* fn(ctx), the launch, between the profile's events where profiling is on.
  * (The launch statistics of a handle stay those of its last MoE forward.) */
 cudaError_t lfm_host_timed(lfm_gpu_moe_t *h, AttnKernelId id, cudaStream_t s, cudaError_t (*fn)(void *), void *ctx);
+
+/* The handle's attention scratch for work on `s`, allocated on first use (not
+ * while `s` captures); work that other streams still do on it comes first. */
+lfm_gpu_status_t lfm_host_scratch(lfm_gpu_moe_t *h, cudaStream_t s, void **out);
+/* ... and after that work's launch. */
+lfm_gpu_status_t lfm_host_scratch_used(lfm_gpu_moe_t *h, cudaStream_t s);
 
 #endif /* LFM_ATTN_INTERNAL_H */

@@ -201,6 +201,7 @@ LFM_API lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv
     if (!type_ok(type)) UNSUPPORTED("type %u (F32=0, F16=1, BF16=30)", type);
     if (n_heads == 0 || n_heads > 65535 || n_heads % kv->n_kv_heads)
         FAIL("n_heads=%u is not a multiple of the cache's %u", n_heads, kv->n_kv_heads);
+    if ((uint64_t)batch->n_tokens * n_heads > 0x7FFFFFFFull) FAIL("%u tokens of %u heads: above 2^31 rows", batch->n_tokens, n_heads);
     if (!isfinite(scale)) FAIL("scale=%g", (double)scale);
     if (!(softcap >= 0.0f) || isinf(softcap)) FAIL("softcap=%g", (double)softcap);
     if (window && !causal) FAIL("a window needs causal attention");
@@ -220,11 +221,20 @@ LFM_API lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv
     a.q_stride = q_stride; a.out_stride = out_stride;
     a.err = hv.err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return launch(h, hv, AK_ATTN, "attn_forward", s,
-                  [&] { return lfm_launch_attn(a, kv->head_dim, s, hv.pdl); });
+    OnDevice g(hv.device);
+    void *scratch = nullptr;
+    st = lfm_host_scratch(h, s, &scratch);
+    if (st != LFM_GPU_OK) return st;
+    const uint32_t span = batch->table_stride * kv->page_tokens;
+    const uint32_t hint = batch->max_kv_len && batch->max_kv_len < span ? batch->max_kv_len : span;
+    st = launch(h, hv, AK_ATTN, "attn_forward", s,
+                [&] { return lfm_launch_attn(a, kv->head_dim, hint, hv.sm_count, scratch, s, hv.pdl); });
+    return st == LFM_GPU_OK ? lfm_host_scratch_used(h, s) : st;
 }
 
 LFM_API lfm_gpu_status_t lfm_gpu_attn_reserve(lfm_gpu_moe_t *h) {
     if (!h) return LFM_GPU_ERR_INVALID_ARG;
-    return LFM_GPU_OK;
+    OnDevice g(lfm_host_view(h).device);
+    void *scratch = nullptr;
+    return lfm_host_scratch(h, nullptr, &scratch);
 }

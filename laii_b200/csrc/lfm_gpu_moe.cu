@@ -121,6 +121,10 @@ struct lfm_gpu_moe {
     bool use_pdl = true;     /* chain the kernels with programmatic dependent launch */
     std::vector<GraphEntry> graphs;
     EpP2P ep;
+    void *attn_scratch = nullptr;      /* parts of split sequences (k_attn.cu)           */
+    cudaEvent_t attn_done = nullptr;   /* behind the last work on it                     */
+    cudaStream_t attn_stream = nullptr;
+    bool attn_used = false;
 };
 
 namespace {
@@ -440,6 +444,7 @@ lfm_gpu_status_t read_device_error(lfm_gpu_moe_t *h) {
     if (e == 0) return LFM_GPU_OK;
     LFM_CUDA(h, cudaMemset(h->dev_err, 0, sizeof(uint32_t)));
     /* an abandoned forward can leave completion counters part-way: clear them */
+    if (h->attn_scratch) LFM_CUDA(h, cudaMemset(h->attn_scratch, 0, LFM_ATTN_COUNTS * sizeof(uint32_t)));
     if (h->ws.base) LFM_CUDA(h, cudaMemset(h->ws.base, 0, h->ws.counters_bytes));
     if (e & LFM_DEVERR_TIMEOUT) return fail(h, LFM_GPU_ERR_TIMEOUT, "device wait timed out (0x%x)", e);
     return fail(h, LFM_GPU_ERR_DEVICE_CHECK, "device bounds check tripped (0x%x)", e);
@@ -462,6 +467,37 @@ lfm_gpu_status_t lfm_host_cuda_fail(lfm_gpu_moe_t *h, cudaError_t e, const char 
 
 cudaError_t lfm_host_timed(lfm_gpu_moe_t *h, AttnKernelId id, cudaStream_t s, cudaError_t (*fn)(void *), void *ctx) {
     return timed(h, K_ATTN_SIDE + (int)id, s, [&] { return fn(ctx); }, 0);
+}
+
+static bool capturing(cudaStream_t s) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &st) != cudaSuccess) cudaGetLastError();
+    return st != cudaStreamCaptureStatusNone;
+}
+
+lfm_gpu_status_t lfm_host_scratch(lfm_gpu_moe_t *h, cudaStream_t s, void **out) {
+    if (!h->attn_scratch) {
+        if (capturing(s)) return fail(h, LFM_GPU_ERR_NOT_READY, "attention scratch not allocated before a stream capture: call lfm_gpu_attn_reserve");
+        void *p = nullptr;
+        if (!h->attn_done) LFM_CUDA(h, cudaEventCreateWithFlags(&h->attn_done, cudaEventDisableTiming));
+        cudaError_t e = cudaMalloc(&p, LFM_ATTN_SCRATCH_BYTES);
+        if (e != cudaSuccess) return cuda_fail(h, e, "attention scratch cudaMalloc");
+        e = cudaMemset(p, 0, LFM_ATTN_COUNTS * sizeof(uint32_t));
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        if (e != cudaSuccess) { cudaFree(p); return cuda_fail(h, e, "attention scratch memset"); }
+        h->attn_scratch = p;
+    }
+    if (h->attn_used && s != h->attn_stream && !capturing(s)) LFM_CUDA(h, cudaStreamWaitEvent(s, h->attn_done, 0));
+    *out = h->attn_scratch;
+    return LFM_GPU_OK;
+}
+
+lfm_gpu_status_t lfm_host_scratch_used(lfm_gpu_moe_t *h, cudaStream_t s) {
+    if (capturing(s)) return LFM_GPU_OK; /* replays are ordered by their caller */
+    LFM_CUDA(h, cudaEventRecord(h->attn_done, s));
+    h->attn_stream = s;
+    h->attn_used = true;
+    return LFM_GPU_OK;
 }
 
 LFM_API lfm_gpu_status_t lfm_gpu_moe_create(lfm_gpu_moe_t **out, int device_id) {
@@ -511,6 +547,11 @@ LFM_API void lfm_gpu_moe_destroy(lfm_gpu_moe_t *h) {
     if (h->ws.base) cudaFree(h->ws.base);
     if (h->dev_err) cudaFree(h->dev_err);
     if (h->loads) cudaFree(h->loads);
+    if (h->attn_scratch) {
+        cudaDeviceSynchronize(); /* callers' streams may still work on it */
+        cudaFree(h->attn_scratch);
+    }
+    if (h->attn_done) cudaEventDestroy(h->attn_done);
     for (ProfRec &r : h->recs) { cudaEventDestroy(r.a); cudaEventDestroy(r.b); }
     if (h->ep.attached) {
         cudaDeviceSynchronize();
