@@ -26,11 +26,12 @@ def _type(dtype: torch.dtype, what: str) -> int:
     return t
 
 
-def _dense(t: Optional[torch.Tensor], what: str, dtype: torch.dtype, device: torch.device, ndim: int) -> Optional[int]:
+def _dense(t: Optional[torch.Tensor], what: str, dtype: torch.dtype, index: int, ndim: int) -> Optional[int]:
+    """The address of a contiguous tensor on CUDA device `index` (None stays None)."""
     if t is None:
         return None
-    if t.dtype != dtype or t.device != device or t.dim() != ndim or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {ndim}-d {dtype} tensor on {device}")
+    if t.dtype != dtype or t.get_device() != index or t.dim() != ndim or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {ndim}-d {dtype} tensor on CUDA device {index}")
     return t.data_ptr()
 
 
@@ -45,7 +46,9 @@ class KVPages:
             raise ValueError(f"pages must be a contiguous uint8 CUDA tensor of whole {size}-byte pages")
         self.pages, self.page_tokens, self.n_kv_heads, self.head_dim = pages, page_tokens, n_kv_heads, head_dim
         self.n_pages = pages.numel() // size
+        self.index = pages.get_device()
         self._c = _native.Kv(pages.data_ptr(), self.n_pages, page_tokens, n_kv_heads, head_dim)
+        self._ref = ctypes.byref(self._c)
 
     @staticmethod
     def page_bytes(page_tokens: int, n_kv_heads: int, head_dim: int) -> int:
@@ -63,18 +66,20 @@ class KVBatch:
     runs (lfm_gpu_kv_batch_t).  max_kv_len plans the work; any value is safe."""
 
     def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, max_kv_len: int = 0):
-        n, dev = kv_len.numel(), kv_len.device
+        n, dev = kv_len.numel(), kv_len.get_device()
         if not kv_len.is_cuda or q_start.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
             raise ValueError("q_start [n + 1], kv_len [n] and page_table [n, pages] on one CUDA device")
-        self.device = dev
+        self.index = dev
         self._keep = (q_start, kv_len, page_table)
         self._c = _native.KvBatch(n, 0, page_table.shape[1], max_kv_len, _dense(q_start, "q_start", torch.int32, dev, 1),
                                   _dense(kv_len, "kv_len", torch.int32, dev, 1),
                                   _dense(page_table, "page_table", torch.int32, dev, 2))
+        self._ref = ctypes.byref(self._c)
 
-    def rows(self, n_tokens: int) -> "ctypes.Structure":
+    def rows(self, n_tokens: int):
+        """The descriptor for a call of n_tokens rows."""
         self._c.n_tokens = n_tokens
-        return self._c
+        return self._ref
 
 
 class Rope:
@@ -85,12 +90,14 @@ class Rope:
         if (cos is None) != (sin is None) or (cos is not None and cos.shape != sin.shape):
             raise ValueError("cos and sin come together, of one shape")
         given = [t for t in (cos, q_norm, k_norm) if t is not None]
-        dev = given[0].device if given else None
+        dev = given[0].get_device() if given else -1
         self._keep = (cos, sin, q_norm, k_norm)
         self.norm_dim = {t.numel() for t in (q_norm, k_norm) if t is not None}
         self._c = _native.Rope(_dense(cos, "cos", torch.float32, dev, 2), _dense(sin, "sin", torch.float32, dev, 2),
                                0 if cos is None else cos.shape[0], 0 if cos is None else 2 * cos.shape[1], int(pairs), eps,
                                _dense(q_norm, "q_norm", torch.float32, dev, 1), _dense(k_norm, "k_norm", torch.float32, dev, 1))
+        self.index = dev
+        self._ref = ctypes.byref(self._c)
 
 
 class GpuAttn:
@@ -98,6 +105,7 @@ class GpuAttn:
 
     def __init__(self, moe: GpuMoE):
         self.moe = moe
+        self.index = moe.device
         self.device = torch.device("cuda", moe.device)
         self._lib = _native.load_gpu()
 
@@ -106,20 +114,20 @@ class GpuAttn:
             raise MoEError(st, self._lib.lfm_gpu_moe_last_error(self.moe._h).decode(errors="replace"))
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        # the address alone: building torch's Stream object takes as long as a launch
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
-    def _rows(self, t: torch.Tensor, what: str, heads: Optional[int], dim: int, dtype=None) -> Tuple[int, int]:
-        """Pointer and token stride of rows [tokens, heads, dim]."""
-        if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads) or t.device != self.device:
-            raise ValueError(f"{what} must be [tokens, {heads or 'heads'}, {dim}] on {self.device}")
-        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
-            raise ValueError(f"{what}: the heads of a token must lie one behind the other")
-        if dtype is not None and t.dtype != dtype:
-            raise ValueError(f"{what} is {t.dtype}, not {dtype}")
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
+    def _rows(self, t: torch.Tensor, what: str, heads: Optional[int], dim: int, dtype) -> int:
+        """Address of rows [tokens, heads, dim]."""
+        shape = t.shape
+        if len(shape) != 3 or not (t.is_contiguous() or (t.stride(2) == 1 and (shape[1] == 1 or t.stride(1) == dim))):
+            raise ValueError(f"{what}: [tokens, heads, {dim}] with the heads of a token one behind the other")
+        if shape[2] != dim or (heads is not None and shape[1] != heads) or t.get_device() != self.index or t.dtype != dtype:
+            raise ValueError(f"{what} must be {dtype} [tokens, {heads or 'heads'}, {dim}] on {self.device}")
+        return t.data_ptr()
 
     def _same_device(self, cache: KVPages, batch: KVBatch):
-        if cache.pages.device != self.device or batch.device != self.device:
+        if cache.index != self.index or batch.index != self.index:
             raise ValueError(f"cache and batch must be on {self.device}")
 
     # -- residual addition, RMSNorm, Q8_K ---------------------------------
@@ -128,11 +136,13 @@ class GpuAttn:
                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
         """(x + delta, its RMSNorm as xb_dtype or None, its RMSNorm as block_q8_K bytes [T, D / 256, 292] or None).
         x fp32 [T, D]; x_out may be x (in place)."""
-        xp = _dense(x, "x", torch.float32, self.device, 2)
+        dev = self.index
+        xp = _dense(x, "x", torch.float32, dev, 2)
         T, D = x.shape
-        dt = 0
+        dp, dt = None, 0
         if delta is not None:
             dt = _type(delta.dtype, "delta")
+            dp = _dense(delta, "delta", delta.dtype, dev, 2)
             if delta.shape != x.shape:
                 raise ValueError("delta must have the shape of x")
         if weight is not None and weight.numel() != D:
@@ -141,22 +151,22 @@ class GpuAttn:
             x_out = torch.empty_like(x)
         elif x_out.shape != x.shape:
             raise ValueError("x_out must have the shape of x")
-        xb = torch.empty(T, D, dtype=xb_dtype, device=self.device) if xb_dtype is not None else None
-        qb = torch.empty(T, D // 256, Q8K_BYTES, dtype=torch.uint8, device=self.device) if q8 else None
+        xb = x.new_empty((T, D), dtype=xb_dtype) if xb_dtype is not None else None
+        qb = x.new_empty((T, D // 256, Q8K_BYTES), dtype=torch.uint8) if q8 else None
         self._check(self._lib.lfm_gpu_add_rmsnorm(
-            self.moe._h, xp, _dense(delta, "delta", delta.dtype if delta is not None else None, self.device, 2), dt, T, D,
-            _dense(weight, "weight", torch.float32, self.device, 1), eps, _dense(x_out, "x_out", torch.float32, self.device, 2),
-            None if xb is None else xb.data_ptr(), 0 if xb is None else _type(xb_dtype, "xb_dtype"),
-            None if qb is None else qb.data_ptr(), self._stream()))
+            self.moe._h, xp, dp, dt, T, D, _dense(weight, "weight", torch.float32, dev, 1), eps,
+            _dense(x_out, "x_out", torch.float32, dev, 2), None if xb is None else xb.data_ptr(),
+            0 if xb is None else _type(xb_dtype, "xb_dtype"), None if qb is None else qb.data_ptr(), self._stream()))
         return x_out, xb, qb
 
     def read_q8(self, q8: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         """The values of block_q8_K rows [T, D / 256, 292] as [T, D]."""
-        p = _dense(q8, "q8", torch.uint8, self.device, 3)
-        if q8.shape[2] != Q8K_BYTES:
+        p = _dense(q8, "q8", torch.uint8, self.index, 3)
+        T, n, size = q8.shape
+        if size != Q8K_BYTES:
             raise ValueError(f"q8 must be [T, D / 256, {Q8K_BYTES}]")
-        out = torch.empty(q8.shape[0], q8.shape[1] * 256, dtype=dtype, device=self.device)
-        self._check(self._lib.lfm_gpu_q8k_read(self.moe._h, p, q8.shape[0], out.shape[1], _type(dtype, "dtype"), out.data_ptr(),
+        out = q8.new_empty((T, n * 256), dtype=dtype)
+        self._check(self._lib.lfm_gpu_q8k_read(self.moe._h, p, T, n * 256, _type(dtype, "dtype"), out.data_ptr(),
                                                self._stream()))
         return out
 
@@ -171,33 +181,35 @@ class GpuAttn:
         if first is None or (k is None) != (v is None):
             raise ValueError("q, or k and v, or all three")
         T, dt, d = first.shape[0], first.dtype, cache.head_dim
-        qa = oa = ka = va = (None, 0)
+        heads = qp = qs = op = os_ = kp = ks = vp = vs = 0
         if q is not None:
-            qa = self._rows(q, "q", None, d, dt)
+            qp, heads = self._rows(q, "q", None, d, dt), q.shape[1]
+            qs = q.stride(0) if T != 1 else heads * d  # the stride of one row says nothing
             if q_out is None:
-                q_out = torch.empty(T, q.shape[1], d, dtype=dt, device=self.device)
-            elif q_out.shape != q.shape:
-                raise ValueError("q_out must have the shape of q")
-            oa = self._rows(q_out, "q_out", q.shape[1], d, dt)
+                q_out = q.new_empty(q.shape)
+            elif q_out.shape[0] < T:
+                raise ValueError("q_out must have the rows of q")
+            op = self._rows(q_out, "q_out", heads, d, dt)
+            os_ = q_out.stride(0) if q_out.shape[0] != 1 else heads * d
         if k is not None:
+            kp, vp = self._rows(k, "k", cache.n_kv_heads, d, dt), self._rows(v, "v", cache.n_kv_heads, d, dt)
+            ks, vs = (k.stride(0), v.stride(0)) if T != 1 else (cache.n_kv_heads * d,) * 2
             if k.shape[0] != T or v.shape[0] != T:
                 raise ValueError("q, k and v must have the same number of tokens")
-            ka, va = self._rows(k, "k", cache.n_kv_heads, d, dt), self._rows(v, "v", cache.n_kv_heads, d, dt)
-        if rope is not None and rope.norm_dim - {d}:
-            raise ValueError(f"q_norm and k_norm must have {d} values")
+        if rope is not None and (rope.norm_dim - {d} or (rope.index >= 0 and rope.index != self.index)):
+            raise ValueError(f"q_norm and k_norm must have {d} values, rotation and norms be on {self.device}")
         self._check(self._lib.lfm_gpu_kv_append(
-            self.moe._h, ctypes.byref(cache._c), ctypes.byref(batch.rows(T)), None if rope is None else ctypes.byref(rope._c),
-            _type(dt, "q"), 0 if q is None else q.shape[1], qa[0], qa[1], oa[0], oa[1], ka[0], ka[1], va[0], va[1],
-            self._stream()))
+            self.moe._h, cache._ref, batch.rows(T), None if rope is None else rope._ref, _type(dt, "q"), heads, qp, qs, op, os_,
+            kp, ks, vp, vs, self._stream()))
         return q_out
 
     def read(self, cache: KVPages, batch: KVBatch, n_tokens: int, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
         """The keys and values that the cache holds for the batch's n_tokens rows, [n_tokens, kv heads, dim] each."""
         self._same_device(cache, batch)
-        k = torch.empty(n_tokens, cache.n_kv_heads, cache.head_dim, dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
-        self._check(self._lib.lfm_gpu_kv_read(self.moe._h, ctypes.byref(cache._c), ctypes.byref(batch.rows(n_tokens)),
-                                              _type(dtype, "dtype"), k.data_ptr(), v.data_ptr(), self._stream()))
+        kv = cache.pages.new_empty((2, n_tokens, cache.n_kv_heads, cache.head_dim), dtype=dtype)
+        k, v = kv.unbind(0)
+        self._check(self._lib.lfm_gpu_kv_read(self.moe._h, cache._ref, batch.rows(n_tokens), _type(dtype, "dtype"),
+                                              k.data_ptr(), v.data_ptr(), self._stream()))
         return k, v
 
     # -- attention ------------------------------------------------------------
@@ -205,16 +217,17 @@ class GpuAttn:
                window: int = 0, softcap: float = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """softmax(scale q k) v over the cache, [tokens, heads, dim] like q (scale None: dim ** -0.5)."""
         self._same_device(cache, batch)
-        d = cache.head_dim
-        qp, qs = self._rows(q, "q", None, d)
+        d, dt = cache.head_dim, q.dtype
+        qp = self._rows(q, "q", None, d, dt)
+        T, heads, _ = shape = q.shape
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape:
-            raise ValueError("out must have the shape of q")
-        op, os_ = self._rows(out, "out", q.shape[1], d, q.dtype)
+            out = q.new_empty(shape)
+        elif out.shape[0] < T:
+            raise ValueError("out must have the rows of q")
+        op = self._rows(out, "out", heads, d, dt)
         self._check(self._lib.lfm_gpu_attn_forward(
-            self.moe._h, ctypes.byref(cache._c), ctypes.byref(batch.rows(q.shape[0])), q.shape[1],
-            d ** -0.5 if scale is None else scale, int(causal), window, softcap, _type(q.dtype, "q"), qp, qs, op, os_,
+            self.moe._h, cache._ref, batch.rows(T), heads, d ** -0.5 if scale is None else scale, causal, window, softcap,
+            _type(dt, "q"), qp, q.stride(0) if T != 1 else heads * d, op, out.stride(0) if out.shape[0] != 1 else heads * d,
             self._stream()))
         return out
 

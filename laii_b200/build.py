@@ -27,7 +27,7 @@ GPU_SO = os.path.join(LIB, "liblfm_gpu_moe.so")
 SYNTH_SO = os.path.join(LIB, "liblfm_synth.so")
 
 CU_SOURCES = ["lfm_gpu_moe.cu", "k_route.cu", "k_gemv.cu", "k_layer.cu", "k_gemm.cu", "k_umma.cu", "k_expert.cu", "k_ep.cu", "k_q6k.cu", "k_synth.cu", "lfm_gguf.cpp",
-              "lfm_gpu_attn.cu", "k_norm.cu", "k_kv.cu", "k_attn.cu"]
+              "lfm_gpu_attn.cu", "k_norm.cu", "k_kv.cu", "k_attn.cu", "k_attn_tile.cu"]
 HEADERS = ["lfm_formats.h", "lfm_synth_core.h", "moe_internal.h", "moe_device.cuh", "attn_internal.h", "attn_device.cuh"]
 
 NVCC_FLAGS = [

@@ -110,4 +110,87 @@ __device__ __forceinline__ uint8_t *lfm_page(const KvDev &kv, const BatchDev &bt
     return nullptr;
 }
 
+/* Rows q0 .. q0 + n of a call of n_tokens. */
+__device__ __forceinline__ bool lfm_sane(const BatchDev &bt, int64_t q0, int64_t n) {
+    return q0 >= 0 && n >= 0 && q0 + n <= (int64_t)bt.n_tokens;
+}
+
+/* One warp: the want-th tile of `per` rows (token, head of a group of G) over the sequences with more than `above`
+ * and at most `most` rows, `skip` tiles left out of each: (sequence, tile) into out, or a sequence of -1. */
+__device__ __forceinline__ void lfm_find_tile(const BatchDev &bt, uint32_t G, uint32_t per, uint32_t skip, uint64_t above,
+                                              uint64_t most, uint64_t want, int *out) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint64_t before = 0;
+    for (uint32_t b0 = 0; b0 < bt.n_seqs; b0 += 32) {
+        uint64_t n = 0;
+        if (b0 + lane < bt.n_seqs) {
+            const int64_t q = bt.q_start[b0 + lane], q_n = (int64_t)bt.q_start[b0 + lane + 1] - q;
+            const uint64_t rows = q_n > 0 && lfm_sane(bt, q, q_n) ? (uint64_t)q_n * G : 0;
+            if (rows > above && rows <= most) n = (rows - 1) / per + 1 - skip;
+        }
+        uint64_t sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t v = __shfl_up_sync(LFM_FULL_MASK, sum, o);
+            if (lane >= (uint32_t)o) sum += v;
+        }
+        const bool here = want >= before + sum - n && want < before + sum;
+        if (here) {
+            out[0] = (int)(b0 + lane);
+            out[1] = (int)(want - (before + sum - n) + skip);
+        }
+        if (__any_sync(LFM_FULL_MASK, here)) return;
+        before += __shfl_sync(LFM_FULL_MASK, sum, 31);
+    }
+    if (lane == 0) out[0] = -1;
+}
+
+/* Codes to fp16: a nibble in an fp16 exponent, bits 0-3 of a half as 1024 + c, bits 4-7 as 64 + c. */
+#define LFM_NIB0_OFF 0x64086408u /* 1032, 1032: the exponent's offset and the code's own 8 */
+#define LFM_NIB1_OFF 0x54805480u /*   72,   72 */
+__device__ __forceinline__ uint32_t lfm_nib0(uint32_t x) { return (x & 0x000F000Fu) | 0x64006400u; }
+__device__ __forceinline__ uint32_t lfm_nib1(uint32_t x) { return (x & 0x00F000F0u) | 0x54005400u; }
+__device__ __forceinline__ uint32_t lfm_hsub2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t lfm_hmul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float lfm_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lfm_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+#define LFM_NO_KEY -1e30f /* the running reference of a row that has seen no key */
+
+/* Eight values of a q row at `at`, saturated to fp16's finite range (NaN stays), negated for a negative scale. */
+__device__ __forceinline__ void lfm_load_q(const AttnArgs &A, size_t at, bool neg, float (&v)[8]) {
+    if (A.type == 0) lfm_load<8>(static_cast<const float *>(A.q) + at, v);
+    else if (A.type == 1) lfm_load<8>(static_cast<const __half *>(A.q) + at, v);
+    else lfm_load<8>(static_cast<const __nv_bfloat16 *>(A.q) + at, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = neg ? -v[i] : v[i];
+        v[i] = x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+    }
+}
+
+/* Keys [lo, hi) that row r (token, head of the group) of a sequence of n_q tokens behind len cached ones sees. */
+__device__ __forceinline__ void lfm_visible(const AttnArgs &A, int64_t n_q, int64_t len, uint32_t r, int64_t &lo,
+                                            int64_t &hi) {
+    hi = A.causal ? len - n_q + (int64_t)(r / A.group) + 1 : len;
+    if (hi < 0) hi = 0;
+    lo = A.window && hi > (int64_t)A.window ? hi - A.window : 0;
+}
+
 #endif /* LFM_ATTN_DEVICE_CUH */

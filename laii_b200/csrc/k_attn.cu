@@ -28,7 +28,6 @@
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32, kStages = 3;
-constexpr float kNone = -1e30f; /* reference of a row that has seen no key */
 
 template <int D>
 struct Cfg {
@@ -38,16 +37,6 @@ struct Cfg {
     static constexpr int kRing = kWarps * kStages * kBytes; /* shared memory        */
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -80,21 +69,6 @@ __device__ __forceinline__ void lds_scales(uint32_t a, uint32_t (&v)[N]) {
     }
 }
 __device__ __forceinline__ float2 half2_of(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-constexpr uint32_t kOff0 = 0x64086408u; /* 1032, 1032 */
-constexpr uint32_t kOff1 = 0x54805480u; /*   72,   72 */
-__device__ __forceinline__ uint32_t nib0(uint32_t x) { return (x & 0x000F000Fu) | 0x64006400u; }
-__device__ __forceinline__ uint32_t nib1(uint32_t x) { return (x & 0x00F000F0u) | 0x54005400u; }
-
 __device__ __forceinline__ void store4(void *p, uint32_t type, size_t at, const float (&v)[4]) {
     if (type == 0) lfm_store<4>(static_cast<float *>(p) + at, v);
     else if (type == 1) lfm_store<4>(static_cast<__half *>(p) + at, v);
@@ -104,6 +78,7 @@ __device__ __forceinline__ void store4(void *p, uint32_t type, size_t at, const 
 struct RowsPlan {
     uint32_t n_splits, chunk; /* blocks of keys a split takes (the last takes what is left) */
     uint32_t extra;           /* blocks past n_seqs that walk the further column tiles       */
+    uint64_t most;            /* rows of the longest sequence that is this kernel's          */
     uint64_t tiles;           /* n_seqs and the most further tiles that there can be         */
     uint64_t units;           /* (tile, head) units that the scratch has room for            */
     float *parts;             /* [units * n_splits][cols][D + 2]                             */
@@ -187,8 +162,6 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
     lfm_pdl_wait();
     const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
 
-    auto sane = [&](int64_t q0, int64_t n_q) { return q0 >= 0 && n_q >= 0 && q0 + n_q <= (int64_t)A.bt.n_tokens; };
-
     for (uint64_t z = blockIdx.x; z < P.tiles; z += P.extra) {
         /* ---- the tile: its sequence and columns ---- */
         int b = (int)z;
@@ -196,59 +169,29 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
         if (z >= A.bt.n_seqs) {
             /* the (z - n_seqs)-th of the tiles behind each sequence's first, in order */
             __syncthreads();
-            if (warp == 0) {
-                uint64_t before = 0;
-                const uint64_t want = z - A.bt.n_seqs;
-                int found = -1;
-                for (uint32_t b0 = 0; b0 < A.bt.n_seqs && found < 0; b0 += 32) {
-                    uint64_t n = 0;
-                    if (b0 + lane < A.bt.n_seqs) {
-                        const int64_t q = A.bt.q_start[b0 + lane], q_n = (int64_t)A.bt.q_start[b0 + lane + 1] - q;
-                        n = q_n > 0 && sane(q, q_n) ? (uint64_t)(q_n * G - 1) / kCols : 0;
-                    }
-                    uint64_t sum = n;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const uint64_t v = __shfl_up_sync(LFM_FULL_MASK, sum, o);
-                        if (lane >= (uint32_t)o) sum += v;
-                    }
-                    const bool here = want >= before + sum - n && want < before + sum;
-                    const uint32_t who = __ballot_sync(LFM_FULL_MASK, here);
-                    if (who) {
-                        found = (int)b0 + __ffs(who) - 1;
-                        if (here) { s_tile[0] = found; s_tile[1] = (int)(want - (before + sum - n)) + 1; }
-                    }
-                    before += __shfl_sync(LFM_FULL_MASK, sum, 31);
-                }
-                if (found < 0 && lane == 0) s_tile[0] = -1;
-            }
+            if (warp == 0) lfm_find_tile(A.bt, G, kCols, 1, 0, P.most, z - A.bt.n_seqs, s_tile);
             __syncthreads();
             b = s_tile[0];
             if (b < 0) return;
             ct = (uint32_t)s_tile[1];
         }
         const int64_t q0 = A.bt.q_start[b], n_q = (int64_t)A.bt.q_start[b + 1] - q0, len = A.bt.kv_len[b];
-        const bool good = sane(q0, n_q) && len >= 0;
+        const bool good = lfm_sane(A.bt, q0, n_q) && len >= 0;
         if (!good && tid == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
         const uint32_t row0 = ct * kCols; /* rows of a sequence: (token, head of the group), below 2^31 */
         const int64_t rows = n_q * G - row0;
-        if (!good || rows <= 0) {
+        if (!good || rows <= 0 || (uint64_t)n_q * G > P.most) {
             if (z < A.bt.n_seqs) return;
             continue;
         }
         const uint32_t last = (uint32_t)(rows < kCols ? rows : kCols) - 1;
-        /* keys [lo, hi) that a row sees; over the tile they grow with the row */
-        auto see = [&](uint32_t r, int64_t &lo, int64_t &hi) {
-            hi = A.causal ? len - n_q + (int64_t)(r / G) + 1 : len;
-            if (hi < 0) hi = 0;
-            lo = A.window && hi > (int64_t)A.window ? hi - A.window : 0;
-        };
+        /* what a row sees grows over the tile */
         int64_t lo0, hi0, lo1, hi1;
-        see(row0, lo0, hi0);
-        see(row0 + last, lo1, hi1);
+        lfm_visible(A, n_q, len, row0, lo0, hi0);
+        lfm_visible(A, n_q, len, row0 + last, lo1, hi1);
         if (tid < kCols) {
             int64_t lo = 0, hi = 0;
-            if (tid <= last) see(row0 + tid, lo, hi);
+            if (tid <= last) lfm_visible(A, n_q, len, row0 + tid, lo, hi);
             s_lo[tid] = lo;
             s_hi[tid] = hi;
         }
@@ -287,18 +230,11 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (on) {
-                        const size_t o = at + 64 * s + 32 * c + 8 * t;
-                        if (A.type == 0) lfm_load<8>(static_cast<const float *>(A.q) + o, v);
-                        else if (A.type == 1) lfm_load<8>(static_cast<const __half *>(A.q) + o, v);
-                        else lfm_load<8>(static_cast<const __nv_bfloat16 *>(A.q) + o, v);
-                    }
+                    if (on) lfm_load_q(A, at + 64 * s + 32 * c + 8 * t, A.scale < 0.0f && !kCap, v);
                     float h[8], sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        float x = A.scale < 0.0f && !kCap ? -v[i] : v[i];
-                        x = x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
-                        h[i] = __half2float(__float2half_rn(x));
+                        h[i] = __half2float(__float2half_rn(v[i]));
                         sum = __fmaf_rn(h[i], (i & 1) ? 72.0f : 1032.0f, sum);
                     }
 #pragma unroll
@@ -314,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
         float o[NT][kS][2][2][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            m[n][0] = m[n][1] = kNone;
+            m[n][0] = m[n][1] = LFM_NO_KEY;
             l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
             for (int s = 0; s < kS; ++s)
@@ -358,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                         for (int c = 0; c < 2; ++c) {
                             const uint32_t u = __byte_perm(x0.x, x0.y, c ? 0x7632 : 0x5410);
                             const uint32_t w = __byte_perm(x1.x, x1.y, c ? 0x7632 : 0x5410);
-                            const uint32_t a0[4] = {nib0(u), nib0(w), nib1(u), nib1(w)};
-                            const uint32_t a1[4] = {nib0(u >> 8), nib0(w >> 8), nib1(u >> 8), nib1(w >> 8)};
+                            const uint32_t a0[4] = {lfm_nib0(u), lfm_nib0(w), lfm_nib1(u), lfm_nib1(w)};
+                            const uint32_t a1[4] = {lfm_nib0(u >> 8), lfm_nib0(w >> 8), lfm_nib1(u >> 8), lfm_nib1(w >> 8)};
                             const float f0 = c ? e0.y : e0.x, f1 = c ? e1.y : e1.x;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
@@ -381,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) z4[n][j] = __fmaf_rn(-2.0f, rcp(1.0f + ex2(z4[n][j] * capz)), 1.0f);
+                        for (int j = 0; j < 4; ++j) z4[n][j] = __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(z4[n][j] * capz)), 1.0f);
                 }
                 if (!whole) {
 #pragma unroll
@@ -407,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                             float x = fmaxf(z4[n][e], z4[n][2 + e]);
 #pragma unroll
                             for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(LFM_FULL_MASK, x, k));
-                            const float nm = fmaxf(m[n][e], x * sc), f = ex2(m[n][e] - nm);
+                            const float nm = fmaxf(m[n][e], x * sc), f = lfm_ex2(m[n][e] - nm);
                             m[n][e] = nm;
                             l[n][e] *= f;
 #pragma unroll
@@ -425,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) z4[n][j] = ex2(__fmaf_rn(z4[n][j], sc, -m[n][j & 1]));
+                    for (int j = 0; j < 4; ++j) z4[n][j] = lfm_ex2(__fmaf_rn(z4[n][j], sc, -m[n][j & 1]));
                     l[n][0] += z4[n][0] + z4[n][2];
                     l[n][1] += z4[n][1] + z4[n][3];
                     pf[n][0] = transpose8(lfm_pack2(z4[n][0], z4[n][1], __half()));
@@ -458,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const uint32_t uu = k ? u >> 8 : u, ww = k ? w >> 8 : w;
-                            const uint32_t a[4] = {hmul2(hsub2(nib0(uu), kOff0), du), hmul2(hsub2(nib1(uu), kOff1), du),
-                                                   hmul2(hsub2(nib0(ww), kOff0), dw), hmul2(hsub2(nib1(ww), kOff1), dw)};
+                            const uint32_t a[4] = {lfm_hmul2(lfm_hsub2(lfm_nib0(uu), LFM_NIB0_OFF), du), lfm_hmul2(lfm_hsub2(lfm_nib1(uu), LFM_NIB1_OFF), du),
+                                                   lfm_hmul2(lfm_hsub2(lfm_nib0(ww), LFM_NIB0_OFF), dw), lfm_hmul2(lfm_hsub2(lfm_nib1(ww), LFM_NIB1_OFF), dw)};
 #pragma unroll
                             for (int n = 0; n < NT; ++n) mma16816(o[n][s][c][k], a, pf[n][0], pf[n][1]);
                         }
@@ -509,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
             for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, s_m[w][col]);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = ex2(s_m[w][col] - mx);
+                const float f = lfm_ex2(s_m[w][col] - mx);
                 const float4 x = *reinterpret_cast<const float4 *>(so + (size_t)(w * kCols + col) * kPitch + d);
                 v[0] = __fmaf_rn(f, x.x, v[0]); v[1] = __fmaf_rn(f, x.y, v[1]);
                 v[2] = __fmaf_rn(f, x.z, v[2]); v[3] = __fmaf_rn(f, x.w, v[3]);
@@ -538,12 +474,12 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                 const float *all = P.parts + unit * P.n_splits * kCols * (D + 2);
                 for (uint32_t i = tid; i < (last + 1) * (D / 4); i += kThreads) {
                     const uint32_t col = i / (D / 4), d = i % (D / 4) * 4;
-                    float mx = kNone, v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.0f;
+                    float mx = LFM_NO_KEY, v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.0f;
                     for (uint32_t k = 0; k < n_act; ++k) mx = fmaxf(mx, __ldcg(all + (size_t)(k * kCols + col) * (D + 2)));
                     for (uint32_t k = 0; k < n_act; ++k) {
                         const float2 *p = reinterpret_cast<const float2 *>(all + (size_t)(k * kCols + col) * (D + 2));
                         const float2 ml = __ldcg(p), x = __ldcg(p + 1 + d / 2), y = __ldcg(p + 2 + d / 2);
-                        const float f = ex2(ml.x - mx);
+                        const float f = lfm_ex2(ml.x - mx);
                         v[0] = __fmaf_rn(f, x.x, v[0]); v[1] = __fmaf_rn(f, x.y, v[1]);
                         v[2] = __fmaf_rn(f, y.x, v[2]); v[3] = __fmaf_rn(f, y.y, v[3]);
                         sum = __fmaf_rn(f, ml.y, sum);
@@ -566,8 +502,11 @@ cudaError_t launch_rows(const AttnArgs &a, const RowsPlan &p, dim3 grid, cudaStr
 
 }  // namespace
 
-cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
-                            cudaStream_t s, bool pdl) {
+/* Rows of a sequence up to which it is this file's: measured, see launch below. */
+constexpr uint64_t kFewRows = 64;
+
+static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, uint64_t few, uint32_t max_kv_len, int sm_count, void *scratch,
+                            bool *used, cudaStream_t s, bool pdl) {
     const uint32_t T = a.bt.n_tokens, B = a.bt.n_seqs, G = a.group, keys = head_dim == 64 ? 64 : 32;
     /* columns of a tile: what an average sequence fills, as far as registers go */
     const uint64_t per = ((uint64_t)T + B - 1) / B * G;
@@ -576,6 +515,7 @@ cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_k
      * of single tokens, and one block in z walks what further tiles there are */
     const uint64_t bound = (uint64_t)T * G / cols;
     RowsPlan p{};
+    p.most = few;
     p.extra = bound == 0 ? 0 : T == B ? 1 : (uint32_t)(bound < 4096 ? bound : 4096);
     p.tiles = B + bound;
     uint64_t span = a.window && a.window < max_kv_len ? (uint64_t)a.window + T + keys : max_kv_len;
@@ -593,6 +533,7 @@ cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_k
     if (n < 1) n = 1;
     p.chunk = (uint32_t)((blocks + n - 1) / n);
     p.n_splits = (uint32_t)((blocks + p.chunk - 1) / p.chunk);
+    *used = p.n_splits > 1;
     p.counts = static_cast<uint32_t *>(scratch);
     p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + LFM_ATTN_COUNTS * sizeof(uint32_t));
     const dim3 grid(B + p.extra, a.kv.hkv, p.n_splits);
@@ -600,4 +541,16 @@ cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_k
         return nt == 1 ? launch_rows<64, 1>(a, p, grid, s, pdl) : nt == 2 ? launch_rows<64, 2>(a, p, grid, s, pdl)
                                                                           : launch_rows<64, 4>(a, p, grid, s, pdl);
     return nt == 1 ? launch_rows<128, 1>(a, p, grid, s, pdl) : launch_rows<128, 2>(a, p, grid, s, pdl);
+}
+
+cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
+                            bool *used, cudaStream_t s, bool pdl) {
+    const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group;
+    *used = false;
+    /* one sequence, or at most as many tokens as make few rows: one kernel takes all.  As many tokens as sequences
+     * are a step of single tokens, whatever the odd sequence holds.  Otherwise each takes its sequences */
+    if (rows <= kFewRows || T == B) return lfm_launch_attn_rows(a, head_dim, ~0ull, max_kv_len, sm_count, scratch, used, s, pdl);
+    if (B == 1) return lfm_launch_attn_tile(a, head_dim, 0, s, pdl);
+    const cudaError_t e = lfm_launch_attn_tile(a, head_dim, kFewRows, s, pdl);
+    return e != cudaSuccess ? e : lfm_launch_attn_rows(a, head_dim, kFewRows, max_kv_len, sm_count, scratch, used, s, pdl);
 }

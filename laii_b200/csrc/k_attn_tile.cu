@@ -1,0 +1,479 @@
+/*
+ * Grouped-query attention over the paged 4-bit cache for many query rows a
+ * sequence (prompts, chunks), on the 5th-generation tensor cores.
+ *
+ * A block takes 256 rows (token, head of the group) of one kv head as two
+ * tiles of M = 128 and walks their keys 128 at a time, once:
+ *   loader    bulk copies of a key block's codes and scales, K and V apart
+ *   4 warps   codes -> fp16 values, a thread a key, into the operand layout of
+ *             the MMA (no swizzle: 8 x 16-byte core matrices).  The layout's
+ *             order of a head's values is that of the codes' words -- values
+ *             4 w + i and 32 + 4 w + i side by side, so a word gives its eight
+ *             with one shift and four pairs of one logic instruction, and the
+ *             two scales of a span are the pair that multiplies them.  q is
+ *             laid out in the same order and the output read back from it
+ *   MMA       one thread: S_h = Q_h K^T (fp32, TMEM), O_h += P_h V with P_h,
+ *             fp16, read from the TMEM columns of S_h; the tiles take turns, so
+ *             one multiplies while the other is in its softmax
+ *   2 x 4 warps  softmax, a thread a row: no exchange between threads.  The
+ *             running reference m only moves when a score passes it by 2^8
+ *             (p <= 256 in fp16); then the thread scales its row of O in TMEM
+ * O in TMEM is scaled by 1 / sum at the end.  Rows that end early in a block
+ * and slots that hold no token are masked in S; values of such slots are zero.
+ */
+#include "attn_device.cuh"
+
+namespace {
+
+constexpr int kM = 128, kRows = 2 * kM, kKeys = 128, kThreads = 512;
+constexpr uint32_t kChunk = kM * 16;  /* bytes between the 8-value chunks of a row */
+
+template <int D>
+struct Cfg {
+    static constexpr int kOp = kKeys * D * 2;               /* an operand tile                      */
+    static constexpr int kRaw = kKeys * (D / 2 + D / 16);   /* its codes and scales                 */
+    static constexpr int kOps = D == 64 ? 6 : 4, kRaws = D == 64 ? 6 : 3;
+    static constexpr int kOffOp = 2 * kOp, kOffRaw = kOffOp + kOps * kOp, kSmem = kOffRaw + kRaws * kRaw;
+    static_assert(kSmem <= 226 * 1024, "shared memory");
+};
+
+constexpr uint32_t kTmemCols = 512, kColS = kKeys, kColO = 2 * kKeys;
+/* kind::f16, A and B fp16, D fp32 (bit 4), M / 16 at bit 24, N / 8 at 17; B transposed (N contiguous) at 16 */
+constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(kKeys >> 3) << 17);
+template <int D>
+constexpr uint32_t kIdescPV = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(D >> 3) << 17) | (1u << 16);
+
+struct Bars {
+    uint64_t raw_full[6], raw_empty[6], op_full[6], op_empty[6], s_full[2], p_full[2], o_full[2];
+    uint32_t tmem;
+    int abort, tile[2];
+};
+
+/* No swizzle, version 1: start, leading and stride byte offsets. */
+__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+        "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+        "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(lfm_smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define R8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+#define W8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define X8(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7])
+/* 32 consecutive 32-bit columns of this thread's TMEM lane. */
+__device__ __forceinline__ void ld32(uint32_t t, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : W8(v, 0), W8(v, 8), W8(v, 16), W8(v, 24)
+        : "r"(t));
+}
+__device__ __forceinline__ void st32(uint32_t t, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        R8(v, 0), R8(v, 8), R8(v, 16), R8(v, 24)
+        : "memory");
+}
+/* Keeps the uses of loaded registers behind the wait. */
+__device__ __forceinline__ void tie32(uint32_t *v) { asm volatile("" : X8(v, 0), X8(v, 8), X8(v, 16), X8(v, 24)::"memory"); }
+
+__device__ __forceinline__ uint64_t pk2(uint32_t x, uint32_t y) { return (uint64_t)x | ((uint64_t)y << 32); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+/* Bounded wait that also gives up once another role has. */
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err) {
+    if (lfm_mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = lfm_globaltimer();
+    while (!lfm_mbar_try_wait_sleep(bar, parity, LFM_WAIT_SLEEP_NS)) {
+        if (*abort) return false;
+        if (lfm_globaltimer() - t0 > LFM_WAIT_LIMIT_NS) {
+            atomicOr(err, LFM_DEVERR_TIMEOUT);
+            *abort = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
+template <int D, bool kCap>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t above) {
+    using C = Cfg<D>;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    __shared__ Bars bars;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.group, kvh = blockIdx.y;
+    volatile int *abort = &bars.abort;
+    if (tid == 0) {
+        for (int i = 0; i < C::kRaws; ++i) {
+            lfm_mbar_init(&bars.raw_full[i], 1);
+            lfm_mbar_init(&bars.raw_empty[i], 4);
+        }
+        for (int i = 0; i < C::kOps; ++i) {
+            lfm_mbar_init(&bars.op_full[i], 4);
+            lfm_mbar_init(&bars.op_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            lfm_mbar_init(&bars.s_full[i], 1);
+            lfm_mbar_init(&bars.p_full[i], 4);
+            lfm_mbar_init(&bars.o_full[i], 1);
+        }
+        bars.abort = 0;
+        lfm_fence_mbar_init();
+    }
+    lfm_pdl_wait();
+    /* the longest walks first: tiles from the last */
+    if (warp == 0) lfm_find_tile(A.bt, G, kRows, 0, above, ~0ull, gridDim.x - 1 - blockIdx.x, bars.tile);
+    __syncthreads();
+    const int b = bars.tile[0];
+    if (b < 0) return;
+    const int64_t q0 = A.bt.q_start[b], n_q = (int64_t)A.bt.q_start[b + 1] - q0, len = A.bt.kv_len[b];
+    if (len < 0) {
+        if (tid == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
+        return;
+    }
+    const uint32_t row0 = (uint32_t)bars.tile[1] * kRows;
+    const uint32_t rows = (uint32_t)min((int64_t)kRows, n_q * (int64_t)G - row0); /* of this block, at least 1 */
+    int64_t lo0, hi0, lo1, hi1;
+    lfm_visible(A, n_q, len, row0, lo0, hi0);
+    lfm_visible(A, n_q, len, row0 + rows - 1, lo1, hi1);
+    const int64_t blk0 = lo0 / kKeys;
+    const uint32_t n = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - blk0) : 0; /* key blocks */
+    auto row_at = [&](uint32_t r, size_t stride) {
+        r += row0;
+        return (size_t)(q0 + r / G) * stride + ((size_t)kvh * G + r % G) * D;
+    };
+    if (n == 0) { /* no key for any row */
+        for (uint32_t i = tid; i < rows * (D / 8); i += kThreads) {
+            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            const size_t at = row_at(i / (D / 8), A.out_stride) + i % (D / 8) * 8;
+            if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + at, z);
+            else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + at, z);
+            else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + at, z);
+        }
+        return;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        fence_before();
+    }
+    /* q: a thread 8 values 4 w .. 4 w + 3 and 32 + 4 w .. of a span, one chunk */
+    for (uint32_t i = tid; i < kRows * (D / 16); i += kThreads) {
+        /* two words a step: values 8 v .. + 7 and 32 + 8 v .. + 7 of the span make chunks 2 v and 2 v + 1 */
+        const uint32_t r = i % kRows, c = i / kRows, s = c >> 2, v = c & 3;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (r < rows) {
+            const size_t at = row_at(r, A.q_stride) + 64 * s + 8 * v;
+            const bool neg = A.scale < 0.0f && !kCap;
+            lfm_load_q(A, at, neg, x);
+            lfm_load_q(A, at + 32, neg, y);
+        }
+        uint8_t *to = sm + (r / kM) * C::kOp + (8 * s + 2 * v) * kChunk + (r % kM) * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<uint4 *>(to + h * kChunk) =
+                make_uint4(lfm_pack2(x[4 * h], y[4 * h], __half()), lfm_pack2(x[4 * h + 1], y[4 * h + 1], __half()),
+                           lfm_pack2(x[4 * h + 2], y[4 * h + 2], __half()), lfm_pack2(x[4 * h + 3], y[4 * h + 3], __half()));
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = bars.tmem, smem = lfm_smem_u32(sm);
+    bool ok = true;
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        const uint32_t h = warp >> 2, r = h * kM + (warp & 3) * 32 + lane;
+        const uint32_t tS = tmem + h * kColS + ((warp & 3) << 21), tO = tmem + kColO + h * D + ((warp & 3) << 21);
+        const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
+        const float capz = kCap ? A.scale * 2.88539008f / A.softcap : 0.0f;
+        int64_t lo = 0, hi = 0;
+        if (r < rows) lfm_visible(A, n_q, len, row0 + r, lo, hi);
+        /* over the tile: every row sees [lo_all, hi_all) */
+        int64_t lo_all = 0, hi_all = 0, unused;
+        if (h * kM < rows) {
+            lfm_visible(A, n_q, len, row0 + h * kM, unused, hi_all);
+            lfm_visible(A, n_q, len, row0 + min(rows, (h + 1) * kM) - 1, lo_all, unused);
+        }
+        const uint64_t sc2 = pk2(__float_as_uint(sc), __float_as_uint(sc));
+        float m = LFM_NO_KEY;
+        uint64_t l2 = 0;
+        for (uint32_t j = 0; j < n; ++j) {
+            ok = __all_sync(LFM_FULL_MASK, wait(&bars.s_full[h], j & 1, abort, A.err));
+            if (!ok) break;
+            fence_after();
+            uint32_t s[kKeys];
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 32) ld32(tS + i, s + i);
+            wait_ld();
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 32) tie32(s + i);
+            if (kCap) {
+#pragma unroll
+                for (int i = 0; i < kKeys; ++i)
+                    s[i] = __float_as_uint(__fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(__uint_as_float(s[i]) * capz)), 1.0f));
+            }
+            const int64_t key0 = (blk0 + j) * kKeys;
+            if (key0 < lo_all || key0 + kKeys > hi_all) {
+                const int to = (int)max((int64_t)0, min((int64_t)kKeys, hi - key0));
+                const int from = (int)max((int64_t)0, min((int64_t)kKeys, lo - key0));
+#pragma unroll
+                for (int i = 0; i < kKeys; ++i)
+                    if (i < from || i >= to) s[i] = 0xFF800000u;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 8) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1])));
+            }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (__any_sync(LFM_FULL_MASK, __fmaf_rn(top, sc, -m) > 8.0f)) {
+                const float nm = fmaxf(m, top * sc), f = lfm_ex2(m - nm);
+                const uint64_t f2 = pk2(__float_as_uint(f), __float_as_uint(f));
+                m = nm;
+                l2 = mul2(l2, f2);
+                if (j) { /* s_full of this block: the products of the one before are in O */
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        ld32(tO + c, o);
+                        wait_ld();
+                        tie32(o);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const uint64_t x = mul2(pk2(o[i], o[i + 1]), f2);
+                            o[i] = (uint32_t)x;
+                            o[i + 1] = (uint32_t)(x >> 32);
+                        }
+                        st32(tO + c, o);
+                    }
+                }
+            }
+            const uint64_t nm2 = pk2(__float_as_uint(-m), __float_as_uint(-m));
+            uint64_t la = 0;
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 2) {
+                const uint64_t x = fma2(pk2(s[i], s[i + 1]), sc2, nm2);
+                const float p0 = lfm_ex2(__uint_as_float((uint32_t)x)), p1 = lfm_ex2(__uint_as_float((uint32_t)(x >> 32)));
+                const uint64_t p = pk2(__float_as_uint(p0), __float_as_uint(p1));
+                if (i & 2) la = add2(la, p);
+                else l2 = add2(l2, p);
+                s[i / 2] = lfm_pack2(p0, p1, __half());
+            }
+            l2 = add2(l2, la);
+            st32(tS, s);
+            st32(tS + 32, s + 32);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) lfm_mbar_arrive(&bars.p_full[h]);
+        }
+        if (ok) ok = __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h], 0, abort, A.err));
+        if (ok) {
+            fence_after();
+            const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const size_t at = r < rows ? row_at(r, A.out_stride) : 0;
+#pragma unroll
+            for (int s = 0; s < D / 64; ++s) {
+                uint32_t o[64];
+                ld32(tO + 64 * s, o);
+                ld32(tO + 64 * s + 32, o + 32);
+                wait_ld();
+                tie32(o);
+                tie32(o + 32);
+                if (r < rows) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) { /* values 0 .. 31 of the span are the even columns */
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[2 * (8 * (c & 3) + i) + (c >> 2)]) * inv;
+                        const size_t to = at + 64 * s + 8 * c;
+                        if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + to, v);
+                        else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + to, v);
+                        else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + to, v);
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const uint32_t sub = min(A.kv.page_tokens, (uint32_t)kKeys), piece = sub * (D / 2 + D / 16);
+        if (warp < 12) {
+            /* codes -> values */
+            const uint32_t key = (warp - 8) * 32 + lane, in = key & (sub - 1);
+            const uint32_t codes = (key / sub) * piece + in * (D / 2), scales = (key / sub) * piece + sub * (D / 2) + in * (D / 16);
+            for (uint32_t u = 0; u < 2 * n; ++u) {
+                const uint32_t rs = u % C::kRaws, os = u % C::kOps;
+                bool w = wait(&bars.raw_full[rs], (u / C::kRaws) & 1, abort, A.err);
+                if (u >= (uint32_t)C::kOps) w = w && wait(&bars.op_empty[os], ((u / C::kOps) & 1) ^ 1, abort, A.err);
+                ok = __all_sync(LFM_FULL_MASK, w);
+                if (!ok) break;
+                const uint8_t *raw = sm + C::kOffRaw + rs * C::kRaw;
+                uint8_t *to = sm + C::kOffOp + os * C::kOp + key * 16;
+                const bool held = (blk0 + (u >> 1)) * kKeys + key < len;
+#pragma unroll
+                for (int s = 0; s < D / 64; ++s) {
+                    const uint4 a = *reinterpret_cast<const uint4 *>(raw + codes + 32 * s);
+                    const uint4 c = *reinterpret_cast<const uint4 *>(raw + codes + 32 * s + 16);
+                    /* a slot that holds no token may hold anything: zero, for V */
+                    const uint32_t d = held ? *reinterpret_cast<const uint32_t *>(raw + scales + 4 * s) : 0u;
+                    const uint32_t x[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t y = x[k] >> 8;
+                        *reinterpret_cast<uint4 *>(to + (8 * s + k) * kChunk) =
+                            make_uint4(lfm_hmul2(lfm_hsub2(lfm_nib0(x[k]), LFM_NIB0_OFF), d),
+                                       lfm_hmul2(lfm_hsub2(lfm_nib1(x[k]), LFM_NIB1_OFF), d),
+                                       lfm_hmul2(lfm_hsub2(lfm_nib0(y), LFM_NIB0_OFF), d),
+                                       lfm_hmul2(lfm_hsub2(lfm_nib1(y), LFM_NIB1_OFF), d));
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    lfm_mbar_arrive(&bars.op_full[os]);
+                    lfm_mbar_arrive(&bars.raw_empty[rs]);
+                }
+            }
+        } else if (warp == 12) {
+            if (lane == 0) {
+                auto full = [&](uint32_t u) { return wait(&bars.op_full[u % C::kOps], (u / C::kOps) & 1, abort, A.err); };
+                auto op = [&](uint32_t u) { return smem + C::kOffOp + (u % C::kOps) * C::kOp; };
+                auto qk = [&](uint32_t h, uint32_t u) {
+                    const uint64_t qd = sdesc(smem + h * C::kOp, kChunk, 128), kd = sdesc(op(u), kChunk, 128);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(tmem + h * kColS, qd + k * (2 * kChunk >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
+                };
+                auto pv = [&](uint32_t h, uint32_t u, bool first) {
+                    const uint64_t vd = sdesc(op(u), 128, kChunk);
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        mma_ts(tmem + kColO + h * D, tmem + h * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
+                };
+                ok = full(0);
+                if (ok) {
+                    fence_after();
+                    qk(0, 0);
+                    commit(&bars.s_full[0]);
+                    qk(1, 0);
+                    commit(&bars.s_full[1]);
+                    commit(&bars.op_empty[0]);
+                }
+                for (uint32_t j = 0; j < n && ok; ++j) {
+                    for (uint32_t h = 0; h < 2 && ok; ++h) {
+                        ok = wait(&bars.p_full[h], j & 1, abort, A.err) && (h || full(2 * j + 1));
+                        if (!ok) break;
+                        fence_after();
+                        pv(h, 2 * j + 1, j == 0);
+                        if (h) commit(&bars.op_empty[(2 * j + 1) % C::kOps]);
+                        if (j + 1 < n) {
+                            if (!h) {
+                                ok = full(2 * j + 2);
+                                if (!ok) break;
+                                fence_after();
+                            }
+                            qk(h, 2 * j + 2);
+                            commit(&bars.s_full[h]);
+                            if (h) commit(&bars.op_empty[(2 * j + 2) % C::kOps]);
+                        } else {
+                            commit(&bars.o_full[h]);
+                        }
+                    }
+                }
+            }
+        } else if (warp == 13) {
+            /* pages: a lane a piece of the block, K then V */
+            for (uint32_t j = 0; j < n; ++j) {
+                const int64_t key = (blk0 + j) * kKeys + (int64_t)lane * sub;
+                const uint8_t *page = nullptr;
+                if (lane * sub < kKeys && key < len) page = lfm_page(A.kv, A.bt, b, key, kvh, A.err);
+                const uint32_t bytes = __popc(__ballot_sync(LFM_FULL_MASK, page != nullptr)) * piece;
+#pragma unroll
+                for (uint32_t k = 0; k < 2; ++k) {
+                    const uint32_t u = 2 * j + k, rs = u % C::kRaws;
+                    ok = ok && (u < (uint32_t)C::kRaws || wait(&bars.raw_empty[rs], ((u / C::kRaws) & 1) ^ 1, abort, A.err));
+                    ok = __all_sync(LFM_FULL_MASK, ok);
+                    if (!ok) break;
+                    if (lane == 0) lfm_mbar_arrive_tx(&bars.raw_full[rs], bytes);
+                    __syncwarp();
+                    if (page)
+                        lfm_bulk_g2s_plain(sm + C::kOffRaw + rs * C::kRaw + lane * piece, page + (k ? A.kv.half : 0), piece,
+                                           &bars.raw_full[rs]);
+                }
+                if (!ok) break;
+            }
+        }
+    }
+    if (!ok) *abort = 1;
+    fence_before();
+    __syncthreads();
+    if (*abort) {
+        /* copies and MMAs already issued end within microseconds: let them land */
+        const uint64_t t0 = lfm_globaltimer();
+        while (lfm_globaltimer() - t0 < 2000000ull) {
+        }
+    }
+    if (warp == 12) {
+        __syncwarp();
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
+}
+
+template <int D>
+cudaError_t launch_tile(const AttnArgs &a, uint64_t above, dim3 grid, cudaStream_t s, bool pdl) {
+    static size_t set[2][16];
+    auto fn = a.softcap > 0.0f ? k_attn_tile<D, true> : k_attn_tile<D, false>;
+    const cudaError_t e = lfm_smem_attr((const void *)fn, Cfg<D>::kSmem, set[a.softcap > 0.0f]);
+    return e != cudaSuccess ? e : lfm_launch_pdl(fn, grid, dim3(kThreads), Cfg<D>::kSmem, s, pdl, a, above);
+}
+
+}  // namespace
+
+cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, cudaStream_t s, bool pdl) {
+    /* a tile for every started kRows rows of a sequence: at most this many */
+    const uint64_t rows = (uint64_t)a.bt.n_tokens * a.group, most = a.bt.n_seqs < a.bt.n_tokens ? a.bt.n_seqs : a.bt.n_tokens;
+    const uint64_t big = rows / (above + 1) < most ? rows / (above + 1) : most; /* sequences of more than `above` rows */
+    const dim3 grid((uint32_t)(rows / kRows + big), a.kv.hkv);
+    if (grid.x == 0) return cudaSuccess;
+    return head_dim == 64 ? launch_tile<64>(a, above, grid, s, pdl) : launch_tile<128>(a, above, grid, s, pdl);
+}

@@ -368,7 +368,8 @@ def _kv(lib, **change):
     from laii_b200 import _native
     c = Case([(2, 20)], 16, 2, 64)
     q = torch.zeros(4, 4, 64, dtype=torch.bfloat16, device="cuda")
-    kv, bt = c.cache._c, c.batch.rows(2)
+    c.batch.rows(2)
+    kv, bt = c.cache._c, c.batch._c
     a = {"n_heads": 4, "scale": 0.1, "causal": 1, "window": 0, "cap": 0.0, "type": 30, "q": q.data_ptr(), "qs": 256,
          "out": q.data_ptr(), "os": 256} | {k: v for k, v in change.items() if not k.startswith(("kv_", "bt_"))}
     for k, v in change.items():
