@@ -148,8 +148,24 @@ __device__ __forceinline__ void lfm_find_tile(const BatchDev &bt, uint32_t G, ui
 /* Codes to fp16: a nibble in an fp16 exponent, bits 0-3 of a half as 1024 + c, bits 4-7 as 64 + c. */
 #define LFM_NIB0_OFF 0x64086408u /* 1032, 1032: the exponent's offset and the code's own 8 */
 #define LFM_NIB1_OFF 0x54805480u /*   72,   72 */
-__device__ __forceinline__ uint32_t lfm_nib0(uint32_t x) { return (x & 0x000F000Fu) | 0x64006400u; }
-__device__ __forceinline__ uint32_t lfm_nib1(uint32_t x) { return (x & 0x00F000F0u) | 0x54005400u; }
+struct LfmNib {
+    uint32_t e0, e1;
+    /* the exponents stay in registers: as two immediates the compiler spends two instructions a pair */
+    __device__ __forceinline__ LfmNib() {
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(e0));
+        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(e1));
+    }
+    __device__ __forceinline__ uint32_t lo(uint32_t x) const {
+        uint32_t r;
+        asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(e0));
+        return r;
+    }
+    __device__ __forceinline__ uint32_t hi(uint32_t x) const {
+        uint32_t r;
+        asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(e1));
+        return r;
+    }
+};
 __device__ __forceinline__ uint32_t lfm_hsub2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

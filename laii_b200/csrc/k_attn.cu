@@ -43,6 +43,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+/* d = A B + c; c in registers of its own, so that a start value is not copied first. */
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -58,10 +65,12 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
     return v;
 }
-/* The D / 32 scales of a key. */
+/* N words. */
 template <int N>
-__device__ __forceinline__ void lds_scales(uint32_t a, uint32_t (&v)[N]) {
-    if constexpr (N == 2) {
+__device__ __forceinline__ void lds(uint32_t a, uint32_t (&v)[N]) {
+    if constexpr (N == 4) {
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
+    } else if constexpr (N == 2) {
         const uint2 u = lds64(a);
         v[0] = u.x; v[1] = u.y;
     } else {
@@ -76,13 +85,16 @@ __device__ __forceinline__ void store4(void *p, uint32_t type, size_t at, const 
 }
 
 struct RowsPlan {
-    uint32_t n_splits, chunk; /* blocks of keys a split takes (the last takes what is left) */
-    uint32_t extra;           /* blocks past n_seqs that walk the further column tiles       */
-    uint64_t most;            /* rows of the longest sequence that is this kernel's          */
-    uint64_t tiles;           /* n_seqs and the most further tiles that there can be         */
-    uint64_t units;           /* (tile, head) units that the scratch has room for            */
-    float *parts;             /* [units * n_splits][cols][D + 2]                             */
-    uint32_t *counts;         /* [units], zero between calls                                 */
+    uint64_t most;    /* rows of the longest sequence that is this kernel's */
+    float *parts;     /* [blocks][2][cols][D + 2]                           */
+    uint32_t *counts; /* [blocks], zero between calls                       */
+};
+
+/* A sequence's share of the work: its tiles of kCols rows, on every kv head, over its blocks of keys. */
+struct Seq {
+    int64_t q0, n_q, len, blk0, blk1;
+    uint64_t tiles, weight;
+    bool sane;
 };
 
 /* A warp's issue and wait state over its blocks first, first + kWarps, ... */
@@ -93,53 +105,47 @@ struct Ring {
     uint32_t kvh, smem, n;   /* n: blocks of this warp */
     int64_t first, end;      /* first block; keys that exist */
     uint64_t *bars;
-    uint32_t id, next;       /* page ids of 8 blocks, four pieces each, a lane a piece */
+    uint32_t id, next;       /* pages of two blocks, 16 lanes each: a lane a part of a page */
 
-    /* Page of piece lane % 4 of block i8 + lane / 4. */
-    __device__ __forceinline__ uint32_t lookup(uint32_t i8) {
-        constexpr int kK = Cfg<D>::kKeys;
-        const uint32_t lane = threadIdx.x & 31, i = i8 + lane / 4, j = lane & 3, P = A.kv.page_tokens;
-        const int64_t key = (first + (int64_t)i * kWarps) * kK + (P < kK ? j * P : 0);
-        if (i >= n || key >= end || (P < kK && j * P >= kK) || (P == kK && j)) return ~0u - 1; /* nothing to copy */
+    /* This lane's page in block i2 + lane / 16: piece lane / 4 % 4 of the block. */
+    __device__ __forceinline__ uint32_t lookup(uint32_t i2) {
+        constexpr uint32_t kK = Cfg<D>::kKeys;
+        const uint32_t lane = threadIdx.x & 31, i = i2 + lane / 16, j = (lane >> 2) & 3, P = A.kv.page_tokens;
+        const int64_t key = (first + (int64_t)i * kWarps) * kK + j * P;
+        if (i >= n || key >= end || (j && j * P >= kK)) return ~0u; /* nothing to copy */
         const int64_t at = key >> A.kv.page_shift;
         uint32_t page = ~0u;
         if (at < (int64_t)A.bt.table_stride) page = (uint32_t)A.bt.page_table[(size_t)b * A.bt.table_stride + (size_t)at];
-        if (page >= A.kv.n_pages) {
-            atomicOr(A.err, LFM_DEVERR_PAGE);
-            return ~0u;
-        }
+        if (page >= A.kv.n_pages) atomicOr(A.err, LFM_DEVERR_PAGE);
         return page;
     }
 
-    /* Copies of block i into its stage: pages of up to a block whole, a longer page's four parts. */
+    /* Copies of block i into its stage, [K codes][K scales][V codes][V scales] of its keys whatever the page's
+     * size: a lane a part (lane % 4) of a page. */
     __device__ __forceinline__ void issue(uint32_t i) {
         constexpr uint32_t kK = Cfg<D>::kKeys;
-        if ((i & 7) == 0 && i) id = next;
-        const uint32_t lane = threadIdx.x & 31, j = lane & 3, P = A.kv.page_tokens;
-        if (lane / 4 == (i & 7)) {
-            uint64_t *bar = bars + i % kStages;
-            if (id < A.kv.n_pages) {
-                const uint8_t *page = A.kv.pages + (size_t)id * A.kv.page_bytes + (size_t)kvh * A.kv.head_bytes;
-                uint32_t to = smem + i % kStages * Cfg<D>::kBytes, bytes;
-                if (P <= kK) {
-                    bytes = P * (D + D / 8);
-                    to += j * bytes;
-                } else {
-                    const uint32_t in = (uint32_t)((first + (int64_t)i * kWarps) * kK) & (P - 1);
-                    bytes = (j & 1) ? kK * (D / 16) : kK * (D / 2);
-                    page += (j & 2 ? A.kv.half : 0) + ((j & 1) ? A.kv.codes + in * (D / 16) : in * (D / 2));
-                    to += (j & 2 ? kK * (D / 2 + D / 16) : 0) + ((j & 1) ? kK * (D / 2) : 0);
-                }
-                lfm_mbar_arrive_tx(bar, bytes);
-                asm volatile(
-                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
-                    "l"(page), "r"(bytes), "r"(lfm_smem_u32(bar))
-                    : "memory");
-            } else {
-                lfm_mbar_arrive(bar);
-            }
+        if ((i & 1) == 0) {
+            id = next;
+            next = lookup(i + 2);
         }
-        if ((i & 7) == 4) next = lookup((i & ~7u) + 8);
+        const uint32_t lane = threadIdx.x & 31, part = lane & 3, j = (lane >> 2) & 3, P = A.kv.page_tokens;
+        const uint32_t keys = P < kK ? P : kK;
+        const bool on = (lane >> 4) == (i & 1) && id < A.kv.n_pages;
+        const uint32_t bytes = on ? keys * ((part & 1) ? D / 16 : D / 2) : 0;
+        const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, bytes);
+        uint64_t *bar = bars + i % kStages;
+        if (lane == 0) lfm_mbar_arrive_tx(bar, all);
+        __syncwarp();
+        if (on) {
+            const uint32_t in = P > kK ? (uint32_t)((first + (int64_t)i * kWarps) * kK) & (P - 1) : 0;
+            const uint8_t *from = A.kv.pages + (size_t)id * A.kv.page_bytes + (size_t)kvh * A.kv.head_bytes +
+                                  (part & 2 ? A.kv.half : 0) + ((part & 1) ? A.kv.codes + in * (D / 16) : in * (D / 2));
+            const uint32_t to = smem + i % kStages * Cfg<D>::kBytes + (part & 2 ? Cfg<D>::kBytes / 2 : 0) +
+                                ((part & 1) ? kK * (D / 2) + j * P * (D / 16) : j * P * (D / 2));
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                         "l"(from), "r"(bytes), "r"(lfm_smem_u32(bar))
+                         : "memory");
+        }
     }
 };
 
@@ -152,38 +158,115 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
     __shared__ uint64_t s_bar[kWarps][kStages];
     __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
     __shared__ int64_t s_hi[kCols], s_lo[kCols];
-    __shared__ int s_tile[2], s_last;
+    __shared__ uint64_t s_sum[kWarps], s_first;
+    __shared__ int s_seq, s_last;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t kvh = blockIdx.y, split = blockIdx.z, G = A.group;
-    if (lane < kStages) lfm_mbar_init(&s_bar[warp][lane], 4);
+    const uint32_t G = A.group;
+    if (lane < kStages) lfm_mbar_init(&s_bar[warp][lane], 1);
     lfm_fence_mbar_init();
     __syncwarp();
     uint32_t phases = 0; /* parity of each stage's next wait */
     lfm_pdl_wait();
+    lfm_pdl_launch_dependents();
     const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
 
-    for (uint64_t z = blockIdx.x; z < P.tiles; z += P.extra) {
-        /* ---- the tile: its sequence and columns ---- */
-        int b = (int)z;
-        uint32_t ct = 0;
-        if (z >= A.bt.n_seqs) {
-            /* the (z - n_seqs)-th of the tiles behind each sequence's first, in order */
-            __syncthreads();
-            if (warp == 0) lfm_find_tile(A.bt, G, kCols, 1, 0, P.most, z - A.bt.n_seqs, s_tile);
-            __syncthreads();
-            b = s_tile[0];
-            if (b < 0) return;
-            ct = (uint32_t)s_tile[1];
+    /* ---- this block's share: all (tile, head) units' key blocks in a row, cut into equal parts ---- */
+    auto sequence = [&](uint32_t b) {
+        Seq q{};
+        q.q0 = A.bt.q_start[b];
+        q.n_q = (int64_t)A.bt.q_start[b + 1] - q.q0;
+        q.len = A.bt.kv_len[b];
+        q.sane = lfm_sane(A.bt, q.q0, q.n_q) && q.len >= 0;
+        const uint64_t rows = q.sane ? (uint64_t)q.n_q * G : 0;
+        if (rows == 0 || rows > P.most) return q;
+        int64_t lo, hi, unused;
+        lfm_visible(A, q.n_q, q.len, 0, lo, unused);
+        lfm_visible(A, q.n_q, q.len, (uint32_t)rows - 1, unused, hi);
+        q.blk0 = lo / C::kKeys;
+        q.blk1 = max(q.blk0 + 1, (hi + C::kKeys - 1) / C::kKeys); /* one where there is no key: rows of zeros */
+        q.tiles = (rows + kCols - 1) / kCols;
+        q.weight = q.tiles * A.kv.hkv * (uint64_t)(q.blk1 - q.blk0);
+        return q;
+    };
+    auto warp_scan = [&](uint64_t v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t u = __shfl_up_sync(LFM_FULL_MASK, v, o);
+            if (lane >= (uint32_t)o) v += u;
         }
-        const int64_t q0 = A.bt.q_start[b], n_q = (int64_t)A.bt.q_start[b + 1] - q0, len = A.bt.kv_len[b];
-        const bool good = lfm_sane(A.bt, q0, n_q) && len >= 0;
-        if (!good && tid == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
+        return v;
+    };
+    uint64_t w = 0; /* this thread's sequence of the last 256 looked at */
+    {
+        uint64_t sum = 0;
+        for (uint32_t b0 = 0; b0 < A.bt.n_seqs; b0 += kThreads) {
+            w = 0;
+            if (b0 + tid < A.bt.n_seqs) {
+                const Seq q = sequence(b0 + tid);
+                if (!q.sane && blockIdx.x == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
+                w = q.weight;
+            }
+            sum += w;
+        }
+        sum = warp_scan(sum);
+        if (lane == 31) s_sum[warp] = sum;
+    }
+    __syncthreads();
+    uint64_t total = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) total += s_sum[i];
+    /* blocks at work: a block of keys for each warp at least */
+    const uint64_t n_cta = min((uint64_t)gridDim.x, (total + kWarps - 1) / kWarps);
+    if (blockIdx.x >= n_cta) return;
+    uint64_t x = total * blockIdx.x / n_cta;
+    const uint64_t x1 = total * (blockIdx.x + 1) / n_cta;
+    /* the part that holds place u */
+    auto owner = [&](uint64_t u) { return (uint32_t)(((u + 1) * n_cta + total - 1) / total - 1); };
+    /* the whole block: the sequence that holds place u, and its first place */
+    auto locate = [&](uint64_t u) {
+        uint64_t before = 0;
+        for (uint32_t b0 = 0; b0 < A.bt.n_seqs; b0 += kThreads) {
+            if (A.bt.n_seqs > kThreads) w = b0 + tid < A.bt.n_seqs ? sequence(b0 + tid).weight : 0;
+            uint64_t sum = warp_scan(w);
+            __syncthreads();
+            if (lane == 31) s_sum[warp] = sum;
+            __syncthreads();
+            sum += before;
+            for (uint32_t i = 0; i < kWarps; ++i) {
+                if (i < warp) sum += s_sum[i];
+                before += s_sum[i];
+            }
+            if (u >= sum - w && u < sum) {
+                s_seq = (int)(b0 + tid);
+                s_first = sum - w;
+            }
+            if (u < before) break;
+        }
+        __syncthreads();
+    };
+    locate(x);
+    uint32_t b = (uint32_t)s_seq;
+    uint64_t first = s_first; /* place of the sequence's first unit */
+    Seq seq = sequence(b);
+
+    while (x < x1) {
+        if (x >= first + seq.weight) { /* the next sequence that has work */
+            first += seq.weight;
+            ++b;
+            seq = sequence(b);
+            if (seq.weight == 0) {
+                locate(x);
+                b = (uint32_t)s_seq;
+                seq = sequence(b);
+            }
+        }
+        const int64_t q0 = seq.q0, n_q = seq.n_q, len = seq.len;
+        const uint64_t n_blk = (uint64_t)(seq.blk1 - seq.blk0), unit = (x - first) / n_blk, u0 = first + unit * n_blk;
+        const uint32_t kvh = (uint32_t)(unit % A.kv.hkv), ct = (uint32_t)(unit / A.kv.hkv);
+        const uint64_t seg = min(x1, u0 + n_blk) - x; /* key blocks of this unit that are ours */
+        const uint32_t own0 = owner(u0), own1 = owner(u0 + n_blk - 1);
         const uint32_t row0 = ct * kCols; /* rows of a sequence: (token, head of the group), below 2^31 */
         const int64_t rows = n_q * G - row0;
-        if (!good || rows <= 0 || (uint64_t)n_q * G > P.most) {
-            if (z < A.bt.n_seqs) return;
-            continue;
-        }
         const uint32_t last = (uint32_t)(rows < kCols ? rows : kCols) - 1;
         /* what a row sees grows over the tile */
         int64_t lo0, hi0, lo1, hi1;
@@ -195,31 +278,21 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
             s_lo[tid] = lo;
             s_hi[tid] = hi;
         }
-        const int64_t blk0 = lo0 / C::kKeys, blk1 = (hi1 + C::kKeys - 1) / C::kKeys;
-        const int64_t n_blk = blk1 - blk0;
-        /* splits that have blocks; a tile without any is split 0's */
-        const uint64_t unit = z * gridDim.y + kvh;
-        const uint32_t n_act = n_blk <= 0 || unit >= P.units ? 1u
-                             : (uint32_t)min((int64_t)P.n_splits, (n_blk + P.chunk - 1) / P.chunk);
-        if (split >= n_act) {
-            if (z < A.bt.n_seqs) return;
-            continue;
-        }
-        const int64_t from = blk0 + (int64_t)split * P.chunk;
-        const int64_t to = split + 1 == n_act ? blk1 : from + P.chunk;
+        const int64_t at0 = seq.blk0 + (int64_t)(x - u0), at1 = at0 + (int64_t)seg;
+        const int64_t from = max(at0, lo0 / C::kKeys), to = min(at1, (hi1 + C::kKeys - 1) / C::kKeys);
         const int64_t mine = to - from - warp;
-        Ring<D> rg{A, b, kvh, lfm_smem_u32(ring) + warp * kStages * C::kBytes,
+        Ring<D> rg{A, (int)b, kvh, lfm_smem_u32(ring) + warp * kStages * C::kBytes,
                    mine > 0 ? (uint32_t)((mine + kWarps - 1) / kWarps) : 0u, from + warp, len, s_bar[warp], 0, 0};
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads(); /* s_lo, s_hi; the ring is free of an earlier tile's join, for the copies too */
-        rg.id = rg.lookup(0);
+        __syncthreads(); /* s_lo, s_hi; the ring is free of an earlier unit's join, for the copies too */
+        rg.next = rg.lookup(0);
 #pragma unroll
         for (uint32_t i = 0; i < kStages; ++i)
             if (i < rg.n) rg.issue(i);
 
         /* ---- Q as B fragments: column g, values 64 s + 32 c + 8 t .. of the head ---- */
         uint32_t qf[NT][kS][2][4];
-        float corr[NT][kS][2][2];
+        float corr[NT][kS][2][4]; /* start values of the scores: minus the codes' offsets times q */
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const uint32_t r = row0 + n * 8 + g;
@@ -241,8 +314,11 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                     for (int i = 0; i < 4; ++i) qf[n][s][c][i] = lfm_pack2(h[i], h[4 + i], __half());
                     sum += __shfl_xor_sync(LFM_FULL_MASK, sum, 1);
                     sum += __shfl_xor_sync(LFM_FULL_MASK, sum, 2);
-                    corr[n][s][c][0] = -__shfl_sync(LFM_FULL_MASK, sum, 8 * t);
-                    corr[n][s][c][1] = -__shfl_sync(LFM_FULL_MASK, sum, 8 * t + 4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        corr[n][s][c][i] = -__shfl_sync(LFM_FULL_MASK, sum, 8 * t + 4 * (i & 1));
+                        asm volatile("" : "+f"(corr[n][s][c][i])); /* four registers, not two */
+                    }
                 }
         }
 
@@ -259,10 +335,16 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
 #pragma unroll
                     for (int i = 0; i < 2; ++i) o[n][s][c][i][0] = o[n][s][c][i][1] = o[n][s][c][i][2] = o[n][s][c][i][3] = 0.0f;
         }
-        const uint32_t sub = min(A.kv.page_tokens, (uint32_t)C::kKeys); /* keys of a contiguous piece */
         const uint32_t rk = g ^ (g >> 2);                     /* key of A row g (rows 8.. : + 8)            */
         const uint32_t ve = 2 * t ^ (t >> 1), vo = ve ^ 1;    /* keys of A columns 2 t and 2 t + 1 for V    */
+        const uint32_t sel0 = t < 2 ? 0x5410 : 0x1054, sel1 = t < 2 ? 0x7632 : 0x3276; /* scales of ve, vo  */
+        constexpr uint32_t kKs = C::kKeys * (D / 2), kV = C::kBytes / 2;
+        const uint32_t atk = rk * (D / 2) + 8 * t, atks = kKs + rk * (D / 16);
+        const uint32_t atve = kV + ve * (D / 2) + 4 * g, atvo = kV + vo * (D / 2) + 4 * g;
+        const uint32_t atvs = kV + kKs + (ve & ~1u) * (D / 16);
         const float capz = kCap ? A.scale * 2.88539008f / A.softcap : 0.0f;
+        constexpr int kPair = NT == 1 ? 2 : 1; /* steps of 16 keys whose scores are looked at together */
+        const LfmNib nib;
         bool ok = true;
         for (uint32_t i = 0; i < rg.n; ++i) {
             const uint32_t st = i % kStages;
@@ -272,42 +354,40 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
             const uint32_t buf = rg.smem + st * C::kBytes;
             const int64_t key0 = (rg.first + (int64_t)i * kWarps) * C::kKeys;
             const bool whole = key0 >= lo1 && key0 + C::kKeys <= hi0; /* every row sees every key */
-            const bool tail = key0 + C::kKeys > len;                  /* slots that hold no token */
-#pragma unroll 1
-            for (uint32_t s16 = 0; s16 < C::kKeys; s16 += 16) {
-                if (tail && key0 + s16 >= len) break;
-                const uint32_t in = s16 & (sub - 1), base = buf + (s16 - in) * (D + D / 8);
-                const uint32_t kc = base + in * (D / 2), ks = base + sub * (D / 2) + in * (D / 16);
-                const uint32_t vc = kc + sub * (D / 2 + D / 16), vs = ks + sub * (D / 2 + D / 16);
+            const int held = (int)min((int64_t)C::kKeys, len - key0); /* slots that hold a token */
+#pragma unroll
+            for (int s16 = 0; s16 < C::kKeys; s16 += 16 * kPair) {
                 /* S^T: rows rk and rk + 8, columns 2 t and 2 t + 1 */
-                float z4[NT][4];
-                {
+                float z4[kPair][NT][4];
+#pragma unroll
+                for (int q = 0; q < kPair; ++q) {
+                    const uint32_t kc = buf + atk + (s16 + 16 * q) * (D / 2), ks = buf + atks + (s16 + 16 * q) * (D / 16);
                     uint32_t d0[kS], d1[kS];
-                    lds_scales<kS>(ks + rk * (D / 16), d0);
-                    lds_scales<kS>(ks + (rk + 8) * (D / 16), d1);
+                    lds(ks, d0);
+                    lds(ks + 8 * (D / 16), d1);
 #pragma unroll
                     for (int s = 0; s < kS; ++s) {
-                        const uint2 x0 = lds64(kc + rk * (D / 2) + 32 * s + 8 * t);
-                        const uint2 x1 = lds64(kc + (rk + 8) * (D / 2) + 32 * s + 8 * t);
+                        const uint2 x0 = lds64(kc + 32 * s), x1 = lds64(kc + 8 * (D / 2) + 32 * s);
                         const float2 e0 = half2_of(d0[s]), e1 = half2_of(d1[s]);
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
                             const uint32_t u = __byte_perm(x0.x, x0.y, c ? 0x7632 : 0x5410);
                             const uint32_t w = __byte_perm(x1.x, x1.y, c ? 0x7632 : 0x5410);
-                            const uint32_t a0[4] = {lfm_nib0(u), lfm_nib0(w), lfm_nib1(u), lfm_nib1(w)};
-                            const uint32_t a1[4] = {lfm_nib0(u >> 8), lfm_nib0(w >> 8), lfm_nib1(u >> 8), lfm_nib1(w >> 8)};
+                            const uint32_t a0[4] = {nib.lo(u), nib.lo(w), nib.hi(u), nib.hi(w)};
+                            const uint32_t a1[4] = {nib.lo(u >> 8), nib.lo(w >> 8), nib.hi(u >> 8), nib.hi(w >> 8)};
                             const float f0 = c ? e0.y : e0.x, f1 = c ? e1.y : e1.x;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                float acc[4] = {corr[n][s][c][0], corr[n][s][c][1], corr[n][s][c][0], corr[n][s][c][1]};
-                                mma16816(acc, a0, qf[n][s][c][0], qf[n][s][c][1]);
+                                float acc[4];
+                                float(&z)[4] = z4[q][n];
+                                mma16816(acc, a0, qf[n][s][c][0], qf[n][s][c][1], corr[n][s][c]);
                                 mma16816(acc, a1, qf[n][s][c][2], qf[n][s][c][3]);
                                 if (s == 0 && c == 0) {
-                                    z4[n][0] = acc[0] * f0; z4[n][1] = acc[1] * f0;
-                                    z4[n][2] = acc[2] * f1; z4[n][3] = acc[3] * f1;
+                                    z[0] = acc[0] * f0; z[1] = acc[1] * f0;
+                                    z[2] = acc[2] * f1; z[3] = acc[3] * f1;
                                 } else {
-                                    z4[n][0] = __fmaf_rn(acc[0], f0, z4[n][0]); z4[n][1] = __fmaf_rn(acc[1], f0, z4[n][1]);
-                                    z4[n][2] = __fmaf_rn(acc[2], f1, z4[n][2]); z4[n][3] = __fmaf_rn(acc[3], f1, z4[n][3]);
+                                    z[0] = __fmaf_rn(acc[0], f0, z[0]); z[1] = __fmaf_rn(acc[1], f0, z[1]);
+                                    z[2] = __fmaf_rn(acc[2], f1, z[2]); z[3] = __fmaf_rn(acc[3], f1, z[3]);
                                 }
                             }
                         }
@@ -315,32 +395,43 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                 }
                 if (kCap) { /* tanh(x) = 1 - 2 / (1 + e^2x) */
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int q = 0; q < kPair; ++q)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) z4[n][j] = __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(z4[n][j] * capz)), 1.0f);
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                z4[q][n][j] = __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(z4[q][n][j] * capz)), 1.0f);
                 }
                 if (!whole) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int64_t key = key0 + s16 + rk + (j >= 2 ? 8 : 0);
-                            const uint32_t col = n * 8 + 2 * t + (j & 1);
-                            if (key < s_lo[col] || key >= s_hi[col]) z4[n][j] = -INFINITY;
+                        for (int e = 0; e < 2; ++e) {
+                            const int64_t lo = s_lo[n * 8 + 2 * t + e] - key0, hi = s_hi[n * 8 + 2 * t + e] - key0;
+#pragma unroll
+                            for (int k = 0; k < 2 * kPair; ++k) {
+                                const int64_t key = s16 + 8 * k + (int)rk;
+                                if (key < lo || key >= hi) z4[k >> 1][n][2 * (k & 1) + e] = -INFINITY;
+                            }
                         }
                 }
+                float top[NT][2];
                 bool grow = false;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        grow |= __fmaf_rn(fmaxf(z4[n][e], z4[n][2 + e]), sc, -m[n][e]) > 8.0f;
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(z4[0][n][e], z4[0][n][2 + e]);
+                        if (kPair == 2) x = fmaxf(x, fmaxf(z4[kPair - 1][n][e], z4[kPair - 1][n][2 + e]));
+                        top[n][e] = x;
+                        grow |= __fmaf_rn(x, sc, -m[n][e]) > 8.0f;
+                    }
                 if (__any_sync(LFM_FULL_MASK, grow)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float x = fmaxf(z4[n][e], z4[n][2 + e]);
+                            float x = top[n][e];
 #pragma unroll
                             for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(LFM_FULL_MASK, x, k));
                             const float nm = fmaxf(m[n][e], x * sc), f = lfm_ex2(m[n][e] - nm);
@@ -357,47 +448,51 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                                     }
                         }
                 }
-                uint32_t pf[NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                for (int q = 0; q < kPair; ++q) {
+                    uint32_t pf[NT][2];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) z4[n][j] = lfm_ex2(__fmaf_rn(z4[n][j], sc, -m[n][j & 1]));
-                    l[n][0] += z4[n][0] + z4[n][2];
-                    l[n][1] += z4[n][1] + z4[n][3];
-                    pf[n][0] = transpose8(lfm_pack2(z4[n][0], z4[n][1], __half()));
-                    pf[n][1] = transpose8(lfm_pack2(z4[n][2], z4[n][3], __half()));
-                }
-                /* O^T: rows are values 64 s + 32 c + 4 g + i of the head */
-                uint32_t dv[4][kS];
-                lds_scales<kS>(vs + ve * (D / 16), dv[0]);
-                lds_scales<kS>(vs + vo * (D / 16), dv[1]);
-                lds_scales<kS>(vs + (ve + 8) * (D / 16), dv[2]);
-                lds_scales<kS>(vs + (vo + 8) * (D / 16), dv[3]);
-                if (tail) { /* what no token holds may be anything */
+                    for (int n = 0; n < NT; ++n) {
+                        float(&z)[4] = z4[q][n];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (key0 + s16 + (k & 1 ? vo : ve) + (k & 2 ? 8 : 0) >= len) {
+                        for (int j = 0; j < 4; ++j) z[j] = lfm_ex2(__fmaf_rn(z[j], sc, -m[n][j & 1]));
+                        l[n][0] += z[0] + z[2];
+                        l[n][1] += z[1] + z[3];
+                        pf[n][0] = transpose8(lfm_pack2(z[0], z[1], __half()));
+                        pf[n][1] = transpose8(lfm_pack2(z[2], z[3], __half()));
+                    }
+                    /* O^T: rows are values 64 s + 32 c + 4 g + i of the head */
+                    const int k16 = s16 + 16 * q;
+                    uint32_t dv[2][2 * kS]; /* scales of a pair of keys, and of the pair eight further */
+                    lds(buf + atvs + k16 * (D / 16), dv[0]);
+                    lds(buf + atvs + (k16 + 8) * (D / 16), dv[1]);
+                    if (held < C::kKeys) { /* what no token holds may be anything */
 #pragma unroll
-                            for (int s = 0; s < kS; ++s) dv[k][s] = 0;
-                        }
-                }
+                        for (int k = 0; k < 4; ++k)
+                            if (k16 + (int)(ve & ~1u) + (k & 1) + (k & 2 ? 8 : 0) >= held) {
 #pragma unroll
-                for (int s = 0; s < kS; ++s) {
-                    const uint32_t at = vc + 32 * s + 4 * g;
-                    const uint32_t x0 = lds32(at + ve * (D / 2)), x1 = lds32(at + vo * (D / 2));
-                    const uint32_t x2 = lds32(at + (ve + 8) * (D / 2)), x3 = lds32(at + (vo + 8) * (D / 2));
+                                for (int s = 0; s < kS; ++s) dv[k >> 1][(k & 1) * kS + s] = 0;
+                            }
+                    }
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint32_t sel = c ? 0x7632 : 0x5410;
-                        const uint32_t u = __byte_perm(x0, x1, sel), w = __byte_perm(x2, x3, sel);
-                        const uint32_t du = __byte_perm(dv[0][s], dv[1][s], sel), dw = __byte_perm(dv[2][s], dv[3][s], sel);
+                    for (int s = 0; s < kS; ++s) {
+                        const uint32_t e = buf + atve + k16 * (D / 2) + 32 * s, o1 = buf + atvo + k16 * (D / 2) + 32 * s;
+                        const uint32_t x0 = lds32(e), x1 = lds32(o1), x2 = lds32(e + 8 * (D / 2)), x3 = lds32(o1 + 8 * (D / 2));
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const uint32_t uu = k ? u >> 8 : u, ww = k ? w >> 8 : w;
-                            const uint32_t a[4] = {lfm_hmul2(lfm_hsub2(lfm_nib0(uu), LFM_NIB0_OFF), du), lfm_hmul2(lfm_hsub2(lfm_nib1(uu), LFM_NIB1_OFF), du),
-                                                   lfm_hmul2(lfm_hsub2(lfm_nib0(ww), LFM_NIB0_OFF), dw), lfm_hmul2(lfm_hsub2(lfm_nib1(ww), LFM_NIB1_OFF), dw)};
+                        for (int c = 0; c < 2; ++c) {
+                            const uint32_t u = __byte_perm(x0, x1, c ? 0x7632 : 0x5410), w = __byte_perm(x2, x3, c ? 0x7632 : 0x5410);
+                            const uint32_t du = __byte_perm(dv[0][s], dv[0][kS + s], c ? sel1 : sel0);
+                            const uint32_t dw = __byte_perm(dv[1][s], dv[1][kS + s], c ? sel1 : sel0);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma16816(o[n][s][c][k], a, pf[n][0], pf[n][1]);
+                            for (int k = 0; k < 2; ++k) {
+                                const uint32_t uu = k ? u >> 8 : u, ww = k ? w >> 8 : w;
+                                const uint32_t a[4] = {lfm_hmul2(lfm_hsub2(nib.lo(uu), LFM_NIB0_OFF), du),
+                                                       lfm_hmul2(lfm_hsub2(nib.hi(uu), LFM_NIB1_OFF), du),
+                                                       lfm_hmul2(lfm_hsub2(nib.lo(ww), LFM_NIB0_OFF), dw),
+                                                       lfm_hmul2(lfm_hsub2(nib.hi(ww), LFM_NIB1_OFF), dw)};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma16816(o[n][s][c][k], a, pf[n][0], pf[n][1]);
+                            }
                         }
                     }
                 }
@@ -430,7 +525,9 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                             make_float4(o[n][s][c][0][e], o[n][s][c][0][2 + e], o[n][s][c][1][e], o[n][s][c][1][2 + e]);
             }
         __syncthreads();
-        float *part = n_act > 1 ? P.parts + (unit * P.n_splits + split) * kCols * (D + 2) : nullptr;
+        const uint32_t n_parts = own1 - own0 + 1;
+        auto part_of = [&](uint32_t c) { return P.parts + ((size_t)c * 2 + (c == own0)) * kCols * (D + 2); };
+        float *part = n_parts > 1 ? part_of(blockIdx.x) : nullptr;
         auto write = [&](uint32_t col, uint32_t d, float (&v)[4], float sum) {
             const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
@@ -461,34 +558,33 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
             }
         }
         if (part) {
-            /* the last split to arrive joins them all, in their order */
+            /* the last part to arrive joins them all, in their order */
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                s_last = atomicAdd(P.counts + unit, 1u) + 1 == n_act;
-                if (s_last) P.counts[unit] = 0;
+                s_last = atomicAdd(P.counts + own0, 1u) + 1 == n_parts;
+                if (s_last) P.counts[own0] = 0;
             }
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                const float *all = P.parts + unit * P.n_splits * kCols * (D + 2);
                 for (uint32_t i = tid; i < (last + 1) * (D / 4); i += kThreads) {
                     const uint32_t col = i / (D / 4), d = i % (D / 4) * 4;
                     float mx = LFM_NO_KEY, v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.0f;
-                    for (uint32_t k = 0; k < n_act; ++k) mx = fmaxf(mx, __ldcg(all + (size_t)(k * kCols + col) * (D + 2)));
-                    for (uint32_t k = 0; k < n_act; ++k) {
-                        const float2 *p = reinterpret_cast<const float2 *>(all + (size_t)(k * kCols + col) * (D + 2));
-                        const float2 ml = __ldcg(p), x = __ldcg(p + 1 + d / 2), y = __ldcg(p + 2 + d / 2);
+                    for (uint32_t c = own0; c <= own1; ++c) mx = fmaxf(mx, __ldcg(part_of(c) + (size_t)col * (D + 2)));
+                    for (uint32_t c = own0; c <= own1; ++c) {
+                        const float2 *p = reinterpret_cast<const float2 *>(part_of(c) + (size_t)col * (D + 2));
+                        const float2 ml = __ldcg(p), x0 = __ldcg(p + 1 + d / 2), y0 = __ldcg(p + 2 + d / 2);
                         const float f = lfm_ex2(ml.x - mx);
-                        v[0] = __fmaf_rn(f, x.x, v[0]); v[1] = __fmaf_rn(f, x.y, v[1]);
-                        v[2] = __fmaf_rn(f, y.x, v[2]); v[3] = __fmaf_rn(f, y.y, v[3]);
+                        v[0] = __fmaf_rn(f, x0.x, v[0]); v[1] = __fmaf_rn(f, x0.y, v[1]);
+                        v[2] = __fmaf_rn(f, y0.x, v[2]); v[3] = __fmaf_rn(f, y0.y, v[3]);
                         sum = __fmaf_rn(f, ml.y, sum);
                     }
                     write(col, d, v, sum);
                 }
             }
         }
-        if (z < A.bt.n_seqs) return;
+        x += seg;
     }
 }
 
@@ -505,52 +601,37 @@ cudaError_t launch_rows(const AttnArgs &a, const RowsPlan &p, dim3 grid, cudaStr
 /* Rows of a sequence up to which it is this file's: measured, see launch below. */
 constexpr uint64_t kFewRows = 64;
 
-static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, uint64_t few, uint32_t max_kv_len, int sm_count, void *scratch,
-                            bool *used, cudaStream_t s, bool pdl) {
-    const uint32_t T = a.bt.n_tokens, B = a.bt.n_seqs, G = a.group, keys = head_dim == 64 ? 64 : 32;
+static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, uint64_t few, uint32_t max_kv_len,
+                                        int sm_count, void *scratch, cudaStream_t s, bool pdl) {
+    const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, G = a.group, keys = head_dim == 64 ? 64 : 32;
     /* columns of a tile: what an average sequence fills, as far as registers go */
-    const uint64_t per = ((uint64_t)T + B - 1) / B * G;
-    const uint32_t nt = per <= 8 ? 1 : per <= 16 || head_dim == 128 ? 2 : 4, cols = 8 * nt;
-    /* tiles beyond each sequence's first: at most T G / cols.  As many tokens as sequences are taken for a step
-     * of single tokens, and one block in z walks what further tiles there are */
-    const uint64_t bound = (uint64_t)T * G / cols;
-    RowsPlan p{};
-    p.most = few;
-    p.extra = bound == 0 ? 0 : T == B ? 1 : (uint32_t)(bound < 4096 ? bound : 4096);
-    p.tiles = B + bound;
-    uint64_t span = a.window && a.window < max_kv_len ? (uint64_t)a.window + T + keys : max_kv_len;
-    if (span > max_kv_len) span = max_kv_len;
-    const uint64_t blocks = span ? (span + keys - 1) / keys : 1;
-    /* splits: enough blocks to fill the GPU a few times over where there are few units, none of them under a
-     * block of keys a warp */
-    const uint64_t want = 4ull * 2 * sm_count, live = (uint64_t)B * a.kv.hkv, most = (blocks + kWarps - 1) / kWarps;
-    uint64_t n = (want + live - 1) / live;
-    if (n > most) n = most;
-    p.units = p.tiles * a.kv.hkv;
-    const size_t part = (size_t)cols * (head_dim + 2) * sizeof(float);
-    if (p.units > LFM_ATTN_COUNTS) p.units = LFM_ATTN_COUNTS;
-    if (n > LFM_ATTN_PARTS_BYTES / part / p.units) n = LFM_ATTN_PARTS_BYTES / part / p.units;
-    if (n < 1) n = 1;
-    p.chunk = (uint32_t)((blocks + n - 1) / n);
-    p.n_splits = (uint32_t)((blocks + p.chunk - 1) / p.chunk);
-    *used = p.n_splits > 1;
-    p.counts = static_cast<uint32_t *>(scratch);
-    p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + LFM_ATTN_COUNTS * sizeof(uint32_t));
-    const dim3 grid(B + p.extra, a.kv.hkv, p.n_splits);
+    const uint64_t per = (T + B - 1) / B * G;
+    const uint32_t nt = per <= 8 ? 1 : per <= 16 || head_dim == 128 ? 2 : 4;
+    /* blocks: as many as run at once, fewer where there are not enough blocks of keys by the hint */
+    uint64_t grid = (uint64_t)sm_count * (head_dim * nt <= 128 ? 2 : 1);
+    const uint64_t work = (B + T * G / (8 * nt)) * a.kv.hkv * ((max_kv_len + keys - 1) / keys + 1);
+    if (grid > (work + kWarps - 1) / kWarps) grid = (work + kWarps - 1) / kWarps;
+    if (grid > LFM_ATTN_COUNTS) grid = LFM_ATTN_COUNTS;
+    RowsPlan p{few, reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + LFM_ATTN_COUNTS * sizeof(uint32_t)),
+               static_cast<uint32_t *>(scratch)};
+    const dim3 g((uint32_t)grid);
     if (head_dim == 64)
-        return nt == 1 ? launch_rows<64, 1>(a, p, grid, s, pdl) : nt == 2 ? launch_rows<64, 2>(a, p, grid, s, pdl)
-                                                                          : launch_rows<64, 4>(a, p, grid, s, pdl);
-    return nt == 1 ? launch_rows<128, 1>(a, p, grid, s, pdl) : launch_rows<128, 2>(a, p, grid, s, pdl);
+        return nt == 1 ? launch_rows<64, 1>(a, p, g, s, pdl) : nt == 2 ? launch_rows<64, 2>(a, p, g, s, pdl)
+                                                                       : launch_rows<64, 4>(a, p, g, s, pdl);
+    return nt == 1 ? launch_rows<128, 1>(a, p, g, s, pdl) : launch_rows<128, 2>(a, p, g, s, pdl);
 }
 
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
                             bool *used, cudaStream_t s, bool pdl) {
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group;
-    *used = false;
+    *used = true;
     /* one sequence, or at most as many tokens as make few rows: one kernel takes all.  As many tokens as sequences
      * are a step of single tokens, whatever the odd sequence holds.  Otherwise each takes its sequences */
-    if (rows <= kFewRows || T == B) return lfm_launch_attn_rows(a, head_dim, ~0ull, max_kv_len, sm_count, scratch, used, s, pdl);
-    if (B == 1) return lfm_launch_attn_tile(a, head_dim, 0, s, pdl);
+    if (rows <= kFewRows || T == B) return lfm_launch_attn_rows(a, head_dim, ~0ull, max_kv_len, sm_count, scratch, s, pdl);
+    if (B == 1) {
+        *used = false;
+        return lfm_launch_attn_tile(a, head_dim, 0, s, pdl);
+    }
     const cudaError_t e = lfm_launch_attn_tile(a, head_dim, kFewRows, s, pdl);
-    return e != cudaSuccess ? e : lfm_launch_attn_rows(a, head_dim, kFewRows, max_kv_len, sm_count, scratch, used, s, pdl);
+    return e != cudaSuccess ? e : lfm_launch_attn_rows(a, head_dim, kFewRows, max_kv_len, sm_count, scratch, s, pdl);
 }

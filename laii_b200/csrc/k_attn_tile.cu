@@ -338,6 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         const uint32_t sub = min(A.kv.page_tokens, (uint32_t)kKeys), piece = sub * (D / 2 + D / 16);
         if (warp < 12) {
             /* codes -> values */
+            const LfmNib nib;
             const uint32_t key = (warp - 8) * 32 + lane, in = key & (sub - 1);
             const uint32_t codes = (key / sub) * piece + in * (D / 2), scales = (key / sub) * piece + sub * (D / 2) + in * (D / 16);
             for (uint32_t u = 0; u < 2 * n; ++u) {
@@ -360,10 +361,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                     for (int k = 0; k < 8; ++k) {
                         const uint32_t y = x[k] >> 8;
                         *reinterpret_cast<uint4 *>(to + (8 * s + k) * kChunk) =
-                            make_uint4(lfm_hmul2(lfm_hsub2(lfm_nib0(x[k]), LFM_NIB0_OFF), d),
-                                       lfm_hmul2(lfm_hsub2(lfm_nib1(x[k]), LFM_NIB1_OFF), d),
-                                       lfm_hmul2(lfm_hsub2(lfm_nib0(y), LFM_NIB0_OFF), d),
-                                       lfm_hmul2(lfm_hsub2(lfm_nib1(y), LFM_NIB1_OFF), d));
+                            make_uint4(lfm_hmul2(lfm_hsub2(nib.lo(x[k]), LFM_NIB0_OFF), d),
+                                       lfm_hmul2(lfm_hsub2(nib.hi(x[k]), LFM_NIB1_OFF), d),
+                                       lfm_hmul2(lfm_hsub2(nib.lo(y), LFM_NIB0_OFF), d),
+                                       lfm_hmul2(lfm_hsub2(nib.hi(y), LFM_NIB1_OFF), d));
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
