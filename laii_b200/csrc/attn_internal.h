@@ -78,7 +78,7 @@ cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_k
                             bool *used, cudaStream_t s, bool pdl);
 /* The tensor-core kernel for the sequences of more than `above` rows (token, head of a group). */
 cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, cudaStream_t s, bool pdl);
-#define LFM_ATTN_COUNTS 512u                                      /* most blocks that share work      */
+#define LFM_ATTN_COUNTS 1024u                                     /* most blocks that share work      */
 #define LFM_ATTN_PARTS_BYTES ((size_t)LFM_ATTN_COUNTS * 2 * 32 * 66 * 4) /* two parts each, 32 x (64 + 2) or 16 x (128 + 2) */
 #define LFM_ATTN_SCRATCH_BYTES (LFM_ATTN_PARTS_BYTES + LFM_ATTN_COUNTS * sizeof(uint32_t))
 

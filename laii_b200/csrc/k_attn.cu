@@ -23,11 +23,13 @@
  * through scratch: the last to finish joins the parts in their order (the same
  * bits on every run).
  */
+#include <type_traits>
+
 #include "attn_device.cuh"
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kStages = 3;
+constexpr int kWarps = 4, kThreads = kWarps * 32, kStages = 3;
 
 template <int D>
 struct Cfg {
@@ -97,60 +99,72 @@ struct Seq {
     bool sane;
 };
 
-/* A warp's issue and wait state over its blocks first, first + kWarps, ... */
+/* A warp's copies of its blocks of keys first, first + kWarps, ... of a unit. */
 template <int D>
 struct Ring {
-    const AttnArgs &A;
-    int b;
-    uint32_t kvh, smem, n;   /* n: blocks of this warp */
-    int64_t first, end;      /* first block; keys that exist */
+    static constexpr uint32_t kK = Cfg<D>::kKeys;
+    const KvDev &kv;
+    const BatchDev &bt;
+    uint32_t *err;
     uint64_t *bars;
-    uint32_t id, next;       /* pages of two blocks, 16 lanes each: a lane a part of a page */
+    uint32_t lane, to, bytes, per; /* this lane's part of a page: where it goes, its bytes, and bytes a token */
+    const int32_t *row;            /* the sequence's page table */
+    const uint8_t *from;           /* the part in page 0 */
+    uint32_t n;                    /* blocks of this warp */
+    int64_t first, end;            /* first block; keys that exist */
+    uint32_t id, next;             /* pages of two blocks, 16 lanes each: a lane a part of a page */
 
-    /* This lane's page in block i2 + lane / 16: piece lane / 4 % 4 of the block. */
+    /* Lane l: part l % 4 (K codes, K scales, V codes, V scales) of piece l / 4 % 4 of a block; a stage is
+     * [K codes][K scales][V codes][V scales] of its keys whatever the page's size. */
+    __device__ __forceinline__ Ring(const AttnArgs &A, uint64_t *bars, uint32_t smem)
+        : kv(A.kv), bt(A.bt), err(A.err), bars(bars), lane(threadIdx.x & 31) {
+        const uint32_t part = lane & 3, j = (lane >> 2) & 3, P = kv.page_tokens;
+        per = (part & 1) ? D / 16 : D / 2;
+        bytes = min(P, kK) * per;
+        to = smem + (part & 2 ? Cfg<D>::kBytes / 2 : 0) + ((part & 1) ? kK * (D / 2) : 0) + j * bytes;
+    }
+    __device__ __forceinline__ void unit(uint32_t b, uint32_t kvh, int64_t first_, uint32_t n_, int64_t end_) {
+        row = bt.page_table + (size_t)b * bt.table_stride;
+        from = kv.pages + (size_t)kvh * kv.head_bytes + (lane & 2 ? kv.half : 0) + (lane & 1 ? kv.codes : 0);
+        first = first_;
+        n = n_;
+        end = end_;
+        next = lookup(0);
+    }
+    /* This lane's page in block i2 + lane / 16. */
     __device__ __forceinline__ uint32_t lookup(uint32_t i2) {
-        constexpr uint32_t kK = Cfg<D>::kKeys;
-        const uint32_t lane = threadIdx.x & 31, i = i2 + lane / 16, j = (lane >> 2) & 3, P = A.kv.page_tokens;
-        const int64_t key = (first + (int64_t)i * kWarps) * kK + j * P;
-        if (i >= n || key >= end || (j && j * P >= kK)) return ~0u; /* nothing to copy */
-        const int64_t at = key >> A.kv.page_shift;
+        const uint32_t i = i2 + lane / 16, at = ((lane >> 2) & 3) * kv.page_tokens;
+        const int64_t key = (first + (int64_t)i * kWarps) * kK + at;
+        if (i >= n || key >= end || (at && at >= kK)) return ~0u; /* nothing to copy */
+        const int64_t place = key >> kv.page_shift;
         uint32_t page = ~0u;
-        if (at < (int64_t)A.bt.table_stride) page = (uint32_t)A.bt.page_table[(size_t)b * A.bt.table_stride + (size_t)at];
-        if (page >= A.kv.n_pages) atomicOr(A.err, LFM_DEVERR_PAGE);
+        if (place < (int64_t)bt.table_stride) page = (uint32_t)row[place];
+        if (page >= kv.n_pages) atomicOr(err, LFM_DEVERR_PAGE);
         return page;
     }
-
-    /* Copies of block i into its stage, [K codes][K scales][V codes][V scales] of its keys whatever the page's
-     * size: a lane a part (lane % 4) of a page. */
-    __device__ __forceinline__ void issue(uint32_t i) {
-        constexpr uint32_t kK = Cfg<D>::kKeys;
+    /* Block i into stage st. */
+    __device__ __forceinline__ void issue(uint32_t i, uint32_t st) {
         if ((i & 1) == 0) {
             id = next;
             next = lookup(i + 2);
         }
-        const uint32_t lane = threadIdx.x & 31, part = lane & 3, j = (lane >> 2) & 3, P = A.kv.page_tokens;
-        const uint32_t keys = P < kK ? P : kK;
-        const bool on = (lane >> 4) == (i & 1) && id < A.kv.n_pages;
-        const uint32_t bytes = on ? keys * ((part & 1) ? D / 16 : D / 2) : 0;
-        const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, bytes);
-        uint64_t *bar = bars + i % kStages;
-        if (lane == 0) lfm_mbar_arrive_tx(bar, all);
+        const bool on = (lane >> 4) == (i & 1) && id < kv.n_pages;
+        const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, on ? bytes : 0u);
+        if (lane == 0) lfm_mbar_arrive_tx(bars + st, all);
         __syncwarp();
         if (on) {
-            const uint32_t in = P > kK ? (uint32_t)((first + (int64_t)i * kWarps) * kK) & (P - 1) : 0;
-            const uint8_t *from = A.kv.pages + (size_t)id * A.kv.page_bytes + (size_t)kvh * A.kv.head_bytes +
-                                  (part & 2 ? A.kv.half : 0) + ((part & 1) ? A.kv.codes + in * (D / 16) : in * (D / 2));
-            const uint32_t to = smem + i % kStages * Cfg<D>::kBytes + (part & 2 ? Cfg<D>::kBytes / 2 : 0) +
-                                ((part & 1) ? kK * (D / 2) + j * P * (D / 16) : j * P * (D / 2));
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
-                         "l"(from), "r"(bytes), "r"(lfm_smem_u32(bar))
+            /* a page longer than a block: the block's keys in it */
+            const uint32_t in = ((uint32_t)(first + (int64_t)i * kWarps) * kK) & (kv.page_tokens - 1);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                             to + st * Cfg<D>::kBytes),
+                         "l"(from + (size_t)id * kv.page_bytes + in * per), "r"(bytes), "r"(lfm_smem_u32(bars + st))
                          : "memory");
         }
     }
 };
 
 template <int D, int NT, bool kCap>
-__global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(AttnArgs A, RowsPlan P) {
+__global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2) k_attn_rows(AttnArgs A, RowsPlan P) {
     using C = Cfg<D>;
     constexpr int kCols = 8 * NT, kS = C::kSpans, kPitch = D + 4;
     static_assert(kWarps * kCols * kPitch * 4 <= C::kRing, "the join fits the ring");
@@ -248,6 +262,10 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
     uint32_t b = (uint32_t)s_seq;
     uint64_t first = s_first; /* place of the sequence's first unit */
     Seq seq = sequence(b);
+    uint64_t n_blk = (uint64_t)(seq.blk1 - seq.blk0), u0 = (x - first) / n_blk; /* blocks of a unit, place of ours */
+    uint32_t kvh = (uint32_t)(u0 % A.kv.hkv), ct = (uint32_t)(u0 / A.kv.hkv);
+    u0 = first + u0 * n_blk;
+    Ring<D> rg(A, s_bar[warp], lfm_smem_u32(ring) + warp * kStages * C::kBytes);
 
     while (x < x1) {
         if (x >= first + seq.weight) { /* the next sequence that has work */
@@ -259,12 +277,15 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                 b = (uint32_t)s_seq;
                 seq = sequence(b);
             }
+            n_blk = (uint64_t)(seq.blk1 - seq.blk0);
+            u0 = first;
+            kvh = ct = 0;
         }
         const int64_t q0 = seq.q0, n_q = seq.n_q, len = seq.len;
-        const uint64_t n_blk = (uint64_t)(seq.blk1 - seq.blk0), unit = (x - first) / n_blk, u0 = first + unit * n_blk;
-        const uint32_t kvh = (uint32_t)(unit % A.kv.hkv), ct = (uint32_t)(unit / A.kv.hkv);
         const uint64_t seg = min(x1, u0 + n_blk) - x; /* key blocks of this unit that are ours */
-        const uint32_t own0 = owner(u0), own1 = owner(u0 + n_blk - 1);
+        /* the blocks that share the unit */
+        const uint32_t own0 = x == u0 ? blockIdx.x : owner(u0);
+        const uint32_t own1 = x + seg == u0 + n_blk ? blockIdx.x : owner(u0 + n_blk - 1);
         const uint32_t row0 = ct * kCols; /* rows of a sequence: (token, head of the group), below 2^31 */
         const int64_t rows = n_q * G - row0;
         const uint32_t last = (uint32_t)(rows < kCols ? rows : kCols) - 1;
@@ -281,14 +302,12 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
         const int64_t at0 = seq.blk0 + (int64_t)(x - u0), at1 = at0 + (int64_t)seg;
         const int64_t from = max(at0, lo0 / C::kKeys), to = min(at1, (hi1 + C::kKeys - 1) / C::kKeys);
         const int64_t mine = to - from - warp;
-        Ring<D> rg{A, (int)b, kvh, lfm_smem_u32(ring) + warp * kStages * C::kBytes,
-                   mine > 0 ? (uint32_t)((mine + kWarps - 1) / kWarps) : 0u, from + warp, len, s_bar[warp], 0, 0};
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads(); /* s_lo, s_hi; the ring is free of an earlier unit's join, for the copies too */
-        rg.next = rg.lookup(0);
+        rg.unit(b, kvh, from + warp, mine > 0 ? (uint32_t)((mine + kWarps - 1) / kWarps) : 0u, len);
 #pragma unroll
         for (uint32_t i = 0; i < kStages; ++i)
-            if (i < rg.n) rg.issue(i);
+            if (i < rg.n) rg.issue(i, i);
 
         /* ---- Q as B fragments: column g, values 64 s + 32 c + 8 t .. of the head ---- */
         uint32_t qf[NT][kS][2][4];
@@ -346,16 +365,11 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
         constexpr int kPair = NT == 1 ? 2 : 1; /* steps of 16 keys whose scores are looked at together */
         const LfmNib nib;
         bool ok = true;
-        for (uint32_t i = 0; i < rg.n; ++i) {
-            const uint32_t st = i % kStages;
-            ok = __all_sync(LFM_FULL_MASK, lfm_mbar_wait(&s_bar[warp][st], (phases >> st) & 1, A.err));
-            phases ^= 1u << st;
-            if (!ok) break;
-            const uint32_t buf = rg.smem + st * C::kBytes;
-            const int64_t key0 = (rg.first + (int64_t)i * kWarps) * C::kKeys;
-            const bool whole = key0 >= lo1 && key0 + C::kKeys <= hi0; /* every row sees every key */
-            const int held = (int)min((int64_t)C::kKeys, len - key0); /* slots that hold a token */
-#pragma unroll
+        /* a block of keys: every row sees all of it (inside), or masks, and `held` slots that hold a token */
+        auto block = [&](auto inside, uint32_t buf, int64_t key0) {
+            const int held = (int)min((int64_t)C::kKeys, len - key0);
+            constexpr bool kWhole = decltype(inside)::value;
+#pragma unroll(kWhole ? C::kKeys / 16 / kPair : 1)
             for (int s16 = 0; s16 < C::kKeys; s16 += 16 * kPair) {
                 /* S^T: rows rk and rk + 8, columns 2 t and 2 t + 1 */
                 float z4[kPair][NT][4];
@@ -402,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                             for (int j = 0; j < 4; ++j)
                                 z4[q][n][j] = __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(z4[q][n][j] * capz)), 1.0f);
                 }
-                if (!whole) {
+                if (!kWhole) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -466,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                     uint32_t dv[2][2 * kS]; /* scales of a pair of keys, and of the pair eight further */
                     lds(buf + atvs + k16 * (D / 16), dv[0]);
                     lds(buf + atvs + (k16 + 8) * (D / 16), dv[1]);
-                    if (held < C::kKeys) { /* what no token holds may be anything */
+                    if (!kWhole) { /* what no token holds may be anything */
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             if (k16 + (int)(ve & ~1u) + (k & 1) + (k & 2 ? 8 : 0) >= held) {
@@ -497,8 +511,18 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
                     }
                 }
             }
+        };
+        for (uint32_t i = 0, st = 0; i < rg.n; ++i, st = st + 1 == kStages ? 0 : st + 1) {
+            ok = __all_sync(LFM_FULL_MASK, lfm_mbar_wait(&s_bar[warp][st], (phases >> st) & 1, A.err));
+            phases ^= 1u << st;
+            if (!ok) break;
+            const uint32_t buf = lfm_smem_u32(ring) + (warp * kStages + st) * C::kBytes;
+            const int64_t key0 = (rg.first + (int64_t)i * kWarps) * C::kKeys;
+            const bool whole = key0 >= lo1 && key0 + C::kKeys <= hi0; /* every row sees every key */
+            if (whole) block(std::true_type(), buf, key0);
+            else block(std::false_type(), buf, key0);
             __syncwarp();
-            if (i + kStages < rg.n) rg.issue(i + kStages);
+            if (i + kStages < rg.n) rg.issue(i + kStages, st);
         }
         if (!ok) { /* a copy never came: wait (bounded) for those still under way before the ring is used again */
             for (uint32_t st = 0; st < kStages; ++st) lfm_mbar_wait(&s_bar[warp][st], (phases >> st) & 1, A.err);
@@ -585,6 +609,11 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) k_attn_rows(A
             }
         }
         x += seg;
+        u0 += n_blk;
+        if (++kvh == A.kv.hkv) {
+            kvh = 0;
+            ++ct;
+        }
     }
 }
 
@@ -608,7 +637,7 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
     const uint64_t per = (T + B - 1) / B * G;
     const uint32_t nt = per <= 8 ? 1 : per <= 16 || head_dim == 128 ? 2 : 4;
     /* blocks: as many as run at once, fewer where there are not enough blocks of keys by the hint */
-    uint64_t grid = (uint64_t)sm_count * (head_dim * nt <= 128 ? 2 : 1);
+    uint64_t grid = (uint64_t)sm_count * (head_dim * nt <= 128 ? 4 : 2);
     const uint64_t work = (B + T * G / (8 * nt)) * a.kv.hkv * ((max_kv_len + keys - 1) / keys + 1);
     if (grid > (work + kWarps - 1) / kWarps) grid = (work + kWarps - 1) / kWarps;
     if (grid > LFM_ATTN_COUNTS) grid = LFM_ATTN_COUNTS;
