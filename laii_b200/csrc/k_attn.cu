@@ -164,7 +164,7 @@ struct Ring {
 };
 
 template <int D, int NT, bool kCap>
-__global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2) k_attn_rows(AttnArgs A, RowsPlan P) {
+__global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3 : 2) k_attn_rows(AttnArgs A, RowsPlan P) {
     using C = Cfg<D>;
     constexpr int kCols = 8 * NT, kS = C::kSpans, kPitch = D + 4;
     static_assert(kWarps * kCols * kPitch * 4 <= C::kRing, "the join fits the ring");
@@ -637,7 +637,7 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
     const uint64_t per = (T + B - 1) / B * G;
     const uint32_t nt = per <= 8 ? 1 : per <= 16 || head_dim == 128 ? 2 : 4;
     /* blocks: as many as run at once, fewer where there are not enough blocks of keys by the hint */
-    uint64_t grid = (uint64_t)sm_count * (head_dim * nt <= 128 ? 4 : 2);
+    uint64_t grid = (uint64_t)sm_count * (head_dim * nt < 128 ? 4 : head_dim * nt == 128 ? 3 : 2);
     const uint64_t work = (B + T * G / (8 * nt)) * a.kv.hkv * ((max_kv_len + keys - 1) / keys + 1);
     if (grid > (work + kWarps - 1) / kWarps) grid = (work + kWarps - 1) / kWarps;
     if (grid > LFM_ATTN_COUNTS) grid = LFM_ATTN_COUNTS;
