@@ -114,6 +114,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
+/* One thread of the warp, all of which run this. */
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 /* Bounded wait that also gives up once another role has. */
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err) {
     if (lfm_mbar_try_wait(bar, parity)) return true;
@@ -288,14 +295,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             }
             const uint64_t nm2 = pk2(__float_as_uint(-m), __float_as_uint(-m));
             uint64_t la = 0;
+            /* 32 at a time, each operation on all of them before the next one: the exponentials' latency is hidden
+             * behind one another */
 #pragma unroll
-            for (int i = 0; i < kKeys; i += 2) {
-                const uint64_t x = fma2(pk2(s[i], s[i + 1]), sc2, nm2);
-                const float p0 = lfm_ex2(__uint_as_float((uint32_t)x)), p1 = lfm_ex2(__uint_as_float((uint32_t)(x >> 32)));
-                const uint64_t p = pk2(__float_as_uint(p0), __float_as_uint(p1));
-                if (i & 2) la = add2(la, p);
-                else l2 = add2(l2, p);
-                s[i / 2] = lfm_pack2(p0, p1, __half());
+            for (int c = 0; c < kKeys; c += 32) {
+#pragma unroll
+                for (int i = c; i < c + 32; i += 2) {
+                    const uint64_t x = fma2(pk2(s[i], s[i + 1]), sc2, nm2);
+                    s[i] = (uint32_t)x;
+                    s[i + 1] = (uint32_t)(x >> 32);
+                }
+#pragma unroll
+                for (int i = c; i < c + 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(s[i]));
+#pragma unroll
+                for (int i = c; i < c + 32; i += 4) {
+                    l2 = add2(l2, pk2(s[i], s[i + 1]));
+                    la = add2(la, pk2(s[i + 2], s[i + 3]));
+                }
+#pragma unroll
+                for (int i = c; i < c + 32; i += 2)
+                    s[i / 2] = lfm_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]), __half());
             }
             l2 = add2(l2, la);
             st32(tS, s);
@@ -375,49 +394,50 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 }
             }
         } else if (warp == 12) {
-            if (lane == 0) {
-                auto full = [&](uint32_t u) { return wait(&bars.op_full[u % C::kOps], (u / C::kOps) & 1, abort, A.err); };
-                auto op = [&](uint32_t u) { return smem + C::kOffOp + (u % C::kOps) * C::kOp; };
-                auto qk = [&](uint32_t h, uint32_t u) {
-                    const uint64_t qd = sdesc(smem + h * C::kOp, kChunk, 128), kd = sdesc(op(u), kChunk, 128);
+            /* The whole warp walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all
+             * columns are ours) then stay in uniform registers.  From a branch of lane 0 alone they take moves
+             * through the pipe that the softmax warps' exponentials fill, and an MMA waits 350 cycles for its turn */
+            auto full = [&](uint32_t u) {
+                const bool w = __all_sync(LFM_FULL_MASK, wait(&bars.op_full[u % C::kOps], (u / C::kOps) & 1, abort, A.err));
+                fence_after();
+                return w;
+            };
+            auto op = [&](uint32_t u) { return smem + C::kOffOp + (u % C::kOps) * C::kOp; };
+            auto qk = [&](uint32_t h, uint32_t u) {
+                const uint64_t qd = sdesc(smem + h * C::kOp, kChunk, 128), kd = sdesc(op(u), kChunk, 128);
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_ss(tmem + h * kColS, qd + k * (2 * kChunk >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
-                };
-                auto pv = [&](uint32_t h, uint32_t u, bool first) {
-                    const uint64_t vd = sdesc(op(u), 128, kChunk);
+                for (int k = 0; k < D / 16; ++k)
+                    mma_ss(h * kColS, qd + k * (2 * kChunk >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
+                commit(&bars.s_full[h]);
+            };
+            auto pv = [&](uint32_t h, uint32_t u, bool first) {
+                const uint64_t vd = sdesc(op(u), 128, kChunk);
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        mma_ts(tmem + kColO + h * D, tmem + h * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
-                };
-                ok = full(0);
-                if (ok) {
+                for (int k = 0; k < kKeys / 16; ++k)
+                    mma_ts(kColO + h * D, h * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
+            };
+            ok = tmem == 0 && full(0);
+            if (ok && elect()) {
+                qk(0, 0);
+                qk(1, 0);
+                commit(&bars.op_empty[0]);
+            }
+            for (uint32_t j = 0; j < n && ok; ++j) {
+                const bool more = j + 1 < n;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    ok = ok && __all_sync(LFM_FULL_MASK, wait(&bars.p_full[h], j & 1, abort, A.err)) && (h || full(2 * j + 1));
+                    if (!ok) break;
                     fence_after();
-                    qk(0, 0);
-                    commit(&bars.s_full[0]);
-                    qk(1, 0);
-                    commit(&bars.s_full[1]);
-                    commit(&bars.op_empty[0]);
-                }
-                for (uint32_t j = 0; j < n && ok; ++j) {
-                    for (uint32_t h = 0; h < 2 && ok; ++h) {
-                        ok = wait(&bars.p_full[h], j & 1, abort, A.err) && (h || full(2 * j + 1));
-                        if (!ok) break;
-                        fence_after();
+                    if (elect()) {
                         pv(h, 2 * j + 1, j == 0);
                         if (h) commit(&bars.op_empty[(2 * j + 1) % C::kOps]);
-                        if (j + 1 < n) {
-                            if (!h) {
-                                ok = full(2 * j + 2);
-                                if (!ok) break;
-                                fence_after();
-                            }
-                            qk(h, 2 * j + 2);
-                            commit(&bars.s_full[h]);
-                            if (h) commit(&bars.op_empty[(2 * j + 2) % C::kOps]);
-                        } else {
-                            commit(&bars.o_full[h]);
-                        }
+                        if (!more) commit(&bars.o_full[h]);
+                    }
+                    if (more && !h) ok = full(2 * j + 2);
+                    if (ok && more && elect()) {
+                        qk(h, 2 * j + 2);
+                        if (h) commit(&bars.op_empty[(2 * j + 2) % C::kOps]);
                     }
                 }
             }
