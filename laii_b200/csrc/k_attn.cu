@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (on) lfm_load_q(A, at + 64 * s + 32 * c + 8 * t, A.scale < 0.0f && !kCap, v);
+                    if (on) lfm_load_q(A, at + 64 * s + 32 * c + 8 * t, A.scale < 0.0f, v);
                     float h[8], sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
         const uint32_t atk = rk * (D / 2) + 8 * t, atks = kKs + rk * (D / 16);
         const uint32_t atve = kV + ve * (D / 2) + 4 * g, atvo = kV + vo * (D / 2) + 4 * g;
         const uint32_t atvs = kV + kKs + (ve & ~1u) * (D / 16);
-        const float capz = kCap ? A.scale * 2.88539008f / A.softcap : 0.0f;
+        const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
         constexpr int kPair = NT == 1 ? 2 : 1; /* steps of 16 keys whose scores are looked at together */
         const LfmNib nib;
         bool ok = true;

@@ -33,18 +33,21 @@ struct Cfg {
     static constexpr int kOp = kKeys * D * 2;               /* an operand tile                      */
     static constexpr int kRaw = kKeys * (D / 2 + D / 16);   /* its codes and scales                 */
     static constexpr int kOps = D == 64 ? 6 : 4, kRaws = D == 64 ? 6 : 3;
+    /* buffers of S (and P) in TMEM, taken in turn by (key block, tile): with a third one the scores of a tile's
+     * next block are ready when its softmax ends; 128-value heads leave room for two */
+    static constexpr uint32_t kBufs = D == 64 ? 3 : 2, kColO = kBufs * kKeys;
     static constexpr int kOffOp = 2 * kOp, kOffRaw = kOffOp + kOps * kOp, kSmem = kOffRaw + kRaws * kRaw;
     static_assert(kSmem <= 226 * 1024, "shared memory");
 };
 
-constexpr uint32_t kTmemCols = 512, kColS = kKeys, kColO = 2 * kKeys;
+constexpr uint32_t kTmemCols = 512, kColS = kKeys;
 /* kind::f16, A and B fp16, D fp32 (bit 4), M / 16 at bit 24, N / 8 at 17; B transposed (N contiguous) at 16 */
 constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(kKeys >> 3) << 17);
 template <int D>
 constexpr uint32_t kIdescPV = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(D >> 3) << 17) | (1u << 16);
 
 struct Bars {
-    uint64_t raw_full[6], raw_empty[6], op_full[6], op_empty[6], s_full[2], p_full[2], o_full[2];
+    uint64_t raw_full[6], raw_empty[6], op_full[6], op_empty[6], s_full[3], p_full[3], o_full[2];
     uint32_t tmem;
     int abort, tile[2];
 };
@@ -94,6 +97,14 @@ __device__ __forceinline__ void st32(uint32_t t, const uint32_t *v) {
         R8(v, 0), R8(v, 8), R8(v, 16), R8(v, 24)
         : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t t, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
+                 R8(v, 0), R8(v, 8)
+                 : "memory");
+}
+__device__ __forceinline__ void max3(float &m, uint32_t a, uint32_t b) {
+    asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+}
 /* Keeps the uses of loaded registers behind the wait. */
 __device__ __forceinline__ void tie32(uint32_t *v) { asm volatile("" : X8(v, 0), X8(v, 8), X8(v, 16), X8(v, 24)::"memory"); }
 
@@ -141,7 +152,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
     using C = Cfg<D>;
     extern __shared__ __align__(1024) uint8_t sm[];
     __shared__ Bars bars;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.group, kvh = blockIdx.y;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.group;
+    const uint32_t kvh = blockIdx.x % A.kv.hkv, tiles = gridDim.x / A.kv.hkv;
     volatile int *abort = &bars.abort;
     if (tid == 0) {
         for (int i = 0; i < C::kRaws; ++i) {
@@ -152,17 +164,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             lfm_mbar_init(&bars.op_full[i], 4);
             lfm_mbar_init(&bars.op_empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < C::kBufs; ++i) {
             lfm_mbar_init(&bars.s_full[i], 1);
             lfm_mbar_init(&bars.p_full[i], 4);
-            lfm_mbar_init(&bars.o_full[i], 1);
         }
+        for (int i = 0; i < 2; ++i) lfm_mbar_init(&bars.o_full[i], 1);
         bars.abort = 0;
         lfm_fence_mbar_init();
     }
     lfm_pdl_wait();
-    /* the longest walks first: tiles from the last */
-    if (warp == 0) lfm_find_tile(A.bt, G, kRows, 0, above, ~0ull, gridDim.x - 1 - blockIdx.x, bars.tile);
+    /* the longest walks first: tiles from the last, all heads of one side by side */
+    if (warp == 0) lfm_find_tile(A.bt, G, kRows, 0, above, ~0ull, tiles - 1 - blockIdx.x / A.kv.hkv, bars.tile);
     __syncthreads();
     const int b = bars.tile[0];
     if (b < 0) return;
@@ -206,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (r < rows) {
             const size_t at = row_at(r, A.q_stride) + 64 * s + 8 * v;
-            const bool neg = A.scale < 0.0f && !kCap;
+            const bool neg = A.scale < 0.0f;
             lfm_load_q(A, at, neg, x);
             lfm_load_q(A, at + 32, neg, y);
         }
@@ -224,11 +236,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
     bool ok = true;
 
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const uint32_t h = warp >> 2, r = h * kM + (warp & 3) * 32 + lane;
-        const uint32_t tS = tmem + h * kColS + ((warp & 3) << 21), tO = tmem + kColO + h * D + ((warp & 3) << 21);
+        const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
         const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
-        const float capz = kCap ? A.scale * 2.88539008f / A.softcap : 0.0f;
+        const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
         int64_t lo = 0, hi = 0;
         if (r < rows) lfm_visible(A, n_q, len, row0 + r, lo, hi);
         /* over the tile: every row sees [lo_all, hi_all) */
@@ -241,42 +252,54 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         float m = LFM_NO_KEY;
         uint64_t l2 = 0;
         for (uint32_t j = 0; j < n; ++j) {
-            ok = __all_sync(LFM_FULL_MASK, wait(&bars.s_full[h], j & 1, abort, A.err));
+            const uint32_t q = 2 * j + h, buf = q % C::kBufs;
+            const uint32_t tS = tmem + buf * kColS + ((warp & 3) << 21);
+            ok = __all_sync(LFM_FULL_MASK, wait(&bars.s_full[buf], (q / C::kBufs) & 1, abort, A.err));
             if (!ok) break;
             fence_after();
-            uint32_t s[kKeys];
-#pragma unroll
-            for (int i = 0; i < kKeys; i += 32) ld32(tS + i, s + i);
-            wait_ld();
-#pragma unroll
-            for (int i = 0; i < kKeys; i += 32) tie32(s + i);
-            if (kCap) {
-#pragma unroll
-                for (int i = 0; i < kKeys; ++i)
-                    s[i] = __float_as_uint(__fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(__uint_as_float(s[i]) * capz)), 1.0f));
-            }
             const int64_t key0 = (blk0 + j) * kKeys;
-            if (key0 < lo_all || key0 + kKeys > hi_all) {
-                const int to = (int)max((int64_t)0, min((int64_t)kKeys, hi - key0));
-                const int from = (int)max((int64_t)0, min((int64_t)kKeys, lo - key0));
+            const bool masked = key0 < lo_all || key0 + kKeys > hi_all;
+            const int to = masked ? (int)max((int64_t)0, min((int64_t)kKeys, hi - key0)) : kKeys;
+            const int from = masked ? (int)max((int64_t)0, min((int64_t)kKeys, lo - key0)) : 0;
+            auto mask = [&](uint32_t *x, int c) {
 #pragma unroll
-                for (int i = 0; i < kKeys; ++i)
-                    if (i < from || i >= to) s[i] = 0xFF800000u;
-            }
+                for (int i = 0; i < 32; ++i)
+                    if (c + i < from || c + i >= to) x[i] = 0xFF800000u;
+            };
+            uint32_t x[2][32]; /* S is read twice, 32 columns at a time: the registers of all 128 are not there */
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < kKeys; i += 8) {
+            for (int c = 0; c < kKeys; c += 64) {
+                ld32(tS + c, x[0]);
+                ld32(tS + c + 32, x[1]);
+                wait_ld();
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1])));
+                for (int k = 0; k < 2; ++k) {
+                    tie32(x[k]);
+                    if (masked) mask(x[k], c + 32 * k);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        max3(mx[0], x[k][i], x[k][i + 1]);
+                        max3(mx[1], x[k][i + 2], x[k][i + 3]);
+                        max3(mx[2], x[k][i + 4], x[k][i + 5]);
+                        max3(mx[3], x[k][i + 6], x[k][i + 7]);
+                    }
+                }
             }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            ld32(tS, x[0]);
+            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            /* tanh(x) = 1 - 2 / (1 + e^2x), which keeps the order */
+            auto cap = [&](float z) { return __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(z * capz)), 1.0f); };
+            if (kCap) top = top > -INFINITY ? cap(top) : top;
             if (__any_sync(LFM_FULL_MASK, __fmaf_rn(top, sc, -m) > 8.0f)) {
                 const float nm = fmaxf(m, top * sc), f = lfm_ex2(m - nm);
                 const uint64_t f2 = pk2(__float_as_uint(f), __float_as_uint(f));
                 m = nm;
                 l2 = mul2(l2, f2);
-                if (j) { /* s_full of this block: the products of the one before are in O */
+                if (j) { /* the products of the block before are in O first */
+                    ok = __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h], (j - 1) & 1, abort, A.err));
+                    if (!ok) break;
+                    fence_after();
 #pragma unroll
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
@@ -295,56 +318,61 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             }
             const uint64_t nm2 = pk2(__float_as_uint(-m), __float_as_uint(-m));
             uint64_t la = 0;
-            /* 32 at a time, each operation on all of them before the next one: the exponentials' latency is hidden
-             * behind one another */
 #pragma unroll
-            for (int c = 0; c < kKeys; c += 32) {
+            for (int c = 0; c < 4; ++c) {
+                uint32_t *y = x[c & 1];
+                wait_ld();
+                tie32(y);
+                if (c < 3) ld32(tS + 32 * c + 32, x[(c + 1) & 1]);
+                if (kCap) {
 #pragma unroll
-                for (int i = c; i < c + 32; i += 2) {
-                    const uint64_t x = fma2(pk2(s[i], s[i + 1]), sc2, nm2);
-                    s[i] = (uint32_t)x;
-                    s[i + 1] = (uint32_t)(x >> 32);
+                    for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(cap(__uint_as_float(y[i])));
+                }
+                if (masked) mask(y, 32 * c);
+                /* each operation on all before the next one: the exponentials' latency hides behind one another */
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const uint64_t z = fma2(pk2(y[i], y[i + 1]), sc2, nm2);
+                    y[i] = (uint32_t)z;
+                    y[i + 1] = (uint32_t)(z >> 32);
                 }
 #pragma unroll
-                for (int i = c; i < c + 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(s[i]));
+                for (int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(y[i]));
+                uint32_t pk[16];
 #pragma unroll
-                for (int i = c; i < c + 32; i += 4) {
-                    l2 = add2(l2, pk2(s[i], s[i + 1]));
-                    la = add2(la, pk2(s[i + 2], s[i + 3]));
+                for (int i = 0; i < 32; i += 2) {
+                    if (i & 2) la = add2(la, pk2(y[i], y[i + 1]));
+                    else l2 = add2(l2, pk2(y[i], y[i + 1]));
+                    pk[i / 2] = lfm_pack2(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), __half());
                 }
-#pragma unroll
-                for (int i = c; i < c + 32; i += 2)
-                    s[i / 2] = lfm_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]), __half());
+                st16(tS + 16 * c, pk); /* over columns that are read by now */
             }
             l2 = add2(l2, la);
-            st32(tS, s);
-            st32(tS + 32, s + 32);
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) lfm_mbar_arrive(&bars.p_full[h]);
+            if (lane == 0) lfm_mbar_arrive(&bars.p_full[buf]);
         }
-        if (ok) ok = __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h], 0, abort, A.err));
+        if (ok) ok = __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h], (n - 1) & 1, abort, A.err));
         if (ok) {
             fence_after();
             const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             const size_t at = r < rows ? row_at(r, A.out_stride) : 0;
 #pragma unroll
-            for (int s = 0; s < D / 64; ++s) {
-                uint32_t o[64];
-                ld32(tO + 64 * s, o);
-                ld32(tO + 64 * s + 32, o + 32);
+            for (int c = 0; c < D / 32; ++c) {
+                /* columns 32 c ..: values 16 k .. + 15 of the span in the even ones, 32 + 16 k .. in the odd ones */
+                uint32_t o[32];
+                ld32(tO + 32 * c, o);
                 wait_ld();
                 tie32(o);
-                tie32(o + 32);
                 if (r < rows) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) { /* values 0 .. 31 of the span are the even columns */
+                    for (int e = 0; e < 4; ++e) {
                         float v[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[2 * (8 * (c & 3) + i) + (c >> 2)]) * inv;
-                        const size_t to = at + 64 * s + 8 * c;
+                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[2 * (8 * (e & 1) + i) + (e >> 1)]) * inv;
+                        const size_t to = at + 64 * (c >> 1) + 16 * (c & 1) + 8 * (e & 1) + 32 * (e >> 1);
                         if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + to, v);
                         else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + to, v);
                         else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + to, v);
@@ -353,7 +381,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const uint32_t sub = min(A.kv.page_tokens, (uint32_t)kKeys), piece = sub * (D / 2 + D / 16);
         if (warp < 12) {
             /* codes -> values */
@@ -397,47 +424,53 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             /* The whole warp walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all
              * columns are ours) then stay in uniform registers.  From a branch of lane 0 alone they take moves
              * through the pipe that the softmax warps' exponentials fill, and an MMA waits 350 cycles for its turn */
-            auto full = [&](uint32_t u) {
-                const bool w = __all_sync(LFM_FULL_MASK, wait(&bars.op_full[u % C::kOps], (u / C::kOps) & 1, abort, A.err));
+            auto full = [&](uint32_t u, uint32_t slot) {
+                const bool w = __all_sync(LFM_FULL_MASK, wait(&bars.op_full[slot], (u / C::kOps) & 1, abort, A.err));
                 fence_after();
                 return w;
             };
-            auto op = [&](uint32_t u) { return smem + C::kOffOp + (u % C::kOps) * C::kOp; };
-            auto qk = [&](uint32_t h, uint32_t u) {
-                const uint64_t qd = sdesc(smem + h * C::kOp, kChunk, 128), kd = sdesc(op(u), kChunk, 128);
+            /* step q = 2 * block + tile; i = q modulo the unrolling, known to the compiler with all that it gives */
+            constexpr uint32_t kUn = C::kOps; /* a multiple of 2 and of kBufs */
+            static_assert(kUn % 2 == 0 && kUn % C::kBufs == 0, "unrolling");
+            auto op = [&](uint32_t i) { return smem + C::kOffOp + i * C::kOp; };
+            auto qk = [&](uint32_t i) {
+                const uint32_t h = i & 1, buf = i % C::kBufs, k0 = i & ~1u;
+                const uint64_t qd = sdesc(smem + h * C::kOp, kChunk, 128), kd = sdesc(op(k0), kChunk, 128);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(h * kColS, qd + k * (2 * kChunk >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
-                commit(&bars.s_full[h]);
+                    mma_ss(buf * kColS, qd + k * (2 * kChunk >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
+                commit(&bars.s_full[buf]);
+                if (h) commit(&bars.op_empty[k0]);
             };
-            auto pv = [&](uint32_t h, uint32_t u, bool first) {
-                const uint64_t vd = sdesc(op(u), 128, kChunk);
+            auto pv = [&](uint32_t i, bool first) {
+                const uint32_t h = i & 1, buf = i % C::kBufs, v0 = i | 1u;
+                const uint64_t vd = sdesc(op(v0), 128, kChunk);
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k)
-                    mma_ts(kColO + h * D, h * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
+                    mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
+                commit(&bars.o_full[h]);
+                if (h) commit(&bars.op_empty[v0]);
             };
-            ok = tmem == 0 && full(0);
-            if (ok && elect()) {
-                qk(0, 0);
-                qk(1, 0);
-                commit(&bars.op_empty[0]);
-            }
-            for (uint32_t j = 0; j < n && ok; ++j) {
-                const bool more = j + 1 < n;
+            ok = tmem == 0;
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    ok = ok && __all_sync(LFM_FULL_MASK, wait(&bars.p_full[h], j & 1, abort, A.err)) && (h || full(2 * j + 1));
+            for (uint32_t q = 0; q < C::kBufs; ++q) {
+                if (!ok || q >= 2 * n) break;
+                if (!(q & 1)) ok = full(q, q);
+                if (ok && elect()) qk(q);
+            }
+            for (uint32_t q0 = 0; q0 < 2 * n && ok; q0 += kUn) {
+#pragma unroll
+                for (uint32_t i = 0; i < kUn; ++i) {
+                    const uint32_t q = q0 + i, buf = i % C::kBufs, next = (i + C::kBufs) % kUn;
+                    if (!ok || q >= 2 * n) break;
+                    ok = __all_sync(LFM_FULL_MASK, wait(&bars.p_full[buf], (q / C::kBufs) & 1, abort, A.err)) &&
+                         ((i & 1) || full(q | 1u, i | 1u));
                     if (!ok) break;
                     fence_after();
-                    if (elect()) {
-                        pv(h, 2 * j + 1, j == 0);
-                        if (h) commit(&bars.op_empty[(2 * j + 1) % C::kOps]);
-                        if (!more) commit(&bars.o_full[h]);
-                    }
-                    if (more && !h) ok = full(2 * j + 2);
-                    if (ok && more && elect()) {
-                        qk(h, 2 * j + 2);
-                        if (h) commit(&bars.op_empty[(2 * j + 2) % C::kOps]);
+                    if (elect()) pv(i, q < 2);
+                    if (q + C::kBufs < 2 * n) {
+                        if (!(next & 1)) ok = full(q + C::kBufs, next);
+                        if (ok && elect()) qk(next);
                     }
                 }
             }
@@ -494,7 +527,9 @@ cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t 
     /* a tile for every started kRows rows of a sequence: at most this many */
     const uint64_t rows = (uint64_t)a.bt.n_tokens * a.group, most = a.bt.n_seqs < a.bt.n_tokens ? a.bt.n_seqs : a.bt.n_tokens;
     const uint64_t big = rows / (above + 1) < most ? rows / (above + 1) : most; /* sequences of more than `above` rows */
-    const dim3 grid((uint32_t)(rows / kRows + big), a.kv.hkv);
-    if (grid.x == 0) return cudaSuccess;
+    const uint64_t blocks = (rows / kRows + big) * a.kv.hkv; /* below 2^31 / 256 * 1024 / group */
+    if (blocks == 0) return cudaSuccess;
+    if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    const dim3 grid((uint32_t)blocks);
     return head_dim == 64 ? launch_tile<64>(a, above, grid, s, pdl) : launch_tile<128>(a, above, grid, s, pdl);
 }
