@@ -50,6 +50,9 @@ struct Bars {
     uint64_t raw_full[6], raw_empty[6], op_full[6], op_empty[6], s_full[3], p_full[3], o_full[2];
     uint32_t tmem;
     int abort, tile[2];
+    /* the block's rows for the epilogue: kept here, their registers are the softmax's */
+    long long q0;
+    uint32_t row0, rows, kvh;
 };
 
 /* No swizzle, version 1: start, leading and stride byte offsets. */
@@ -204,6 +207,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         }
         return;
     }
+    if (tid == 0) {
+        bars.q0 = q0;
+        bars.row0 = row0;
+        bars.rows = rows;
+        bars.kvh = kvh;
+    }
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
                      "r"(kTmemCols)
@@ -236,17 +245,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
     bool ok = true;
 
     if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;"); /* 256 x 152 + 256 x 104 = 512 x 128 */
         const uint32_t h = warp >> 2, r = h * kM + (warp & 3) * 32 + lane;
         const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
         const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
         const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
-        int64_t lo = 0, hi = 0;
-        if (r < rows) lfm_visible(A, n_q, len, row0 + r, lo, hi);
-        /* over the tile: every row sees [lo_all, hi_all) */
-        int64_t lo_all = 0, hi_all = 0, unused;
-        if (h * kM < rows) {
-            lfm_visible(A, n_q, len, row0 + h * kM, unused, hi_all);
-            lfm_visible(A, n_q, len, row0 + min(rows, (h + 1) * kM) - 1, lo_all, unused);
+        /* what the row sees, in keys from the first block; the blocks [inside0, inside1) every row of the tile sees whole */
+        int lo = 0, hi = 0, inside0 = 0, inside1 = 0;
+        {
+            int64_t a = 0, e = 0, a_all = 0, e_all = 0, unused;
+            if (r < rows) lfm_visible(A, n_q, len, row0 + r, a, e);
+            if (h * kM < rows) {
+                lfm_visible(A, n_q, len, row0 + h * kM, unused, e_all);
+                lfm_visible(A, n_q, len, row0 + min(rows, (h + 1) * kM) - 1, a_all, unused);
+            }
+            const int64_t base = blk0 * kKeys; /* positions are below 2^31 */
+            lo = (int)max((int64_t)0, a - base);
+            hi = (int)max((int64_t)0, e - base);
+            inside0 = (int)((max((int64_t)0, a_all - base) + kKeys - 1) / kKeys);
+            inside1 = (int)(max((int64_t)0, e_all - base) / kKeys);
         }
         const uint64_t sc2 = pk2(__float_as_uint(sc), __float_as_uint(sc));
         float m = LFM_NO_KEY;
@@ -257,10 +274,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             ok = __all_sync(LFM_FULL_MASK, wait(&bars.s_full[buf], (q / C::kBufs) & 1, abort, A.err));
             if (!ok) break;
             fence_after();
-            const int64_t key0 = (blk0 + j) * kKeys;
-            const bool masked = key0 < lo_all || key0 + kKeys > hi_all;
-            const int to = masked ? (int)max((int64_t)0, min((int64_t)kKeys, hi - key0)) : kKeys;
-            const int from = masked ? (int)max((int64_t)0, min((int64_t)kKeys, lo - key0)) : 0;
+            const bool masked = (int)j < inside0 || (int)j >= inside1;
+            const int from = lo - (int)j * kKeys, to = hi - (int)j * kKeys;
             auto mask = [&](uint32_t *x, int c) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
@@ -358,7 +373,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             fence_after();
             const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            const size_t at = r < rows ? row_at(r, A.out_stride) : 0;
+            volatile Bars *vb = &bars;
+            const uint32_t row = vb->row0 + r;
+            const bool on = r < vb->rows;
+            const size_t at = (size_t)(vb->q0 + row / A.group) * A.out_stride + ((size_t)vb->kvh * A.group + row % A.group) * D;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 /* columns 32 c ..: values 16 k .. + 15 of the span in the even ones, 32 + 16 k .. in the odd ones */
@@ -366,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 ld32(tO + 32 * c, o);
                 wait_ld();
                 tie32(o);
-                if (r < rows) {
+                if (on) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float v[8];
@@ -381,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             }
         }
     } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         const uint32_t sub = min(A.kv.page_tokens, (uint32_t)kKeys), piece = sub * (D / 2 + D / 16);
         if (warp < 12) {
             /* codes -> values */
