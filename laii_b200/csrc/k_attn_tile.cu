@@ -3,18 +3,20 @@
  * sequence (prompts, chunks), on the 5th-generation tensor cores.
  *
  * A block takes 256 rows (token, head of the group) of one kv head as two
- * tiles of M = 128 and walks their keys 128 at a time, once:
+ * tiles of M = 128 and walks their keys 64 at a time, once:
  *   loader    bulk copies of a key block's codes and scales, K and V apart
- *   4 warps   codes -> fp16 values, a thread a key, into the operand layout of
+ *   4 warps   codes -> fp16 values, two threads a key, into the operand layout of
  *             the MMA (no swizzle: 8 x 16-byte core matrices).  The layout's
  *             order of a head's values is that of the codes' words -- values
  *             4 w + i and 32 + 4 w + i side by side, so a word gives its eight
  *             with one shift and four pairs of one logic instruction, and the
  *             two scales of a span are the pair that multiplies them.  q is
  *             laid out in the same order and the output read back from it
- *   MMA       one thread: S_h = Q_h K^T (fp32, TMEM), O_h += P_h V with P_h,
- *             fp16, read from the TMEM columns of S_h; the tiles take turns, so
- *             one multiplies while the other is in its softmax
+ *   MMA       one thread: S = Q_h K^T (fp32, TMEM), O_h += P V with P, fp16,
+ *             read from the TMEM columns of its S.  S has as many buffers as
+ *             TMEM leaves beside O (6 of 64 columns for 64-value heads, 4 for
+ *             128), taken in turn by (key block, tile), so the scores of a
+ *             tile's next block are there when its softmax ends
  *   2 x 4 warps  softmax, a thread a row: no exchange between threads.  The
  *             running reference m only moves when a score passes it by 2^8
  *             (p <= 256 in fp16); then the thread scales its row of O in TMEM
@@ -25,18 +27,16 @@
 
 namespace {
 
-constexpr int kM = 128, kRows = 2 * kM, kKeys = 128, kThreads = 512;
-constexpr uint32_t kChunk = kM * 16;  /* bytes between the 8-value chunks of a row */
+constexpr int kM = 128, kRows = 2 * kM, kKeys = 64, kThreads = 512;
+constexpr uint32_t kChunkQ = kM * 16, kChunk = kKeys * 16; /* bytes between the 8-value chunks of a row */
 
 template <int D>
 struct Cfg {
-    static constexpr int kOp = kKeys * D * 2;               /* an operand tile                      */
-    static constexpr int kRaw = kKeys * (D / 2 + D / 16);   /* its codes and scales                 */
-    static constexpr int kOps = D == 64 ? 6 : 4, kRaws = D == 64 ? 6 : 3;
-    /* buffers of S (and P) in TMEM, taken in turn by (key block, tile): with a third one the scores of a tile's
-     * next block are ready when its softmax ends; 128-value heads leave room for two */
-    static constexpr uint32_t kBufs = D == 64 ? 3 : 2, kColO = kBufs * kKeys;
-    static constexpr int kOffOp = 2 * kOp, kOffRaw = kOffOp + kOps * kOp, kSmem = kOffRaw + kRaws * kRaw;
+    static constexpr int kQ = kM * D * 2, kOp = kKeys * D * 2; /* a tile of q; of keys or values */
+    static constexpr int kRaw = kKeys * (D / 2 + D / 16);      /* its codes and scales           */
+    static constexpr int kOps = D == 64 ? 12 : 8, kRaws = D == 64 ? 12 : 6;
+    static constexpr uint32_t kBufs = D == 64 ? 6 : 4, kColO = kBufs * kKeys; /* of S, before O in TMEM */
+    static constexpr int kOffOp = 2 * kQ, kOffRaw = kOffOp + kOps * kOp, kSmem = kOffRaw + kRaws * kRaw;
     static_assert(kSmem <= 226 * 1024, "shared memory");
 };
 
@@ -47,7 +47,7 @@ template <int D>
 constexpr uint32_t kIdescPV = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(D >> 3) << 17) | (1u << 16);
 
 struct Bars {
-    uint64_t raw_full[6], raw_empty[6], op_full[6], op_empty[6], s_full[3], p_full[3], o_full[2];
+    uint64_t raw_full[12], raw_empty[12], op_full[12], op_empty[12], s_full[6], p_full[6], o_full[2][2];
     uint32_t tmem;
     int abort, tile[2];
     /* the block's rows for the epilogue: kept here, their registers are the softmax's */
@@ -99,11 +99,6 @@ __device__ __forceinline__ void st32(uint32_t t, const uint32_t *v) {
         "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
         R8(v, 0), R8(v, 8), R8(v, 16), R8(v, 24)
         : "memory");
-}
-__device__ __forceinline__ void st16(uint32_t t, const uint32_t *v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
-                 R8(v, 0), R8(v, 8)
-                 : "memory");
 }
 __device__ __forceinline__ void max3(float &m, uint32_t a, uint32_t b) {
     asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
@@ -171,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             lfm_mbar_init(&bars.s_full[i], 1);
             lfm_mbar_init(&bars.p_full[i], 4);
         }
-        for (int i = 0; i < 2; ++i) lfm_mbar_init(&bars.o_full[i], 1);
+        for (int i = 0; i < 4; ++i) lfm_mbar_init(&bars.o_full[i >> 1][i & 1], 1);
         bars.abort = 0;
         lfm_fence_mbar_init();
     }
@@ -213,40 +208,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         bars.rows = rows;
         bars.kvh = kvh;
     }
-    if (warp == 12) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
-                     "r"(kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        fence_before();
-    }
-    /* q: a thread 8 values 4 w .. 4 w + 3 and 32 + 4 w .. of a span, one chunk */
-    for (uint32_t i = tid; i < kRows * (D / 16); i += kThreads) {
-        /* two words a step: values 8 v .. + 7 and 32 + 8 v .. + 7 of the span make chunks 2 v and 2 v + 1 */
-        const uint32_t r = i % kRows, c = i / kRows, s = c >> 2, v = c & 3;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (r < rows) {
-            const size_t at = row_at(r, A.q_stride) + 64 * s + 8 * v;
-            const bool neg = A.scale < 0.0f;
-            lfm_load_q(A, at, neg, x);
-            lfm_load_q(A, at + 32, neg, y);
-        }
-        uint8_t *to = sm + (r / kM) * C::kOp + (8 * s + 2 * v) * kChunk + (r % kM) * 16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<uint4 *>(to + h * kChunk) =
-                make_uint4(lfm_pack2(x[4 * h], y[4 * h], __half()), lfm_pack2(x[4 * h + 1], y[4 * h + 1], __half()),
-                           lfm_pack2(x[4 * h + 2], y[4 * h + 2], __half()), lfm_pack2(x[4 * h + 3], y[4 * h + 3], __half()));
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-    fence_after();
-    const uint32_t tmem = bars.tmem, smem = lfm_smem_u32(sm);
+    const uint32_t smem = lfm_smem_u32(sm);
     bool ok = true;
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 152;"); /* 256 x 152 + 256 x 104 = 512 x 128 */
         const uint32_t h = warp >> 2, r = h * kM + (warp & 3) * 32 + lane;
+        {
+            /* this thread's row of q: values 8 v .. + 7 and 32 + 8 v .. + 7 of a span make chunks 2 v and 2 v + 1 */
+            const size_t at = r < rows ? row_at(r, A.q_stride) : 0;
+            uint8_t *to = sm + h * C::kQ + (r % kM) * 16;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (r < rows) {
+                    lfm_load_q(A, at + 64 * (c >> 2) + 8 * (c & 3), A.scale < 0.0f, x);
+                    lfm_load_q(A, at + 64 * (c >> 2) + 8 * (c & 3) + 32, A.scale < 0.0f, y);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    *reinterpret_cast<uint4 *>(to + (2 * c + k) * kChunkQ) =
+                        make_uint4(lfm_pack2(x[4 * k], y[4 * k], __half()), lfm_pack2(x[4 * k + 1], y[4 * k + 1], __half()),
+                                   lfm_pack2(x[4 * k + 2], y[4 * k + 2], __half()), lfm_pack2(x[4 * k + 3], y[4 * k + 3], __half()));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        fence_before();
+        lfm_bar_sync(1, 288); /* with the MMA warp: q is there, and TMEM */
+        fence_after();
+        const uint32_t tmem = bars.tmem;
         const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
         const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
         const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
@@ -266,6 +256,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             inside1 = (int)(max((int64_t)0, e_all - base) / kKeys);
         }
         const uint64_t sc2 = pk2(__float_as_uint(sc), __float_as_uint(sc));
+        /* O holds the products of block j.  A barrier's parity tells two phases apart: with the scores of block
+         * j + 1 the products of j - 2 are done (kBufs <= 6), so those of j and j - 1 take a barrier each, in turn */
+        auto products = [&](uint32_t j) {
+            return __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h][j & 1], (j >> 1) & 1, abort, A.err));
+        };
         float m = LFM_NO_KEY;
         uint64_t l2 = 0;
         for (uint32_t j = 0; j < n; ++j) {
@@ -276,43 +271,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             fence_after();
             const bool masked = (int)j < inside0 || (int)j >= inside1;
             const int from = lo - (int)j * kKeys, to = hi - (int)j * kKeys;
-            auto mask = [&](uint32_t *x, int c) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (c + i < from || c + i >= to) x[i] = 0xFF800000u;
-            };
-            uint32_t x[2][32]; /* S is read twice, 32 columns at a time: the registers of all 128 are not there */
+            uint32_t x[kKeys];
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            ld32(tS, x);
+            ld32(tS + 32, x + 32);
+            wait_ld();
+            tie32(x);
+            tie32(x + 32);
+            if (kCap) { /* tanh(x) = 1 - 2 / (1 + e^2x) */
 #pragma unroll
-            for (int c = 0; c < kKeys; c += 64) {
-                ld32(tS + c, x[0]);
-                ld32(tS + c + 32, x[1]);
-                wait_ld();
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    tie32(x[k]);
-                    if (masked) mask(x[k], c + 32 * k);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        max3(mx[0], x[k][i], x[k][i + 1]);
-                        max3(mx[1], x[k][i + 2], x[k][i + 3]);
-                        max3(mx[2], x[k][i + 4], x[k][i + 5]);
-                        max3(mx[3], x[k][i + 6], x[k][i + 7]);
-                    }
-                }
+                for (int i = 0; i < kKeys; ++i)
+                    x[i] = __float_as_uint(__fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(__uint_as_float(x[i]) * capz)), 1.0f));
             }
-            ld32(tS, x[0]);
-            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            /* tanh(x) = 1 - 2 / (1 + e^2x), which keeps the order */
-            auto cap = [&](float z) { return __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(z * capz)), 1.0f); };
-            if (kCap) top = top > -INFINITY ? cap(top) : top;
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < kKeys; ++i)
+                    if (i < from || i >= to) x[i] = 0xFF800000u;
+            }
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 8) {
+                max3(mx[0], x[i], x[i + 1]);
+                max3(mx[1], x[i + 2], x[i + 3]);
+                max3(mx[2], x[i + 4], x[i + 5]);
+                max3(mx[3], x[i + 6], x[i + 7]);
+            }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             if (__any_sync(LFM_FULL_MASK, __fmaf_rn(top, sc, -m) > 8.0f)) {
                 const float nm = fmaxf(m, top * sc), f = lfm_ex2(m - nm);
                 const uint64_t f2 = pk2(__float_as_uint(f), __float_as_uint(f));
                 m = nm;
                 l2 = mul2(l2, f2);
                 if (j) { /* the products of the block before are in O first */
-                    ok = __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h], (j - 1) & 1, abort, A.err));
+                    ok = products(j - 1);
                     if (!ok) break;
                     fence_after();
 #pragma unroll
@@ -333,42 +323,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             }
             const uint64_t nm2 = pk2(__float_as_uint(-m), __float_as_uint(-m));
             uint64_t la = 0;
+            /* each operation on all before the next one: the exponentials' latency hides behind one another */
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t *y = x[c & 1];
-                wait_ld();
-                tie32(y);
-                if (c < 3) ld32(tS + 32 * c + 32, x[(c + 1) & 1]);
-                if (kCap) {
+            for (int i = 0; i < kKeys; i += 2) {
+                const uint64_t z = fma2(pk2(x[i], x[i + 1]), sc2, nm2);
+                x[i] = (uint32_t)z;
+                x[i + 1] = (uint32_t)(z >> 32);
+            }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(cap(__uint_as_float(y[i])));
-                }
-                if (masked) mask(y, 32 * c);
-                /* each operation on all before the next one: the exponentials' latency hides behind one another */
+            for (int i = 0; i < kKeys; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[i]));
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const uint64_t z = fma2(pk2(y[i], y[i + 1]), sc2, nm2);
-                    y[i] = (uint32_t)z;
-                    y[i + 1] = (uint32_t)(z >> 32);
-                }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(y[i]));
-                uint32_t pk[16];
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    if (i & 2) la = add2(la, pk2(y[i], y[i + 1]));
-                    else l2 = add2(l2, pk2(y[i], y[i + 1]));
-                    pk[i / 2] = lfm_pack2(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), __half());
-                }
-                st16(tS + 16 * c, pk); /* over columns that are read by now */
+            for (int i = 0; i < kKeys; i += 2) {
+                if (i & 2) la = add2(la, pk2(x[i], x[i + 1]));
+                else l2 = add2(l2, pk2(x[i], x[i + 1]));
+                x[i / 2] = lfm_pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __half());
             }
             l2 = add2(l2, la);
+            st32(tS, x);
             wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) lfm_mbar_arrive(&bars.p_full[buf]);
         }
-        if (ok) ok = __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h], (n - 1) & 1, abort, A.err));
+        /* the barrier of the last products may still be two of its phases back: the one before goes first */
+        if (ok && n > 1) ok = products(n - 2);
+        if (ok) ok = products(n - 1);
         if (ok) {
             fence_after();
             const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
@@ -400,12 +379,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        const uint32_t sub = min(A.kv.page_tokens, (uint32_t)kKeys), piece = sub * (D / 2 + D / 16);
         if (warp < 12) {
             /* codes -> values */
             const LfmNib nib;
-            const uint32_t key = (warp - 8) * 32 + lane, in = key & (sub - 1);
-            const uint32_t codes = (key / sub) * piece + in * (D / 2), scales = (key / sub) * piece + sub * (D / 2) + in * (D / 16);
+            /* two threads a key: halves of its words */
+            const uint32_t key = (warp & 1) * 32 + lane, half = (warp >> 1) & 1;
+            const uint32_t codes = key * (D / 2) + half * (D / 4), scales = kKeys * (D / 2) + key * (D / 16) + (D == 64 ? 0 : 4 * half);
             for (uint32_t u = 0; u < 2 * n; ++u) {
                 const uint32_t rs = u % C::kRaws, os = u % C::kOps;
                 bool w = wait(&bars.raw_full[rs], (u / C::kRaws) & 1, abort, A.err);
@@ -413,19 +392,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 ok = __all_sync(LFM_FULL_MASK, w);
                 if (!ok) break;
                 const uint8_t *raw = sm + C::kOffRaw + rs * C::kRaw;
-                uint8_t *to = sm + C::kOffOp + os * C::kOp + key * 16;
+                uint8_t *to = sm + C::kOffOp + os * C::kOp + key * 16 + half * (D / 16) * kChunk;
+                /* a slot that holds no token may hold anything: zero, for V */
                 const bool held = (blk0 + (u >> 1)) * kKeys + key < len;
+                const uint32_t d = held ? *reinterpret_cast<const uint32_t *>(raw + scales) : 0u;
 #pragma unroll
-                for (int s = 0; s < D / 64; ++s) {
-                    const uint4 a = *reinterpret_cast<const uint4 *>(raw + codes + 32 * s);
-                    const uint4 c = *reinterpret_cast<const uint4 *>(raw + codes + 32 * s + 16);
-                    /* a slot that holds no token may hold anything: zero, for V */
-                    const uint32_t d = held ? *reinterpret_cast<const uint32_t *>(raw + scales + 4 * s) : 0u;
-                    const uint32_t x[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+                for (int c = 0; c < D / 64; ++c) {
+                    const uint4 a = *reinterpret_cast<const uint4 *>(raw + codes + 16 * c);
+                    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
+                    for (int k = 0; k < 4; ++k) {
                         const uint32_t y = x[k] >> 8;
-                        *reinterpret_cast<uint4 *>(to + (8 * s + k) * kChunk) =
+                        *reinterpret_cast<uint4 *>(to + (4 * c + k) * kChunk) =
                             make_uint4(lfm_hmul2(lfm_hsub2(nib.lo(x[k]), LFM_NIB0_OFF), d),
                                        lfm_hmul2(lfm_hsub2(nib.hi(x[k]), LFM_NIB1_OFF), d),
                                        lfm_hmul2(lfm_hsub2(nib.lo(y), LFM_NIB0_OFF), d),
@@ -440,6 +418,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 }
             }
         } else if (warp == 12) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
+                         "r"(kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+            fence_before();
+            lfm_bar_sync(1, 288);
+            fence_after();
             /* The whole warp walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all
              * columns are ours) then stay in uniform registers.  From a branch of lane 0 alone they take moves
              * through the pipe that the softmax warps' exponentials fill, and an MMA waits 350 cycles for its turn */
@@ -449,15 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 return w;
             };
             /* step q = 2 * block + tile; i = q modulo the unrolling, known to the compiler with all that it gives */
-            constexpr uint32_t kUn = C::kOps; /* a multiple of 2 and of kBufs */
-            static_assert(kUn % 2 == 0 && kUn % C::kBufs == 0, "unrolling");
+            constexpr uint32_t kUn = C::kOps; /* a multiple of 4 and of kBufs */
+            static_assert(kUn % 4 == 0 && kUn % C::kBufs == 0, "unrolling");
             auto op = [&](uint32_t i) { return smem + C::kOffOp + i * C::kOp; };
             auto qk = [&](uint32_t i) {
                 const uint32_t h = i & 1, buf = i % C::kBufs, k0 = i & ~1u;
-                const uint64_t qd = sdesc(smem + h * C::kOp, kChunk, 128), kd = sdesc(op(k0), kChunk, 128);
+                const uint64_t qd = sdesc(smem + h * C::kQ, kChunkQ, 128), kd = sdesc(op(k0), kChunk, 128);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(buf * kColS, qd + k * (2 * kChunk >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
+                    mma_ss(buf * kColS, qd + k * (2 * kChunkQ >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
                 commit(&bars.s_full[buf]);
                 if (h) commit(&bars.op_empty[k0]);
             };
@@ -467,10 +452,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k)
                     mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
-                commit(&bars.o_full[h]);
+                commit(&bars.o_full[h][(i >> 1) & 1]);
                 if (h) commit(&bars.op_empty[v0]);
             };
-            ok = tmem == 0;
+            ok = bars.tmem == 0;
 #pragma unroll
             for (uint32_t q = 0; q < C::kBufs; ++q) {
                 if (!ok || q >= 2 * n) break;
@@ -494,23 +479,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 }
             }
         } else if (warp == 13) {
-            /* pages: a lane a piece of the block, K then V */
+            /* a lane the codes or the scales of a page's tokens in the block, K then V: [codes][scales] of all keys */
+            const uint32_t P = A.kv.page_tokens, sub = min(P, (uint32_t)kKeys), piece = lane >> 1, part = lane & 1;
+            const uint32_t per = part ? D / 16 : D / 2, bytes = sub * per;
+            const uint32_t to = C::kOffRaw + (part ? kKeys * (D / 2) : 0) + piece * bytes;
             for (uint32_t j = 0; j < n; ++j) {
-                const int64_t key = (blk0 + j) * kKeys + (int64_t)lane * sub;
+                const int64_t key = (blk0 + j) * kKeys + (int64_t)piece * sub;
                 const uint8_t *page = nullptr;
-                if (lane * sub < kKeys && key < len) page = lfm_page(A.kv, A.bt, b, key, kvh, A.err);
-                const uint32_t bytes = __popc(__ballot_sync(LFM_FULL_MASK, page != nullptr)) * piece;
+                if (piece * sub < kKeys && key < len) page = lfm_page(A.kv, A.bt, b, key, kvh, A.err);
+                const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, page ? bytes : 0u);
+                const uint32_t in = ((uint32_t)key & (P - 1)) * per + (part ? A.kv.codes : 0);
 #pragma unroll
                 for (uint32_t k = 0; k < 2; ++k) {
                     const uint32_t u = 2 * j + k, rs = u % C::kRaws;
                     ok = ok && (u < (uint32_t)C::kRaws || wait(&bars.raw_empty[rs], ((u / C::kRaws) & 1) ^ 1, abort, A.err));
                     ok = __all_sync(LFM_FULL_MASK, ok);
                     if (!ok) break;
-                    if (lane == 0) lfm_mbar_arrive_tx(&bars.raw_full[rs], bytes);
+                    if (lane == 0) lfm_mbar_arrive_tx(&bars.raw_full[rs], all);
                     __syncwarp();
                     if (page)
-                        lfm_bulk_g2s_plain(sm + C::kOffRaw + rs * C::kRaw + lane * piece, page + (k ? A.kv.half : 0), piece,
-                                           &bars.raw_full[rs]);
+                        lfm_bulk_g2s_plain(sm + to + rs * C::kRaw, page + in + (k ? A.kv.half : 0), bytes, &bars.raw_full[rs]);
                 }
                 if (!ok) break;
             }
@@ -528,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
     if (warp == 12) {
         __syncwarp();
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars.tmem), "r"(kTmemCols));
     }
 }
 
