@@ -428,53 +428,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             /* The whole warp walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all
              * columns are ours) then stay in uniform registers.  From a branch of lane 0 alone they take moves
              * through the pipe that the softmax warps' exponentials fill, and an MMA waits 350 cycles for its turn */
-            auto full = [&](uint32_t u, uint32_t slot) {
-                const bool w = __all_sync(LFM_FULL_MASK, wait(&bars.op_full[slot], (u / C::kOps) & 1, abort, A.err));
+            auto full = [&](uint32_t u) {
+                const bool w = __all_sync(LFM_FULL_MASK, wait(&bars.op_full[u % C::kOps], (u / C::kOps) & 1, abort, A.err));
                 fence_after();
                 return w;
             };
-            /* step q = 2 * block + tile; i = q modulo the unrolling, known to the compiler with all that it gives */
-            constexpr uint32_t kUn = C::kOps; /* a multiple of 4 and of kBufs */
-            static_assert(kUn % 4 == 0 && kUn % C::kBufs == 0, "unrolling");
-            auto op = [&](uint32_t i) { return smem + C::kOffOp + i * C::kOp; };
-            auto qk = [&](uint32_t i) {
-                const uint32_t h = i & 1, buf = i % C::kBufs, k0 = i & ~1u;
-                const uint64_t qd = sdesc(smem + h * C::kQ, kChunkQ, 128), kd = sdesc(op(k0), kChunk, 128);
+            const uint64_t kd0 = sdesc(smem + C::kOffOp, kChunk, 128), vd0 = sdesc(smem + C::kOffOp, 128, kChunk);
+            /* block j, tile h: one of the two is known to the compiler; operands u = 2 j (keys), 2 j + 1 (values) */
+            auto qk = [&](uint32_t j, uint32_t h) {
+                const uint32_t buf = (2 * j + h) % C::kBufs, slot = 2 * j % C::kOps;
+                const uint64_t qd = sdesc(smem + h * C::kQ, kChunkQ, 128), kd = kd0 + slot * (C::kOp >> 4);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
                     mma_ss(buf * kColS, qd + k * (2 * kChunkQ >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
                 commit(&bars.s_full[buf]);
-                if (h) commit(&bars.op_empty[k0]);
+                if (h) commit(&bars.op_empty[slot]);
             };
-            auto pv = [&](uint32_t i, bool first) {
-                const uint32_t h = i & 1, buf = i % C::kBufs, v0 = i | 1u;
-                const uint64_t vd = sdesc(op(v0), 128, kChunk);
+            auto pv = [&](uint32_t j, uint32_t h) {
+                const uint32_t buf = (2 * j + h) % C::kBufs, slot = (2 * j + 1) % C::kOps;
+                const uint64_t vd = vd0 + slot * (C::kOp >> 4);
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k)
-                    mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
-                commit(&bars.o_full[h][(i >> 1) & 1]);
-                if (h) commit(&bars.op_empty[v0]);
+                    mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, j > 0 || k > 0);
+                commit(&bars.o_full[h][j & 1]);
+                if (h) commit(&bars.op_empty[slot]);
             };
+            constexpr uint32_t kAhead = C::kBufs / 2; /* blocks whose scores are asked for ahead */
             ok = bars.tmem == 0;
-#pragma unroll
-            for (uint32_t q = 0; q < C::kBufs; ++q) {
-                if (!ok || q >= 2 * n) break;
-                if (!(q & 1)) ok = full(q, q);
-                if (ok && elect()) qk(q);
+            for (uint32_t j = 0; j < kAhead && j < n && ok; ++j) {
+                ok = full(2 * j);
+                if (ok && elect()) {
+                    qk(j, 0);
+                    qk(j, 1);
+                }
             }
-            for (uint32_t q0 = 0; q0 < 2 * n && ok; q0 += kUn) {
+            for (uint32_t j = 0; j < n && ok; ++j) {
+                const bool more = j + kAhead < n;
+                ok = full(2 * j + 1) && (!more || full(2 * (j + kAhead)));
 #pragma unroll
-                for (uint32_t i = 0; i < kUn; ++i) {
-                    const uint32_t q = q0 + i, buf = i % C::kBufs, next = (i + C::kBufs) % kUn;
-                    if (!ok || q >= 2 * n) break;
-                    ok = __all_sync(LFM_FULL_MASK, wait(&bars.p_full[buf], (q / C::kBufs) & 1, abort, A.err)) &&
-                         ((i & 1) || full(q | 1u, i | 1u));
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const uint32_t q = 2 * j + h;
+                    ok = ok && __all_sync(LFM_FULL_MASK, wait(&bars.p_full[q % C::kBufs], (q / C::kBufs) & 1, abort, A.err));
                     if (!ok) break;
                     fence_after();
-                    if (elect()) pv(i, q < 2);
-                    if (q + C::kBufs < 2 * n) {
-                        if (!(next & 1)) ok = full(q + C::kBufs, next);
-                        if (ok && elect()) qk(next);
+                    if (elect()) {
+                        pv(j, h);
+                        if (more) qk(j + kAhead, h);
                     }
                 }
             }
