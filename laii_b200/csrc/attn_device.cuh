@@ -189,16 +189,20 @@ __device__ __forceinline__ float lfm_rcp(float x) {
 
 #define LFM_NO_KEY -1e30f /* the running reference of a row that has seen no key */
 
-/* Eight values of a q row at `at`, saturated to fp16's finite range (NaN stays), negated for a negative scale. */
-__device__ __forceinline__ void lfm_load_q(const AttnArgs &A, size_t at, bool neg, float (&v)[8]) {
-    if (A.type == 0) lfm_load<8>(static_cast<const float *>(A.q) + at, v);
-    else if (A.type == 1) lfm_load<8>(static_cast<const __half *>(A.q) + at, v);
-    else lfm_load<8>(static_cast<const __nv_bfloat16 *>(A.q) + at, v);
+/* Eight values of q within fp16's finite range (NaN stays), negated for a negative scale. */
+__device__ __forceinline__ void lfm_fit_q(bool neg, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float x = neg ? -v[i] : v[i];
         v[i] = x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
     }
+}
+/* Eight values of a q row at `at`, so fitted. */
+__device__ __forceinline__ void lfm_load_q(const AttnArgs &A, size_t at, bool neg, float (&v)[8]) {
+    if (A.type == 0) lfm_load<8>(static_cast<const float *>(A.q) + at, v);
+    else if (A.type == 1) lfm_load<8>(static_cast<const __half *>(A.q) + at, v);
+    else lfm_load<8>(static_cast<const __nv_bfloat16 *>(A.q) + at, v);
+    lfm_fit_q(neg, v);
 }
 
 /* Keys [lo, hi) that row r (token, head of the group) of a sequence of n_q tokens behind len cached ones sees. */

@@ -23,6 +23,8 @@
  * O in TMEM is scaled by 1 / sum at the end.  Rows that end early in a block
  * and slots that hold no token are masked in S; values of such slots are zero.
  */
+#include <type_traits>
+
 #include "attn_device.cuh"
 
 namespace {
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         }
         for (int i = 0; i < C::kOps; ++i) {
             lfm_mbar_init(&bars.op_full[i], 4);
-            lfm_mbar_init(&bars.op_empty[i], 1);
+            lfm_mbar_init(&bars.op_empty[i], 2);
         }
         for (uint32_t i = 0; i < C::kBufs; ++i) {
             lfm_mbar_init(&bars.s_full[i], 1);
@@ -218,23 +220,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             /* this thread's row of q: values 8 v .. + 7 and 32 + 8 v .. + 7 of a span make chunks 2 v and 2 v + 1 */
             const size_t at = r < rows ? row_at(r, A.q_stride) : 0;
             uint8_t *to = sm + h * C::kQ + (r % kM) * 16;
+            const bool neg = A.scale < 0.0f;
+            auto load = [&](const auto *q) { /* the type is told apart once, so the loads are under way together */
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (r < rows) {
-                    lfm_load_q(A, at + 64 * (c >> 2) + 8 * (c & 3), A.scale < 0.0f, x);
-                    lfm_load_q(A, at + 64 * (c >> 2) + 8 * (c & 3) + 32, A.scale < 0.0f, y);
+                for (int c = 0; c < D / 16; ++c) {
+                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (r < rows) {
+                        lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3), x);
+                        lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3) + 32, y);
+                    }
+                    lfm_fit_q(neg, x);
+                    lfm_fit_q(neg, y);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        *reinterpret_cast<uint4 *>(to + (2 * c + k) * kChunkQ) =
+                            make_uint4(lfm_pack2(x[4 * k], y[4 * k], __half()), lfm_pack2(x[4 * k + 1], y[4 * k + 1], __half()),
+                                       lfm_pack2(x[4 * k + 2], y[4 * k + 2], __half()), lfm_pack2(x[4 * k + 3], y[4 * k + 3], __half()));
                 }
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    *reinterpret_cast<uint4 *>(to + (2 * c + k) * kChunkQ) =
-                        make_uint4(lfm_pack2(x[4 * k], y[4 * k], __half()), lfm_pack2(x[4 * k + 1], y[4 * k + 1], __half()),
-                                   lfm_pack2(x[4 * k + 2], y[4 * k + 2], __half()), lfm_pack2(x[4 * k + 3], y[4 * k + 3], __half()));
-            }
+            };
+            if (A.type == 0) load(static_cast<const float *>(A.q));
+            else if (A.type == 1) load(static_cast<const __half *>(A.q));
+            else load(static_cast<const __nv_bfloat16 *>(A.q));
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         fence_before();
-        lfm_bar_sync(1, 288); /* with the MMA warp: q is there, and TMEM */
+        lfm_bar_sync(1, 320); /* with the MMA warps: q is there, and TMEM */
         fence_after();
         const uint32_t tmem = bars.tmem;
         const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
@@ -417,66 +427,69 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                     lfm_mbar_arrive(&bars.raw_empty[rs]);
                 }
             }
-        } else if (warp == 12) {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
-                         "r"(kTmemCols)
-                         : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else if (warp == 12 || warp == 14) {
+            if (warp == 12) {
+                asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
+                             "r"(kTmemCols)
+                             : "memory");
+                asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+            }
             fence_before();
-            lfm_bar_sync(1, 288);
+            lfm_bar_sync(1, 320);
             fence_after();
-            /* The whole warp walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all
-             * columns are ours) then stay in uniform registers.  From a branch of lane 0 alone they take moves
-             * through the pipe that the softmax warps' exponentials fill, and an MMA waits 350 cycles for its turn */
+            /* A warp a tile: what one spends on barriers between its MMAs is the other's tensor time.  The whole warp
+             * walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all columns are ours) then
+             * stay in uniform registers.  From a branch of lane 0 alone they take moves through the pipe that the
+             * softmax warps' exponentials fill, and an MMA waits 350 cycles for its turn */
             auto full = [&](uint32_t u) {
                 const bool w = __all_sync(LFM_FULL_MASK, wait(&bars.op_full[u % C::kOps], (u / C::kOps) & 1, abort, A.err));
                 fence_after();
                 return w;
             };
             const uint64_t kd0 = sdesc(smem + C::kOffOp, kChunk, 128), vd0 = sdesc(smem + C::kOffOp, 128, kChunk);
-            /* block j, tile h: one of the two is known to the compiler; operands u = 2 j (keys), 2 j + 1 (values) */
-            auto qk = [&](uint32_t j, uint32_t h) {
-                const uint32_t buf = (2 * j + h) % C::kBufs, slot = 2 * j % C::kOps;
-                const uint64_t qd = sdesc(smem + h * C::kQ, kChunkQ, 128), kd = kd0 + slot * (C::kOp >> 4);
+            auto walk = [&](auto tile) {
+                constexpr uint32_t h = decltype(tile)::value;
+                const uint64_t qd = sdesc(smem + h * C::kQ, kChunkQ, 128);
+                /* keys of block j are operand 2 j, its values 2 j + 1 */
+                auto qk = [&](uint32_t j) {
+                    const uint32_t buf = (2 * j + h) % C::kBufs, slot = 2 * j % C::kOps;
+                    const uint64_t kd = kd0 + slot * (C::kOp >> 4);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                    mma_ss(buf * kColS, qd + k * (2 * kChunkQ >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
-                commit(&bars.s_full[buf]);
-                if (h) commit(&bars.op_empty[slot]);
-            };
-            auto pv = [&](uint32_t j, uint32_t h) {
-                const uint32_t buf = (2 * j + h) % C::kBufs, slot = (2 * j + 1) % C::kOps;
-                const uint64_t vd = vd0 + slot * (C::kOp >> 4);
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(buf * kColS, qd + k * (2 * kChunkQ >> 4), kd + k * (2 * kChunk >> 4), kIdescQK, k > 0);
+                    commit(&bars.s_full[buf]);
+                    commit(&bars.op_empty[slot]);
+                };
+                auto pv = [&](uint32_t j) {
+                    const uint32_t buf = (2 * j + h) % C::kBufs, slot = (2 * j + 1) % C::kOps;
+                    const uint64_t vd = vd0 + slot * (C::kOp >> 4);
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, j > 0 || k > 0);
-                commit(&bars.o_full[h][j & 1]);
-                if (h) commit(&bars.op_empty[slot]);
-            };
-            constexpr uint32_t kAhead = C::kBufs / 2; /* blocks whose scores are asked for ahead */
-            ok = bars.tmem == 0;
-            for (uint32_t j = 0; j < kAhead && j < n && ok; ++j) {
-                ok = full(2 * j);
-                if (ok && elect()) {
-                    qk(j, 0);
-                    qk(j, 1);
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, j > 0 || k > 0);
+                    commit(&bars.o_full[h][j & 1]);
+                    commit(&bars.op_empty[slot]);
+                };
+                constexpr uint32_t kAhead = C::kBufs / 2; /* blocks whose scores are asked for ahead */
+                ok = bars.tmem == 0;
+                for (uint32_t j = 0; j < kAhead && j < n && ok; ++j) {
+                    ok = full(2 * j);
+                    if (ok && elect()) qk(j);
                 }
-            }
-            for (uint32_t j = 0; j < n && ok; ++j) {
-                const bool more = j + kAhead < n;
-                ok = full(2 * j + 1) && (!more || full(2 * (j + kAhead)));
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
+                for (uint32_t j = 0; j < n && ok; ++j) {
                     const uint32_t q = 2 * j + h;
-                    ok = ok && __all_sync(LFM_FULL_MASK, wait(&bars.p_full[q % C::kBufs], (q / C::kBufs) & 1, abort, A.err));
+                    const bool more = j + kAhead < n;
+                    ok = full(2 * j + 1) && (!more || full(2 * (j + kAhead))) &&
+                         __all_sync(LFM_FULL_MASK, wait(&bars.p_full[q % C::kBufs], (q / C::kBufs) & 1, abort, A.err));
                     if (!ok) break;
                     fence_after();
                     if (elect()) {
-                        pv(j, h);
-                        if (more) qk(j + kAhead, h);
+                        pv(j);
+                        if (more) qk(j + kAhead);
                     }
                 }
-            }
+            };
+            if (warp == 12) walk(std::integral_constant<uint32_t, 0>());
+            else walk(std::integral_constant<uint32_t, 1>());
         } else if (warp == 13) {
             /* a lane the codes or the scales of a page's tokens in the block, K then V: [codes][scales] of all keys */
             const uint32_t P = A.kv.page_tokens, sub = min(P, (uint32_t)kKeys), piece = lane >> 1, part = lane & 1;
