@@ -86,17 +86,6 @@ __device__ __forceinline__ void lfm_store(T *p, const float (&v)[N]) {
     else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
 }
 
-/* The whole block: the sequence that owns row `tok`, or -1 (padding, or
- * offsets that do not contain it).  s_seq: one shared int. */
-__device__ __forceinline__ int lfm_find_seq(const BatchDev &bt, uint32_t tok, int *s_seq) {
-    if (threadIdx.x == 0) *s_seq = -1;
-    __syncthreads();
-    for (uint32_t b = threadIdx.x; b < bt.n_seqs; b += blockDim.x)
-        if ((int64_t)bt.q_start[b] <= (int64_t)tok && (int64_t)tok < (int64_t)bt.q_start[b + 1]) *s_seq = (int)b;
-    __syncthreads();
-    return *s_seq;
-}
-
 /* Start of kv head `head` in the page of token `pos` of sequence b; nullptr
  * (and the error bit) where the table or the pool does not reach. */
 __device__ __forceinline__ uint8_t *lfm_page(const KvDev &kv, const BatchDev &bt, int b, int64_t pos, uint32_t head,

@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const float *x, const void
     const size_t col = 256u * warp + 4u * lane, at = (size_t)blockIdx.x * D + col;
     float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f}, v[8];
     lfm_pdl_wait();
+    lfm_pdl_launch_dependents();
     {
         float a[4], b[4];
         lfm_load<4>(x + at, a);
@@ -113,6 +114,7 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const float *x, const void
 /* A warp a block: the values d * q. */
 __global__ void __launch_bounds__(256) k_q8k_read(const uint8_t *q8, size_t n_blocks, uint32_t type, void *out) {
     lfm_pdl_wait();
+    lfm_pdl_launch_dependents();
     const size_t b = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const uint32_t lane = threadIdx.x & 31;
     if (b >= n_blocks) return;
