@@ -73,11 +73,13 @@ cudaError_t lfm_launch_q8k_read(const uint8_t *q8, uint32_t rows, uint32_t D, ui
 cudaError_t lfm_launch_kv_append(const AppendArgs &a, uint32_t head_dim, uint32_t type, cudaStream_t s, bool pdl);
 cudaError_t lfm_launch_kv_read(const ReadArgs &a, uint32_t head_dim, uint32_t type, cudaStream_t s, bool pdl);
 /* max_kv_len bounds the blocks launched, scratch holds the parts of split sequences (LFM_ATTN_SCRATCH_BYTES, the leading
- * LFM_ATTN_COUNTS words zero; the kernels leave them zero); *used: whether this call does. */
+ * LFM_ATTN_COUNTS words zero; the kernels leave them zero). */
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
-                            bool *used, cudaStream_t s, bool pdl);
-/* The tensor-core kernel for the sequences of more than `above` rows (token, head of a group). */
-cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, cudaStream_t s, bool pdl);
+                            cudaStream_t s, bool pdl);
+/* The tensor-core kernel for the sequences of more than `above` rows (token, head of a group); count: two words, zero
+ * before and after. */
+cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, int sm_count, uint32_t *count,
+                                 cudaStream_t s, bool pdl);
 #define LFM_ATTN_COUNTS 1024u                                     /* most blocks that share work      */
 #define LFM_ATTN_PARTS_BYTES ((size_t)LFM_ATTN_COUNTS * 2 * 32 * 66 * 4) /* two parts each, 32 x (64 + 2) or 16 x (128 + 2) */
 #define LFM_ATTN_SCRATCH_BYTES (LFM_ATTN_PARTS_BYTES + LFM_ATTN_COUNTS * sizeof(uint32_t))

@@ -640,7 +640,7 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
     uint64_t grid = (uint64_t)sm_count * (head_dim * nt < 128 ? 4 : head_dim * nt == 128 ? 3 : 2);
     const uint64_t work = (B + T * G / (8 * nt)) * a.kv.hkv * ((max_kv_len + keys - 1) / keys + 1);
     if (grid > (work + kWarps - 1) / kWarps) grid = (work + kWarps - 1) / kWarps;
-    if (grid > LFM_ATTN_COUNTS) grid = LFM_ATTN_COUNTS;
+    if (grid > LFM_ATTN_COUNTS - 2) grid = LFM_ATTN_COUNTS - 2;
     RowsPlan p{few, reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + LFM_ATTN_COUNTS * sizeof(uint32_t)),
                static_cast<uint32_t *>(scratch)};
     const dim3 g((uint32_t)grid);
@@ -651,16 +651,13 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
 }
 
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
-                            bool *used, cudaStream_t s, bool pdl) {
+                            cudaStream_t s, bool pdl) {
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group;
-    *used = true;
     /* one sequence, or at most as many tokens as make few rows: one kernel takes all.  As many tokens as sequences
      * are a step of single tokens, whatever the odd sequence holds.  Otherwise each takes its sequences */
     if (rows <= kFewRows || T == B) return lfm_launch_attn_rows(a, head_dim, ~0ull, max_kv_len, sm_count, scratch, s, pdl);
-    if (B == 1) {
-        *used = false;
-        return lfm_launch_attn_tile(a, head_dim, 0, s, pdl);
-    }
-    const cudaError_t e = lfm_launch_attn_tile(a, head_dim, kFewRows, s, pdl);
+    uint32_t *count = static_cast<uint32_t *>(scratch) + LFM_ATTN_COUNTS - 2;
+    if (B == 1) return lfm_launch_attn_tile(a, head_dim, 0, sm_count, count, s, pdl);
+    const cudaError_t e = lfm_launch_attn_tile(a, head_dim, kFewRows, sm_count, count, s, pdl);
     return e != cudaSuccess ? e : lfm_launch_attn_rows(a, head_dim, kFewRows, max_kv_len, sm_count, scratch, s, pdl);
 }

@@ -20,6 +20,9 @@
  *   2 x 4 warps  softmax, a thread a row: no exchange between threads.  The
  *             running reference m only moves when a score passes it by 2^8
  *             (p <= 256 in fp16); then the thread scales its row of O in TMEM
+ * The blocks are persistent, one an SM, and take the tiles from a counter, the
+ * longest first: loader and dequantisation run ahead into the next tile while
+ * the softmax warps finish one.
  * O in TMEM is scaled by 1 / sum at the end.  Rows that end early in a block
  * and slots that hold no token are masked in S; values of such slots are zero.
  */
@@ -48,13 +51,18 @@ constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32
 template <int D>
 constexpr uint32_t kIdescPV = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(D >> 3) << 17) | (1u << 16);
 
+/* 256 rows of a kv head: rows row0 .. of sequence b, key blocks blk0 .. + n. */
+struct Job {
+    int64_t q0, n_q, len, blk0;
+    uint32_t row0, rows, kvh, n;
+    int b; /* -1: no more */
+};
 struct Bars {
     uint64_t raw_full[12], raw_empty[12], op_full[12], op_empty[12], s_full[6], p_full[6], o_full[2][2];
+    uint64_t q_full[2], job_full[2], job_empty[2];
     uint32_t tmem;
     int abort, tile[2];
-    /* the block's rows for the epilogue: kept here, their registers are the softmax's */
-    long long q0;
-    uint32_t row0, rows, kvh;
+    Job job[2]; /* the one at work and the next */
 };
 
 /* No swizzle, version 1: start, leading and stride byte offsets. */
@@ -162,12 +170,11 @@ __device__ __forceinline__ bool test(uint64_t *bar, uint32_t parity) {
 }
 
 template <int D, bool kCap>
-__global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t above) {
+__global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t above, uint32_t tiles, uint32_t *count) {
     using C = Cfg<D>;
     extern __shared__ __align__(1024) uint8_t sm[];
     __shared__ Bars bars;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.group;
-    const uint32_t kvh = blockIdx.x % A.kv.hkv, tiles = gridDim.x / A.kv.hkv;
     volatile int *abort = &bars.abort;
     if (tid == 0) {
         for (int i = 0; i < C::kRaws; ++i) {
@@ -183,63 +190,73 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             lfm_mbar_init(&bars.p_full[i], 4);
         }
         for (int i = 0; i < 4; ++i) lfm_mbar_init(&bars.o_full[i >> 1][i & 1], 1);
+        for (int i = 0; i < 2; ++i) {
+            lfm_mbar_init(&bars.q_full[i], 4);
+            lfm_mbar_init(&bars.job_full[i], 1);
+            lfm_mbar_init(&bars.job_empty[i], 14); /* softmax, dequantisation and MMA warps */
+        }
         bars.abort = 0;
         lfm_fence_mbar_init();
     }
-    lfm_pdl_wait();
-    /* the longest walks first: tiles from the last, all heads of one side by side */
-    if (warp == 0) lfm_find_tile(A.bt, G, kRows, 0, above, ~0ull, tiles - 1 - blockIdx.x / A.kv.hkv, bars.tile);
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        fence_before();
+    }
     __syncthreads();
-    const int b = bars.tile[0];
-    if (b < 0) return;
-    const int64_t q0 = A.bt.q_start[b], n_q = (int64_t)A.bt.q_start[b + 1] - q0, len = A.bt.kv_len[b];
-    if (len < 0) {
-        if (tid == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
-        return;
-    }
-    const uint32_t row0 = (uint32_t)bars.tile[1] * kRows;
-    const uint32_t rows = (uint32_t)min((int64_t)kRows, n_q * (int64_t)G - row0); /* of this block, at least 1 */
-    int64_t lo0, hi0, lo1, hi1;
-    lfm_visible(A, n_q, len, row0, lo0, hi0);
-    lfm_visible(A, n_q, len, row0 + rows - 1, lo1, hi1);
-    const int64_t blk0 = lo0 / kKeys;
-    const uint32_t n = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - blk0) : 0; /* key blocks */
-    auto row_at = [&](uint32_t r, size_t stride) {
-        r += row0;
-        return (size_t)(q0 + r / G) * stride + ((size_t)kvh * G + r % G) * D;
-    };
-    if (n == 0) { /* no key for any row */
-        for (uint32_t i = tid; i < rows * (D / 8); i += kThreads) {
-            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            const size_t at = row_at(i / (D / 8), A.out_stride) + i % (D / 8) * 8;
-            if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + at, z);
-            else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + at, z);
-            else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + at, z);
-        }
-        return;
-    }
-    if (tid == 0) {
-        bars.q0 = q0;
-        bars.row0 = row0;
-        bars.rows = rows;
-        bars.kvh = kvh;
-    }
+    fence_after();
+    lfm_pdl_wait();
     const uint32_t smem = lfm_smem_u32(sm);
     bool ok = true;
+    /* job `it`, for all roles but the loader; false at the end */
+    auto take = [&](uint32_t it) {
+        ok = __all_sync(LFM_FULL_MASK, wait(&bars.job_full[it & 1], (it >> 1) & 1, abort, A.err));
+        return ok && bars.job[it & 1].b >= 0;
+    };
+    auto drop = [&](uint32_t it) {
+        __syncwarp();
+        if (lane == 0) lfm_mbar_arrive(&bars.job_empty[it & 1]);
+    };
+    uint32_t base = 0; /* key blocks of the jobs before: ring slots and phases go on from job to job */
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 152;"); /* 256 x 152 + 256 x 104 = 512 x 128 */
-        const uint32_t h = warp >> 2, r = h * kM + (warp & 3) * 32 + lane;
+        const uint32_t h = warp >> 2, r = h * kM + (warp & 3) * 32 + lane, tmem = bars.tmem;
+      for (uint32_t it = 0; take(it); ++it) {
+        const Job &jb = bars.job[it & 1];
+        const uint32_t n = jb.n;
+        /* this thread's row of q or out */
+        auto row_at = [&](size_t stride) {
+            const uint32_t row = jb.row0 + r;
+            return (size_t)(jb.q0 + row / G) * stride + ((size_t)jb.kvh * G + row % G) * D;
+        };
+        if (n == 0) { /* no key for any row */
+            if (r < jb.rows) {
+                const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                const size_t at = row_at(A.out_stride);
+                for (int c = 0; c < D; c += 8) {
+                    if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + at + c, z);
+                    else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + at + c, z);
+                    else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + at + c, z);
+                }
+            }
+            drop(it);
+            continue;
+        }
         {
-            /* this thread's row of q: values 8 v .. + 7 and 32 + 8 v .. + 7 of a span make chunks 2 v and 2 v + 1 */
-            const size_t at = r < rows ? row_at(r, A.q_stride) : 0;
+            /* values 8 v .. + 7 and 32 + 8 v .. + 7 of a span make chunks 2 v and 2 v + 1; the last job's products,
+             * waited for below, are done with the space */
+            const bool on = r < jb.rows;
+            const size_t at = on ? row_at(A.q_stride) : 0;
             uint8_t *to = sm + h * C::kQ + (r % kM) * 16;
             const bool neg = A.scale < 0.0f;
             auto load = [&](const auto *q) { /* the type is told apart once, so the loads are under way together */
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
                     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (r < rows) {
+                    if (on) {
                         lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3), x);
                         lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3) + 32, y);
                     }
@@ -256,11 +273,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             else if (A.type == 1) load(static_cast<const __half *>(A.q));
             else load(static_cast<const __nv_bfloat16 *>(A.q));
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) lfm_mbar_arrive(&bars.q_full[h]);
         }
-        fence_before();
-        lfm_bar_sync(1, 320); /* with the MMA warps: q is there, and TMEM */
-        fence_after();
-        const uint32_t tmem = bars.tmem;
         const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
         const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
         const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
@@ -268,27 +283,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         int lo = 0, hi = 0, inside0 = 0, inside1 = 0;
         {
             int64_t a = 0, e = 0, a_all = 0, e_all = 0, unused;
-            if (r < rows) lfm_visible(A, n_q, len, row0 + r, a, e);
-            if (h * kM < rows) {
-                lfm_visible(A, n_q, len, row0 + h * kM, unused, e_all);
-                lfm_visible(A, n_q, len, row0 + min(rows, (h + 1) * kM) - 1, a_all, unused);
+            if (r < jb.rows) lfm_visible(A, jb.n_q, jb.len, jb.row0 + r, a, e);
+            if (h * kM < jb.rows) {
+                lfm_visible(A, jb.n_q, jb.len, jb.row0 + h * kM, unused, e_all);
+                lfm_visible(A, jb.n_q, jb.len, jb.row0 + min(jb.rows, (h + 1) * kM) - 1, a_all, unused);
             }
-            const int64_t base = blk0 * kKeys; /* positions are below 2^31 */
-            lo = (int)max((int64_t)0, a - base);
-            hi = (int)max((int64_t)0, e - base);
-            inside0 = (int)((max((int64_t)0, a_all - base) + kKeys - 1) / kKeys);
-            inside1 = (int)(max((int64_t)0, e_all - base) / kKeys);
+            const int64_t key0 = jb.blk0 * kKeys; /* positions are below 2^31 */
+            lo = (int)max((int64_t)0, a - key0);
+            hi = (int)max((int64_t)0, e - key0);
+            inside0 = (int)((max((int64_t)0, a_all - key0) + kKeys - 1) / kKeys);
+            inside1 = (int)(max((int64_t)0, e_all - key0) / kKeys);
         }
         const uint64_t sc2 = pk2(__float_as_uint(sc), __float_as_uint(sc));
         /* O holds the products of block j.  A barrier's parity tells two phases apart: with the scores of block
          * j + 1 the products of j - 2 are done (kBufs <= 6), so those of j and j - 1 take a barrier each, in turn */
         auto products = [&](uint32_t j) {
-            return __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h][j & 1], (j >> 1) & 1, abort, A.err));
+            return __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h][(base + j) & 1], ((base + j) >> 1) & 1, abort, A.err));
         };
         float m = LFM_NO_KEY;
         uint64_t l2 = 0;
         for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t q = 2 * j + h, buf = q % C::kBufs;
+            const uint32_t q = 2 * (base + j) + h, buf = q % C::kBufs;
             const uint32_t tS = tmem + buf * kColS + ((warp & 3) << 21);
             ok = __all_sync(LFM_FULL_MASK, wait(&bars.s_full[buf], (q / C::kBufs) & 1, abort, A.err));
             if (!ok) break;
@@ -372,14 +387,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         /* the barrier of the last products may still be two of its phases back: the one before goes first */
         if (ok && n > 1) ok = products(n - 2);
         if (ok) ok = products(n - 1);
-        if (ok) {
+        if (!ok) break;
+        {
             fence_after();
             const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            volatile Bars *vb = &bars;
-            const uint32_t row = vb->row0 + r;
-            const bool on = r < vb->rows;
-            const size_t at = (size_t)(vb->q0 + row / A.group) * A.out_stride + ((size_t)vb->kvh * A.group + row % A.group) * D;
+            const bool on = r < jb.rows;
+            const size_t at = on ? row_at(A.out_stride) : 0;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 /* columns 32 c ..: values 16 k .. + 15 of the span in the even ones, 32 + 16 k .. in the odd ones */
@@ -401,6 +415,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 }
             }
         }
+        base += n;
+        drop(it);
+      }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp < 12) {
@@ -409,7 +426,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             /* two threads a key: halves of its words */
             const uint32_t key = (warp & 1) * 32 + lane, half = (warp >> 1) & 1;
             const uint32_t codes = key * (D / 2) + half * (D / 4), scales = kKeys * (D / 2) + key * (D / 16) + (D == 64 ? 0 : 4 * half);
-            for (uint32_t u = 0; u < 2 * n; ++u) {
+          for (uint32_t it = 0; take(it); ++it) {
+            const uint32_t n = bars.job[it & 1].n;
+            const int64_t len = bars.job[it & 1].len, blk0 = bars.job[it & 1].blk0 - base;
+            for (uint32_t u = 2 * base; u < 2 * (base + n); ++u) {
                 const uint32_t rs = u % C::kRaws, os = u % C::kOps;
                 bool w = wait(&bars.raw_full[rs], (u / C::kRaws) & 1, abort, A.err);
                 if (u >= (uint32_t)C::kOps) w = w && wait(&bars.op_empty[os], ((u / C::kOps) & 1) ^ 1, abort, A.err);
@@ -441,16 +461,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                     lfm_mbar_arrive(&bars.raw_empty[rs]);
                 }
             }
+            if (!ok) break;
+            base += n;
+            drop(it);
+          }
         } else if (warp == 12 || warp == 14) {
-            if (warp == 12) {
-                asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lfm_smem_u32(&bars.tmem)),
-                             "r"(kTmemCols)
-                             : "memory");
-                asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-            }
-            fence_before();
-            lfm_bar_sync(1, 320);
-            fence_after();
             /* A warp a tile: what one spends on barriers between its MMAs is the other's tensor time.  The whole warp
              * walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all columns are ours) then
              * stay in uniform registers.  From a branch of lane 0 alone they take moves through the pipe that the
@@ -474,39 +489,49 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                     commit(&bars.s_full[buf]);
                     commit(&bars.op_empty[slot]);
                 };
-                auto pv = [&](uint32_t j) {
+                auto pv = [&](uint32_t j, bool first) {
                     const uint32_t buf = (2 * j + h) % C::kBufs, slot = (2 * j + 1) % C::kOps;
                     const uint64_t vd = vd0 + slot * (C::kOp >> 4);
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k)
-                        mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, j > 0 || k > 0);
+                        mma_ts(C::kColO + h * D, buf * kColS + 8 * k, vd + k * (256 >> 4), kIdescPV<D>, !first || k > 0);
                     commit(&bars.o_full[h][j & 1]);
                     commit(&bars.op_empty[slot]);
                 };
                 constexpr uint32_t kAhead = C::kBufs / 2; /* blocks whose scores are asked for ahead */
                 ok = bars.tmem == 0;
-                for (uint32_t j = 0; j < kAhead && j < n && ok; ++j) {
-                    ok = full(2 * j);
-                    if (ok && elect()) qk(j);
-                }
-                bool ready = false; /* block j's keys (those asked for ahead), values and probabilities */
-                for (uint32_t j = 0; j < n && ok; ++j) {
-                    const uint32_t q = 2 * j + h;
-                    const bool more = j + kAhead < n;
-                    if (!__all_sync(LFM_FULL_MASK, ready))
-                        ok = full(2 * j + 1) && (!more || full(2 * (j + kAhead))) &&
-                             __all_sync(LFM_FULL_MASK, wait(&bars.p_full[q % C::kBufs], (q / C::kBufs) & 1, abort, A.err));
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t u = 2 * j + 3, v = 2 * (j + 1 + kAhead), q1 = q + 2;
-                    const bool a = test(&bars.op_full[u % C::kOps], (u / C::kOps) & 1);
-                    const bool b = test(&bars.op_full[v % C::kOps], (v / C::kOps) & 1);
-                    const bool c = test(&bars.p_full[q1 % C::kBufs], (q1 / C::kBufs) & 1);
-                    if (elect()) {
-                        pv(j);
-                        if (more) qk(j + kAhead);
+                for (uint32_t it = 0, jobs = 0; ok && take(it); ++it) {
+                    const uint32_t end = base + bars.job[it & 1].n;
+                    if (end > base) {
+                        ok = __all_sync(LFM_FULL_MASK, wait(&bars.q_full[h], jobs & 1, abort, A.err));
+                        ++jobs;
                     }
-                    ready = a && (b || j + 1 + kAhead >= n) && c;
+                    for (uint32_t j = base; j < base + kAhead && j < end && ok; ++j) {
+                        ok = full(2 * j);
+                        if (ok && elect()) qk(j);
+                    }
+                    bool ready = false; /* block j's keys (those asked for ahead), values and probabilities */
+                    for (uint32_t j = base; j < end && ok; ++j) {
+                        const uint32_t q = 2 * j + h;
+                        const bool more = j + kAhead < end;
+                        if (!__all_sync(LFM_FULL_MASK, ready))
+                            ok = full(2 * j + 1) && (!more || full(2 * (j + kAhead))) &&
+                                 __all_sync(LFM_FULL_MASK, wait(&bars.p_full[q % C::kBufs], (q / C::kBufs) & 1, abort, A.err));
+                        if (!ok) break;
+                        fence_after();
+                        const uint32_t u = 2 * j + 3, v = 2 * (j + 1 + kAhead), q1 = q + 2;
+                        const bool a = test(&bars.op_full[u % C::kOps], (u / C::kOps) & 1);
+                        const bool b = test(&bars.op_full[v % C::kOps], (v / C::kOps) & 1);
+                        const bool c = test(&bars.p_full[q1 % C::kBufs], (q1 / C::kBufs) & 1);
+                        if (elect()) {
+                            pv(j, j == base);
+                            if (more) qk(j + kAhead);
+                        }
+                        ready = j + 1 < end && a && (b || j + 1 + kAhead >= end) && c;
+                    }
+                    if (!ok) break;
+                    base = end;
+                    drop(it);
                 }
             };
             if (warp == 12) walk(std::integral_constant<uint32_t, 0>());
@@ -516,24 +541,71 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             const uint32_t P = A.kv.page_tokens, sub = min(P, (uint32_t)kKeys), piece = lane >> 1, part = lane & 1;
             const uint32_t per = part ? D / 16 : D / 2, bytes = sub * per;
             const uint32_t to = C::kOffRaw + (part ? kKeys * (D / 2) : 0) + piece * bytes;
-            for (uint32_t j = 0; j < n; ++j) {
-                const int64_t key = (blk0 + j) * kKeys + (int64_t)piece * sub;
-                const uint8_t *page = nullptr;
-                if (piece * sub < kKeys && key < len) page = lfm_page(A.kv, A.bt, b, key, kvh, A.err);
-                const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, page ? bytes : 0u);
-                const uint32_t in = ((uint32_t)key & (P - 1)) * per + (part ? A.kv.codes : 0);
-#pragma unroll
-                for (uint32_t k = 0; k < 2; ++k) {
-                    const uint32_t u = 2 * j + k, rs = u % C::kRaws;
-                    ok = ok && (u < (uint32_t)C::kRaws || wait(&bars.raw_empty[rs], ((u / C::kRaws) & 1) ^ 1, abort, A.err));
-                    ok = __all_sync(LFM_FULL_MASK, ok);
-                    if (!ok) break;
-                    if (lane == 0) lfm_mbar_arrive_tx(&bars.raw_full[rs], all);
+            uint32_t w = blockIdx.x;
+            for (uint32_t it = 0; ok; ++it) {
+                /* the next job: the longest walks first (tiles from the last), all heads of one side by side */
+                Job jb;
+                jb.b = -1;
+                jb.n = 0;
+                for (; w < tiles * A.kv.hkv; w = gridDim.x + __shfl_sync(LFM_FULL_MASK, w, 0)) {
+                    lfm_find_tile(A.bt, G, kRows, 0, above, ~0ull, tiles - 1 - w / A.kv.hkv, bars.tile);
                     __syncwarp();
-                    if (page)
-                        lfm_bulk_g2s_plain(sm + to + rs * C::kRaw, page + in + (k ? A.kv.half : 0), bytes, &bars.raw_full[rs]);
+                    const int b = *(volatile int *)&bars.tile[0];
+                    jb.row0 = (uint32_t)*(volatile int *)&bars.tile[1] * kRows;
+                    jb.kvh = w % A.kv.hkv;
+                    __syncwarp();
+                    if (lane == 0) w = atomicAdd(count, 1u); /* of the one after */
+                    if (b < 0) continue;
+                    jb.q0 = A.bt.q_start[b];
+                    jb.n_q = (int64_t)A.bt.q_start[b + 1] - jb.q0;
+                    jb.len = A.bt.kv_len[b];
+                    if (jb.len < 0) {
+                        if (lane == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
+                        continue;
+                    }
+                    jb.rows = (uint32_t)min((int64_t)kRows, jb.n_q * (int64_t)G - jb.row0); /* at least 1 */
+                    int64_t lo0, hi0, lo1, hi1;
+                    lfm_visible(A, jb.n_q, jb.len, jb.row0, lo0, hi0);
+                    lfm_visible(A, jb.n_q, jb.len, jb.row0 + jb.rows - 1, lo1, hi1);
+                    jb.blk0 = lo0 / kKeys;
+                    jb.n = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - jb.blk0) : 0;
+                    jb.b = b;
+                    break;
                 }
+                if (jb.b >= 0) w = gridDim.x + __shfl_sync(LFM_FULL_MASK, w, 0);
+                if (it > 1) ok = __all_sync(LFM_FULL_MASK, wait(&bars.job_empty[it & 1], ((it >> 1) & 1) ^ 1, abort, A.err));
                 if (!ok) break;
+                if (lane == 0) {
+                    bars.job[it & 1] = jb;
+                    lfm_mbar_arrive(&bars.job_full[it & 1]);
+                }
+                if (jb.b < 0) break;
+                const uint32_t n = jb.n;
+                for (uint32_t j = 0; j < n; ++j) {
+                    const int64_t key = (jb.blk0 + j) * kKeys + (int64_t)piece * sub;
+                    const uint8_t *page = nullptr;
+                    if (piece * sub < kKeys && key < jb.len) page = lfm_page(A.kv, A.bt, jb.b, key, jb.kvh, A.err);
+                    const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, page ? bytes : 0u);
+                    const uint32_t in = ((uint32_t)key & (P - 1)) * per + (part ? A.kv.codes : 0);
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        const uint32_t u = 2 * (base + j) + k, rs = u % C::kRaws;
+                        ok = ok && (u < (uint32_t)C::kRaws || wait(&bars.raw_empty[rs], ((u / C::kRaws) & 1) ^ 1, abort, A.err));
+                        ok = __all_sync(LFM_FULL_MASK, ok);
+                        if (!ok) break;
+                        if (lane == 0) lfm_mbar_arrive_tx(&bars.raw_full[rs], all);
+                        __syncwarp();
+                        if (page)
+                            lfm_bulk_g2s_plain(sm + to + rs * C::kRaw, page + in + (k ? A.kv.half : 0), bytes, &bars.raw_full[rs]);
+                    }
+                    if (!ok) break;
+                }
+                base += n;
+            }
+            /* the last block to come here leaves the counters zero */
+            if (lane == 0 && atomicAdd(count + 1, 1u) == gridDim.x - 1) {
+                count[0] = 0;
+                count[1] = 0;
             }
         }
     }
@@ -554,22 +626,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
 }
 
 template <int D>
-cudaError_t launch_tile(const AttnArgs &a, uint64_t above, dim3 grid, cudaStream_t s, bool pdl) {
+cudaError_t launch_tile(const AttnArgs &a, uint64_t above, uint32_t tiles, uint32_t *count, dim3 grid, cudaStream_t s, bool pdl) {
     static size_t set[2][16];
     auto fn = a.softcap > 0.0f ? k_attn_tile<D, true> : k_attn_tile<D, false>;
     const cudaError_t e = lfm_smem_attr((const void *)fn, Cfg<D>::kSmem, set[a.softcap > 0.0f]);
-    return e != cudaSuccess ? e : lfm_launch_pdl(fn, grid, dim3(kThreads), Cfg<D>::kSmem, s, pdl, a, above);
+    return e != cudaSuccess ? e : lfm_launch_pdl(fn, grid, dim3(kThreads), Cfg<D>::kSmem, s, pdl, a, above, tiles, count);
 }
 
 }  // namespace
 
-cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, cudaStream_t s, bool pdl) {
+cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, int sm_count, uint32_t *count,
+                                 cudaStream_t s, bool pdl) {
     /* a tile for every started kRows rows of a sequence: at most this many */
     const uint64_t rows = (uint64_t)a.bt.n_tokens * a.group, most = a.bt.n_seqs < a.bt.n_tokens ? a.bt.n_seqs : a.bt.n_tokens;
     const uint64_t big = rows / (above + 1) < most ? rows / (above + 1) : most; /* sequences of more than `above` rows */
-    const uint64_t blocks = (rows / kRows + big) * a.kv.hkv; /* below 2^31 / 256 * 1024 / group */
-    if (blocks == 0) return cudaSuccess;
-    if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
-    const dim3 grid((uint32_t)blocks);
-    return head_dim == 64 ? launch_tile<64>(a, above, grid, s, pdl) : launch_tile<128>(a, above, grid, s, pdl);
+    const uint64_t tiles = rows / kRows + big, jobs = tiles * a.kv.hkv;
+    if (jobs == 0) return cudaSuccess;
+    if (jobs > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    const dim3 grid((uint32_t)(jobs < (uint64_t)sm_count ? jobs : (uint64_t)sm_count));
+    return head_dim == 64 ? launch_tile<64>(a, above, (uint32_t)tiles, count, grid, s, pdl)
+                          : launch_tile<128>(a, above, (uint32_t)tiles, count, grid, s, pdl);
 }

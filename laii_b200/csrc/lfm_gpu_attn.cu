@@ -223,14 +223,13 @@ LFM_API lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     OnDevice g(hv.device);
     void *scratch = nullptr;
-    bool used = false;
     st = lfm_host_scratch(h, s, &scratch);
     if (st != LFM_GPU_OK) return st;
     const uint32_t span = batch->table_stride * kv->page_tokens;
     const uint32_t hint = batch->max_kv_len && batch->max_kv_len < span ? batch->max_kv_len : span;
     st = launch(h, hv, AK_ATTN, "attn_forward", s,
-                [&] { return lfm_launch_attn(a, kv->head_dim, hint, hv.sm_count, scratch, &used, s, hv.pdl); });
-    return st == LFM_GPU_OK && used ? lfm_host_scratch_used(h, s) : st;
+                [&] { return lfm_launch_attn(a, kv->head_dim, hint, hv.sm_count, scratch, s, hv.pdl); });
+    return st == LFM_GPU_OK ? lfm_host_scratch_used(h, s) : st;
 }
 
 LFM_API lfm_gpu_status_t lfm_gpu_attn_reserve(lfm_gpu_moe_t *h) {
