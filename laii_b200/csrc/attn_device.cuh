@@ -186,14 +186,6 @@ __device__ __forceinline__ void lfm_fit_q(bool neg, float (&v)[8]) {
         v[i] = x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
     }
 }
-/* Eight values of a q row at `at`, so fitted. */
-__device__ __forceinline__ void lfm_load_q(const AttnArgs &A, size_t at, bool neg, float (&v)[8]) {
-    if (A.type == 0) lfm_load<8>(static_cast<const float *>(A.q) + at, v);
-    else if (A.type == 1) lfm_load<8>(static_cast<const __half *>(A.q) + at, v);
-    else lfm_load<8>(static_cast<const __nv_bfloat16 *>(A.q) + at, v);
-    lfm_fit_q(neg, v);
-}
-
 /* Keys [lo, hi) that row r (token, head of the group) of a sequence of n_q tokens behind len cached ones sees. */
 __device__ __forceinline__ void lfm_visible(const AttnArgs &A, int64_t n_q, int64_t len, uint32_t r, int64_t &lo,
                                             int64_t &hi) {

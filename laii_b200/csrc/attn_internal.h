@@ -80,6 +80,8 @@ cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_k
  * before and after. */
 cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, int sm_count, uint32_t *count,
                                  cudaStream_t s, bool pdl);
+/* ... and its tiles of rows of one kv head, at most. */
+uint64_t lfm_attn_tiles(const AttnArgs &a, uint64_t above);
 #define LFM_ATTN_COUNTS 1024u                                     /* most blocks that share work      */
 #define LFM_ATTN_PARTS_BYTES ((size_t)LFM_ATTN_COUNTS * 2 * 32 * 66 * 4) /* two parts each, 32 x (64 + 2) or 16 x (128 + 2) */
 #define LFM_ATTN_SCRATCH_BYTES (LFM_ATTN_PARTS_BYTES + LFM_ATTN_COUNTS * sizeof(uint32_t))

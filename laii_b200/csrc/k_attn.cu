@@ -312,34 +312,49 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
         /* ---- Q as B fragments: column g, values 64 s + 32 c + 8 t .. of the head ---- */
         uint32_t qf[NT][kS][2][4];
         float corr[NT][kS][2][4]; /* start values of the scores: minus the codes' offsets times q */
+        auto load = [&](const auto *q) { /* the type is told apart once, so the loads are under way together */
+            float v[NT][kS][2][8];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const uint32_t r = row0 + n * 8 + g;
-            const bool on = n * 8 + g <= last;
-            const size_t at = on ? (size_t)(q0 + r / G) * A.q_stride + ((size_t)kvh * G + r % G) * D : 0;
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t r = row0 + n * 8 + g;
+                const bool on = n * 8 + g <= last;
+                const size_t at = on ? (size_t)(q0 + r / G) * A.q_stride + ((size_t)kvh * G + r % G) * D : 0;
 #pragma unroll
-            for (int s = 0; s < kS; ++s)
+                for (int s = 0; s < kS; ++s)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (on) lfm_load_q(A, at + 64 * s + 32 * c + 8 * t, A.scale < 0.0f, v);
-                    float h[8], sum = 0.0f;
+                    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        h[i] = __half2float(__float2half_rn(v[i]));
-                        sum = __fmaf_rn(h[i], (i & 1) ? 72.0f : 1032.0f, sum);
+                        for (int i = 0; i < 8; ++i) v[n][s][c][i] = 0.0f;
+                        if (on) lfm_load<8>(q + at + 64 * s + 32 * c + 8 * t, v[n][s][c]);
                     }
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) qf[n][s][c][i] = lfm_pack2(h[i], h[4 + i], __half());
-                    sum += __shfl_xor_sync(LFM_FULL_MASK, sum, 1);
-                    sum += __shfl_xor_sync(LFM_FULL_MASK, sum, 2);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        corr[n][s][c][i] = -__shfl_sync(LFM_FULL_MASK, sum, 8 * t + 4 * (i & 1));
-                        asm volatile("" : "+f"(corr[n][s][c][i])); /* four registers, not two */
+                for (int s = 0; s < kS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        lfm_fit_q(A.scale < 0.0f, v[n][s][c]);
+                        float h[8], sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            h[i] = __half2float(__float2half_rn(v[n][s][c][i]));
+                            sum = __fmaf_rn(h[i], (i & 1) ? 72.0f : 1032.0f, sum);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) qf[n][s][c][i] = lfm_pack2(h[i], h[4 + i], __half());
+                        sum += __shfl_xor_sync(LFM_FULL_MASK, sum, 1);
+                        sum += __shfl_xor_sync(LFM_FULL_MASK, sum, 2);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            corr[n][s][c][i] = -__shfl_sync(LFM_FULL_MASK, sum, 8 * t + 4 * (i & 1));
+                            asm volatile("" : "+f"(corr[n][s][c][i])); /* four registers, not two */
+                        }
                     }
-                }
-        }
+        };
+        if (A.type == 0) load(static_cast<const float *>(A.q));
+        else if (A.type == 1) load(static_cast<const __half *>(A.q));
+        else load(static_cast<const __nv_bfloat16 *>(A.q));
 
         /* ---- the keys ---- */
         float o[NT][kS][2][2][4], m[NT][2], l[NT][2];
@@ -595,14 +610,34 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
                 for (uint32_t i = tid; i < (last + 1) * (D / 4); i += kThreads) {
                     const uint32_t col = i / (D / 4), d = i % (D / 4) * 4;
                     float mx = LFM_NO_KEY, v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.0f;
-                    for (uint32_t c = own0; c <= own1; ++c) mx = fmaxf(mx, __ldcg(part_of(c) + (size_t)col * (D + 2)));
-                    for (uint32_t c = own0; c <= own1; ++c) {
-                        const float2 *p = reinterpret_cast<const float2 *>(part_of(c) + (size_t)col * (D + 2));
-                        const float2 ml = __ldcg(p), x0 = __ldcg(p + 1 + d / 2), y0 = __ldcg(p + 2 + d / 2);
-                        const float f = lfm_ex2(ml.x - mx);
-                        v[0] = __fmaf_rn(f, x0.x, v[0]); v[1] = __fmaf_rn(f, x0.y, v[1]);
-                        v[2] = __fmaf_rn(f, y0.x, v[2]); v[3] = __fmaf_rn(f, y0.y, v[3]);
-                        sum = __fmaf_rn(f, ml.y, sum);
+                    for (uint32_t c0 = own0; c0 <= own1; c0 += 8) { /* eight parts' loads under way together */
+                        float2 ml[8], a[8], b[8];
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) {
+                            ml[k] = make_float2(LFM_NO_KEY, 0.0f);
+                            a[k] = b[k] = make_float2(0.0f, 0.0f);
+                            if (c0 + k <= own1) {
+                                const float2 *p = reinterpret_cast<const float2 *>(part_of(c0 + k) + (size_t)col * (D + 2));
+                                ml[k] = __ldcg(p);
+                                a[k] = __ldcg(p + 1 + d / 2);
+                                b[k] = __ldcg(p + 2 + d / 2);
+                            }
+                        }
+                        float top = mx;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+                        const float old = lfm_ex2(mx - top);
+                        mx = top;
+                        sum *= old;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] *= old;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float f = lfm_ex2(ml[k].x - mx);
+                            v[0] = __fmaf_rn(f, a[k].x, v[0]); v[1] = __fmaf_rn(f, a[k].y, v[1]);
+                            v[2] = __fmaf_rn(f, b[k].x, v[2]); v[3] = __fmaf_rn(f, b[k].y, v[3]);
+                            sum = __fmaf_rn(f, ml[k].y, sum);
+                        }
                     }
                     write(col, d, v, sum);
                 }
@@ -627,9 +662,6 @@ cudaError_t launch_rows(const AttnArgs &a, const RowsPlan &p, dim3 grid, cudaStr
 
 }  // namespace
 
-/* Rows of a sequence up to which it is this file's: measured, see launch below. */
-constexpr uint64_t kFewRows = 64;
-
 static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, uint64_t few, uint32_t max_kv_len,
                                         int sm_count, void *scratch, cudaStream_t s, bool pdl) {
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, G = a.group, keys = head_dim == 64 ? 64 : 32;
@@ -650,14 +682,25 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
     return nt == 1 ? launch_rows<128, 1>(a, p, g, s, pdl) : launch_rows<128, 2>(a, p, g, s, pdl);
 }
 
+/* Which kernel takes a sequence.  Per SM, 32 rows against 64 keys take this file's kernel 0.44 us (64-value heads;
+ * 128: 0.98) and 256 rows, however few of them there are, the tile kernel 1.1 us (1.15).  This one cuts its work into
+ * equal parts for all SMs; a tile is one SM's from end to end.  So of two sides, in units of 32 rows x all keys
+ * against whole rounds of tiles, the shorter.  Measured, 32 / 8 heads, rows of a sequence (token, head of the group):
+ *   32 sequences of 4096 keys, 64-value heads   64 rows: 115 us here, 162 there;  96: 164, 163;  128: 212, 163
+ *                              128-value heads  32 rows: 132, 189;  64: 241, 190;  128: 452, 185
+ *   8 sequences of 4096 keys, 64-value heads    128 rows: 67, 83;  256: 113, 70
+ *   1 sequence of 16384 keys, 64-value heads    512 rows: 104, 242
+ * In a batch that is not all this kernel's, sequences of few rows still are: 64 (128-value heads: 32). */
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
                             cudaStream_t s, bool pdl) {
-    const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group;
-    /* one sequence, or at most as many tokens as make few rows: one kernel takes all.  As many tokens as sequences
-     * are a step of single tokens, whatever the odd sequence holds.  Otherwise each takes its sequences */
-    if (rows <= kFewRows || T == B) return lfm_launch_attn_rows(a, head_dim, ~0ull, max_kv_len, sm_count, scratch, s, pdl);
+    const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group, few = B == 1 ? 0 : head_dim == 64 ? 64 : 32;
+    const uint64_t units = (rows + 16 * B) / 32 * a.kv.hkv, tiles = lfm_attn_tiles(a, few) * a.kv.hkv;
+    const uint64_t rounds = (tiles + sm_count - 1) / sm_count * sm_count;
+    /* as many tokens as sequences are a step of single tokens, whatever an odd sequence holds: one kernel takes all
+     * (64 sequences of 8192 keys: 86 us, 92 with a launch for each) */
+    if (T == B || (head_dim == 64 ? units * 2 < rounds * 5 : units * 6 < rounds * 7))
+        return lfm_launch_attn_rows(a, head_dim, ~0ull, max_kv_len, sm_count, scratch, s, pdl);
     uint32_t *count = static_cast<uint32_t *>(scratch) + LFM_ATTN_COUNTS - 2;
-    if (B == 1) return lfm_launch_attn_tile(a, head_dim, 0, sm_count, count, s, pdl);
-    const cudaError_t e = lfm_launch_attn_tile(a, head_dim, kFewRows, sm_count, count, s, pdl);
-    return e != cudaSuccess ? e : lfm_launch_attn_rows(a, head_dim, kFewRows, max_kv_len, sm_count, scratch, s, pdl);
+    const cudaError_t e = lfm_launch_attn_tile(a, head_dim, few, sm_count, count, s, pdl);
+    return e != cudaSuccess || B == 1 ? e : lfm_launch_attn_rows(a, head_dim, few, max_kv_len, sm_count, scratch, s, pdl);
 }

@@ -635,12 +635,15 @@ cudaError_t launch_tile(const AttnArgs &a, uint64_t above, uint32_t tiles, uint3
 
 }  // namespace
 
+/* One for every started kRows rows of a sequence of more than `above`: at most this many. */
+uint64_t lfm_attn_tiles(const AttnArgs &a, uint64_t above) {
+    const uint64_t rows = (uint64_t)a.bt.n_tokens * a.group, most = rows / (above + 1);
+    return rows / kRows + (most < a.bt.n_seqs ? most : a.bt.n_seqs);
+}
+
 cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, int sm_count, uint32_t *count,
                                  cudaStream_t s, bool pdl) {
-    /* a tile for every started kRows rows of a sequence: at most this many */
-    const uint64_t rows = (uint64_t)a.bt.n_tokens * a.group, most = a.bt.n_seqs < a.bt.n_tokens ? a.bt.n_seqs : a.bt.n_tokens;
-    const uint64_t big = rows / (above + 1) < most ? rows / (above + 1) : most; /* sequences of more than `above` rows */
-    const uint64_t tiles = rows / kRows + big, jobs = tiles * a.kv.hkv;
+    const uint64_t tiles = lfm_attn_tiles(a, above), jobs = tiles * a.kv.hkv;
     if (jobs == 0) return cudaSuccess;
     if (jobs > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
     const dim3 grid((uint32_t)(jobs < (uint64_t)sm_count ? jobs : (uint64_t)sm_count));
