@@ -104,10 +104,10 @@ __device__ __forceinline__ bool lfm_sane(const BatchDev &bt, int64_t q0, int64_t
     return q0 >= 0 && n >= 0 && q0 + n <= (int64_t)bt.n_tokens;
 }
 
-/* One warp: the want-th tile of `per` rows (token, head of a group of G) over the sequences with more than `above`
- * and at most `most` rows, `skip` tiles left out of each: (sequence, tile) into out, or a sequence of -1. */
-__device__ __forceinline__ void lfm_find_tile(const BatchDev &bt, uint32_t G, uint32_t per, uint32_t skip, uint64_t above,
-                                              uint64_t most, uint64_t want, int *out) {
+/* One warp: the want-th tile of `per` rows (token, head of a group of G) over the sequences of more than `above` rows:
+ * (sequence, tile) into out, or a sequence of -1.  Returns the tiles looked through: all where there is no such. */
+__device__ __forceinline__ uint64_t lfm_find_tile(const BatchDev &bt, uint32_t G, uint32_t per, uint64_t above, uint64_t want,
+                                                  int *out) {
     const uint32_t lane = threadIdx.x & 31;
     uint64_t before = 0;
     for (uint32_t b0 = 0; b0 < bt.n_seqs; b0 += 32) {
@@ -115,7 +115,7 @@ __device__ __forceinline__ void lfm_find_tile(const BatchDev &bt, uint32_t G, ui
         if (b0 + lane < bt.n_seqs) {
             const int64_t q = bt.q_start[b0 + lane], q_n = (int64_t)bt.q_start[b0 + lane + 1] - q;
             const uint64_t rows = q_n > 0 && lfm_sane(bt, q, q_n) ? (uint64_t)q_n * G : 0;
-            if (rows > above && rows <= most) n = (rows - 1) / per + 1 - skip;
+            if (rows > above) n = (rows - 1) / per + 1;
         }
         uint64_t sum = n;
 #pragma unroll
@@ -126,12 +126,13 @@ __device__ __forceinline__ void lfm_find_tile(const BatchDev &bt, uint32_t G, ui
         const bool here = want >= before + sum - n && want < before + sum;
         if (here) {
             out[0] = (int)(b0 + lane);
-            out[1] = (int)(want - (before + sum - n) + skip);
+            out[1] = (int)(want - (before + sum - n));
         }
-        if (__any_sync(LFM_FULL_MASK, here)) return;
         before += __shfl_sync(LFM_FULL_MASK, sum, 31);
+        if (__any_sync(LFM_FULL_MASK, here)) return before;
     }
     if (lane == 0) out[0] = -1;
+    return before;
 }
 
 /* Codes to fp16: a nibble in an fp16 exponent, bits 0-3 of a half as 1024 + c, bits 4-7 as 64 + c. */

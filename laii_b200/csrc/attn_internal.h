@@ -76,15 +76,20 @@ cudaError_t lfm_launch_kv_read(const ReadArgs &a, uint32_t head_dim, uint32_t ty
  * LFM_ATTN_COUNTS words zero; the kernels leave them zero). */
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
                             cudaStream_t s, bool pdl);
-/* The tensor-core kernel for the sequences of more than `above` rows (token, head of a group); count: two words, zero
- * before and after. */
-cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, int sm_count, uint32_t *count,
+/* The tensor-core kernel for the sequences of more than `above` rows (token, head of a group). */
+struct TilePlan {
+    uint64_t above, blocks, cost;  /* key blocks of the longest walk by max_kv_len; blocks that the busiest SM walks */
+    uint32_t tiles, parts;         /* tiles of rows of one kv head, at most; most parts of one */
+    uint32_t *counts;              /* zero before and after */
+    float *part;
+};
+TilePlan lfm_attn_tile_plan(const AttnArgs &a, uint32_t head_dim, uint64_t above, uint32_t max_kv_len, int sm_count);
+cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, const TilePlan &plan, int sm_count, void *scratch,
                                  cudaStream_t s, bool pdl);
-/* ... and its tiles of rows of one kv head, at most. */
-uint64_t lfm_attn_tiles(const AttnArgs &a, uint64_t above);
-#define LFM_ATTN_COUNTS 1024u                                     /* most blocks that share work      */
-#define LFM_ATTN_PARTS_BYTES ((size_t)LFM_ATTN_COUNTS * 2 * 32 * 66 * 4) /* two parts each, 32 x (64 + 2) or 16 x (128 + 2) */
-#define LFM_ATTN_SCRATCH_BYTES (LFM_ATTN_PARTS_BYTES + LFM_ATTN_COUNTS * sizeof(uint32_t))
+#define LFM_ATTN_COUNTS 4096u /* words */
+#define LFM_ATTN_BLOCKS 1022u /* most blocks of the few-row kernel: two parts each, 32 x (64 + 2) or 16 x (128 + 2) floats */
+#define LFM_ATTN_TILES 592u   /* most parts of split tiles: 256 x (128 + 2) floats, more than the former */
+#define LFM_ATTN_SCRATCH_BYTES (LFM_ATTN_COUNTS * sizeof(uint32_t) + (size_t)LFM_ATTN_TILES * 256 * 130 * 4)
 
 /* ---- the handle, as lfm_gpu_moe.cu keeps it ------------------------------ */
 enum AttnKernelId { AK_NORM, AK_Q8K_READ, AK_APPEND, AK_KV_READ, AK_ATTN };

@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
     __shared__ int64_t s_hi[kCols], s_lo[kCols];
     __shared__ uint64_t s_sum[kWarps], s_first;
     __shared__ int s_seq, s_last;
+    __shared__ uint32_t s_units[kWarps];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t G = A.group;
     if (lane < kStages) lfm_mbar_init(&s_bar[warp][lane], 1);
@@ -213,24 +214,36 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
     uint64_t w = 0; /* this thread's sequence of the last 256 looked at */
     {
         uint64_t sum = 0;
+        uint32_t units = 0;
         for (uint32_t b0 = 0; b0 < A.bt.n_seqs; b0 += kThreads) {
             w = 0;
             if (b0 + tid < A.bt.n_seqs) {
                 const Seq q = sequence(b0 + tid);
                 if (!q.sane && blockIdx.x == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
                 w = q.weight;
+                units += (uint32_t)min(q.tiles * A.kv.hkv, (uint64_t)(1u << 20));
+                units = min(units, 1u << 20);
             }
             sum += w;
         }
         sum = warp_scan(sum);
         if (lane == 31) s_sum[warp] = sum;
+        units = __reduce_add_sync(LFM_FULL_MASK, min(units, 1u << 20)); /* beyond the blocks it makes no difference */
+        if (lane == 0) s_units[warp] = units;
     }
     __syncthreads();
     uint64_t total = 0;
+    uint32_t units = 0;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) total += s_sum[i];
-    /* blocks at work: a block of keys for each warp at least */
-    const uint64_t n_cta = min((uint64_t)gridDim.x, (total + kWarps - 1) / kWarps);
+    for (int i = 0; i < kWarps; ++i) {
+        total += s_sum[i];
+        units += s_units[i];
+    }
+    /* blocks at work: a block of keys for each warp, or one for each unit where units are shorter */
+    uint64_t n_cta = min((uint64_t)gridDim.x, max((total + kWarps - 1) / kWarps, (uint64_t)units));
+    /* units that are all alike: cuts that fall between them, where that leaves few blocks idle.  A block that ends one
+     * unit and begins another loads q and joins twice */
+    if (units && units <= n_cta && total % units == 0 && 4 * (n_cta / units * units) >= 3 * n_cta) n_cta = n_cta / units * units;
     if (blockIdx.x >= n_cta) return;
     uint64_t x = total * blockIdx.x / n_cta;
     const uint64_t x1 = total * (blockIdx.x + 1) / n_cta;
@@ -670,9 +683,10 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
     const uint32_t nt = per <= 8 ? 1 : per <= 16 || head_dim == 128 ? 2 : 4;
     /* blocks: as many as run at once, fewer where there are not enough blocks of keys by the hint */
     uint64_t grid = (uint64_t)sm_count * (head_dim * nt < 128 ? 4 : head_dim * nt == 128 ? 3 : 2);
-    const uint64_t work = (B + T * G / (8 * nt)) * a.kv.hkv * ((max_kv_len + keys - 1) / keys + 1);
-    if (grid > (work + kWarps - 1) / kWarps) grid = (work + kWarps - 1) / kWarps;
-    if (grid > LFM_ATTN_COUNTS - 2) grid = LFM_ATTN_COUNTS - 2;
+    const uint64_t units = (B + T * G / (8 * nt)) * a.kv.hkv, work = units * ((max_kv_len + keys - 1) / keys + 1);
+    const uint64_t most = work / kWarps > units ? work / kWarps : units;
+    if (grid > most) grid = most;
+    if (grid > LFM_ATTN_BLOCKS) grid = LFM_ATTN_BLOCKS;
     RowsPlan p{few, reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + LFM_ATTN_COUNTS * sizeof(uint32_t)),
                static_cast<uint32_t *>(scratch)};
     const dim3 g((uint32_t)grid);
@@ -683,24 +697,28 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
 }
 
 /* Which kernel takes a sequence.  Per SM, 32 rows against 64 keys take this file's kernel 0.44 us (64-value heads;
- * 128: 0.98) and 256 rows, however few of them there are, the tile kernel 1.1 us (1.15).  This one cuts its work into
- * equal parts for all SMs; a tile is one SM's from end to end.  So of two sides, in units of 32 rows x all keys
- * against whole rounds of tiles, the shorter.  Measured, 32 / 8 heads, rows of a sequence (token, head of the group):
- *   32 sequences of 4096 keys, 64-value heads   64 rows: 115 us here, 162 there;  96: 164, 163;  128: 212, 163
- *                              128-value heads  32 rows: 132, 189;  64: 241, 190;  128: 452, 185
- *   8 sequences of 4096 keys, 64-value heads    128 rows: 67, 83;  256: 113, 70
- *   1 sequence of 16384 keys, 64-value heads    512 rows: 104, 242
- * In a batch that is not all this kernel's, sequences of few rows still are: 64 (128-value heads: 32). */
+ * 128: 0.98), and 256 rows, however few of them there are, the tile kernel 1.1 us (1.15).  This one spreads any work
+ * over all SMs, the tile kernel whole rounds of tiles or of their parts; a call for both pays for two launches.  So
+ * both sides are estimated, in blocks of keys, and the shorter taken.  Measured, 32 / 8 heads, rows of a sequence
+ * (token, head of the group), this kernel and the other:
+ *   32 sequences of 4096 keys, 64-value heads   64 rows: 110 us, 115;  128: 201, 174;  256: 376, 140
+ *                              128-value heads  32 rows: 122, 136;  64: 225, 216;  128: 428, 213
+ *   8 sequences of 4096 keys, 64-value heads    64 rows: 37, 43;  128: 55, 78;  256: 107, 72
+ *   1 sequence of 16384 keys, 64-value heads    128 rows: 39, 48;  256: 59, 45;  512: 104, 50
+ *   1 sequence of 2048 keys, 64-value heads     256 rows: 21, 23;  512: 26, 25;  1024: 33, 26
+ * In a batch for both, sequences of up to 64 rows (128-value heads: 32) are this kernel's. */
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
                             cudaStream_t s, bool pdl) {
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group, few = B == 1 ? 0 : head_dim == 64 ? 64 : 32;
-    const uint64_t units = (rows + 16 * B) / 32 * a.kv.hkv, tiles = lfm_attn_tiles(a, few) * a.kv.hkv;
-    const uint64_t rounds = (tiles + sm_count - 1) / sm_count * sm_count;
-    /* as many tokens as sequences are a step of single tokens, whatever an odd sequence holds: one kernel takes all
-     * (64 sequences of 8192 keys: 86 us, 92 with a launch for each) */
-    if (T == B || (head_dim == 64 ? units * 2 < rounds * 5 : units * 6 < rounds * 7))
+    const TilePlan p = lfm_attn_tile_plan(a, head_dim, few, max_kv_len, sm_count);
+    const uint64_t here = (rows + 16 * B) / 32 * a.kv.hkv * (p.blocks + 12);   /* 12: a unit's cost beside its blocks */
+    const uint64_t there = (p.cost + (B == 1 ? 3 : 10)) * (uint64_t)sm_count;  /* 10: the second launch */
+    /* sequences of few rows by their average, and of no odd one that could be long: a step of single tokens (64
+     * sequences of 8192 keys: 86 us, 92 with an idle launch of the other kernel), a batch to verify (16 sequences of
+     * 8 tokens and 8192 keys: 63, 70) */
+    const bool short_ones = T <= B || (rows <= few * B && (T - B + 1) * a.group <= 1024);
+    if (short_ones || (head_dim == 64 ? here * 2 < there * 5 : here * 6 < there * 7))
         return lfm_launch_attn_rows(a, head_dim, ~0ull, max_kv_len, sm_count, scratch, s, pdl);
-    uint32_t *count = static_cast<uint32_t *>(scratch) + LFM_ATTN_COUNTS - 2;
-    const cudaError_t e = lfm_launch_attn_tile(a, head_dim, few, sm_count, count, s, pdl);
+    const cudaError_t e = lfm_launch_attn_tile(a, head_dim, p, sm_count, scratch, s, pdl);
     return e != cudaSuccess || B == 1 ? e : lfm_launch_attn_rows(a, head_dim, few, max_kv_len, sm_count, scratch, s, pdl);
 }

@@ -35,6 +35,9 @@ namespace {
 constexpr int kM = 128, kRows = 2 * kM, kKeys = 64, kThreads = 512;
 constexpr uint32_t kChunkQ = kM * 16, kChunk = kKeys * 16; /* bytes between the 8-value chunks of a row */
 
+/* Key blocks that a part of a split tile has at least; what a tile costs beside its blocks, in blocks. */
+constexpr uint32_t kPartBlocks = 8, kJobBlocks = 6;
+
 template <int D>
 struct Cfg {
     static constexpr int kQ = kM * D * 2, kOp = kKeys * D * 2; /* a tile of q; of keys or values */
@@ -51,10 +54,10 @@ constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32
 template <int D>
 constexpr uint32_t kIdescPV = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(D >> 3) << 17) | (1u << 16);
 
-/* 256 rows of a kv head: rows row0 .. of sequence b, key blocks blk0 .. + n. */
+/* 256 rows of a kv head: rows row0 .. of sequence b, key blocks blk0 .. + n; part `part` of `parts` of tile `tile`. */
 struct Job {
     int64_t q0, n_q, len, blk0;
-    uint32_t row0, rows, kvh, n;
+    uint32_t row0, rows, kvh, n, tile, part, parts;
     int b; /* -1: no more */
 };
 struct Bars {
@@ -170,8 +173,9 @@ __device__ __forceinline__ bool test(uint64_t *bar, uint32_t parity) {
 }
 
 template <int D, bool kCap>
-__global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t above, uint32_t tiles, uint32_t *count) {
+__global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan plan) {
     using C = Cfg<D>;
+    uint32_t *const ticket = plan.counts + LFM_ATTN_COUNTS - 2;
     extern __shared__ __align__(1024) uint8_t sm[];
     __shared__ Bars bars;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.group;
@@ -208,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
     __syncthreads();
     fence_after();
     lfm_pdl_wait();
+    lfm_pdl_launch_dependents();
     const uint32_t smem = lfm_smem_u32(sm);
     bool ok = true;
     /* job `it`, for all roles but the loader; false at the end */
@@ -391,26 +396,79 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
         {
             fence_after();
             const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             const bool on = r < jb.rows;
             const size_t at = on ? row_at(A.out_stride) : 0;
+            /* columns 32 c ..: values 16 k .. + 15 of the span in the even ones, 32 + 16 k .. in the odd ones */
+            auto write = [&](int c, const float *o, float inv) {
+                if (!on) return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = o[2 * (8 * (e & 1) + i) + (e >> 1)] * inv;
+                    const size_t to = at + 64 * (c >> 1) + 16 * (c & 1) + 8 * (e & 1) + 32 * (e >> 1);
+                    if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + to, v);
+                    else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + to, v);
+                    else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + to, v);
+                }
+            };
+            /* a part: [value / 4][row] of 16 bytes, then the rows' m and sum */
+            auto part_of = [&](uint32_t s) { return plan.part + ((size_t)jb.tile * plan.parts + s) * kRows * (D + 2); };
+            float *const mine = jb.parts > 1 ? part_of(jb.part) : nullptr;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                /* columns 32 c ..: values 16 k .. + 15 of the span in the even ones, 32 + 16 k .. in the odd ones */
-                uint32_t o[32];
-                ld32(tO + 32 * c, o);
+                uint32_t u[32];
+                float o[32];
+                ld32(tO + 32 * c, u);
                 wait_ld();
-                tie32(o);
-                if (on) {
+                tie32(u);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v[8];
+                for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
+                if (!mine) {
+                    write(c, o, l > 0.0f ? 1.0f / l : 0.0f);
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[2 * (8 * (e & 1) + i) + (e >> 1)]) * inv;
-                        const size_t to = at + 64 * (c >> 1) + 16 * (c & 1) + 8 * (e & 1) + 32 * (e >> 1);
-                        if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + to, v);
-                        else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + to, v);
-                        else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + to, v);
+                    for (int k = 0; k < 8; ++k)
+                        __stcg(reinterpret_cast<float4 *>(mine) + (size_t)(8 * c + k) * kRows + r,
+                               make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+                }
+            }
+            if (mine) {
+                /* the last warp to arrive with a part of these 32 rows joins them all, in their order */
+                __stcg(reinterpret_cast<float2 *>(mine + kRows * D) + r, make_float2(m, l));
+                __threadfence();
+                __syncwarp();
+                uint32_t *const arrived = plan.counts + jb.tile * 8 + warp;
+                uint32_t before = 0;
+                if (lane == 0) before = atomicAdd(arrived, 1u);
+                if (__shfl_sync(LFM_FULL_MASK, before, 0) + 1 == jb.parts) {
+                    __threadfence();
+                    if (lane == 0) *arrived = 0;
+                    auto ml = [&](uint32_t s) { return __ldcg(reinterpret_cast<const float2 *>(part_of(s) + kRows * D) + r); };
+                    float top = LFM_NO_KEY, sum = 0.0f;
+#pragma unroll 4
+                    for (uint32_t s = 0; s < jb.parts; ++s) top = fmaxf(top, ml(s).x);
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                        sum = 0.0f;
+#pragma unroll 2
+                        for (uint32_t s = 0; s < jb.parts; ++s) {
+                            const float2 x = ml(s);
+                            const float f = lfm_ex2(x.x - top);
+                            sum = __fmaf_rn(f, x.y, sum);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const float4 y = __ldcg(reinterpret_cast<const float4 *>(part_of(s)) + (size_t)(8 * c + k) * kRows + r);
+                                o[4 * k] = __fmaf_rn(f, y.x, o[4 * k]);
+                                o[4 * k + 1] = __fmaf_rn(f, y.y, o[4 * k + 1]);
+                                o[4 * k + 2] = __fmaf_rn(f, y.z, o[4 * k + 2]);
+                                o[4 * k + 3] = __fmaf_rn(f, y.w, o[4 * k + 3]);
+                            }
+                        }
+                        write(c, o, sum > 0.0f ? 1.0f / sum : 0.0f);
                     }
                 }
             }
@@ -542,19 +600,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
             const uint32_t per = part ? D / 16 : D / 2, bytes = sub * per;
             const uint32_t to = C::kOffRaw + (part ? kKeys * (D / 2) : 0) + piece * bytes;
             uint32_t w = blockIdx.x;
+            const uint64_t found = lfm_find_tile(A.bt, G, kRows, plan.above, ~0ull, bars.tile);
+            const uint32_t tiles = (uint32_t)min((uint64_t)plan.tiles, found);
             for (uint32_t it = 0; ok; ++it) {
                 /* the next job: the longest walks first (tiles from the last), all heads of one side by side */
                 Job jb;
                 jb.b = -1;
                 jb.n = 0;
-                for (; w < tiles * A.kv.hkv; w = gridDim.x + __shfl_sync(LFM_FULL_MASK, w, 0)) {
-                    lfm_find_tile(A.bt, G, kRows, 0, above, ~0ull, tiles - 1 - w / A.kv.hkv, bars.tile);
+                for (; w < tiles * A.kv.hkv * plan.parts; w = gridDim.x + __shfl_sync(LFM_FULL_MASK, w, 0)) {
+                    const uint32_t tile = w / (A.kv.hkv * plan.parts);
+                    lfm_find_tile(A.bt, G, kRows, plan.above, tiles - 1 - tile, bars.tile);
                     __syncwarp();
                     const int b = *(volatile int *)&bars.tile[0];
                     jb.row0 = (uint32_t)*(volatile int *)&bars.tile[1] * kRows;
                     jb.kvh = w % A.kv.hkv;
+                    jb.tile = tile * A.kv.hkv + jb.kvh;
+                    jb.part = w / A.kv.hkv % plan.parts;
                     __syncwarp();
-                    if (lane == 0) w = atomicAdd(count, 1u); /* of the one after */
+                    if (lane == 0) w = atomicAdd(ticket, 1u); /* of the one after */
                     if (b < 0) continue;
                     jb.q0 = A.bt.q_start[b];
                     jb.n_q = (int64_t)A.bt.q_start[b + 1] - jb.q0;
@@ -568,7 +631,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                     lfm_visible(A, jb.n_q, jb.len, jb.row0, lo0, hi0);
                     lfm_visible(A, jb.n_q, jb.len, jb.row0 + jb.rows - 1, lo1, hi1);
                     jb.blk0 = lo0 / kKeys;
-                    jb.n = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - jb.blk0) : 0;
+                    const uint32_t all = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - jb.blk0) : 0;
+                    jb.parts = min(plan.parts, max(1u, all / kPartBlocks));
+                    if (jb.part >= jb.parts) continue;
+                    const uint32_t at = (uint32_t)((uint64_t)all * jb.part / jb.parts);
+                    jb.n = (uint32_t)((uint64_t)all * (jb.part + 1) / jb.parts) - at;
+                    jb.blk0 += at;
                     jb.b = b;
                     break;
                 }
@@ -603,9 +671,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
                 base += n;
             }
             /* the last block to come here leaves the counters zero */
-            if (lane == 0 && atomicAdd(count + 1, 1u) == gridDim.x - 1) {
-                count[0] = 0;
-                count[1] = 0;
+            if (lane == 0 && atomicAdd(ticket + 1, 1u) == gridDim.x - 1) {
+                ticket[0] = 0;
+                ticket[1] = 0;
             }
         }
     }
@@ -626,27 +694,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, uint64_t 
 }
 
 template <int D>
-cudaError_t launch_tile(const AttnArgs &a, uint64_t above, uint32_t tiles, uint32_t *count, dim3 grid, cudaStream_t s, bool pdl) {
+cudaError_t launch_tile(const AttnArgs &a, const TilePlan &p, dim3 grid, cudaStream_t s, bool pdl) {
     static size_t set[2][16];
     auto fn = a.softcap > 0.0f ? k_attn_tile<D, true> : k_attn_tile<D, false>;
     const cudaError_t e = lfm_smem_attr((const void *)fn, Cfg<D>::kSmem, set[a.softcap > 0.0f]);
-    return e != cudaSuccess ? e : lfm_launch_pdl(fn, grid, dim3(kThreads), Cfg<D>::kSmem, s, pdl, a, above, tiles, count);
+    return e != cudaSuccess ? e : lfm_launch_pdl(fn, grid, dim3(kThreads), Cfg<D>::kSmem, s, pdl, a, p);
 }
 
 }  // namespace
 
-/* One for every started kRows rows of a sequence of more than `above`: at most this many. */
-uint64_t lfm_attn_tiles(const AttnArgs &a, uint64_t above) {
-    const uint64_t rows = (uint64_t)a.bt.n_tokens * a.group, most = rows / (above + 1);
-    return rows / kRows + (most < a.bt.n_seqs ? most : a.bt.n_seqs);
+TilePlan lfm_attn_tile_plan(const AttnArgs &a, uint32_t head_dim, uint64_t above, uint32_t max_kv_len, int sm_count) {
+    /* a tile for every started kRows rows of a sequence of more than `above`: at most this many */
+    const uint64_t rows = (uint64_t)a.bt.n_tokens * a.group, most = rows / (above + 1), sms = (uint64_t)sm_count;
+    TilePlan p{};
+    p.above = above;
+    p.tiles = (uint32_t)((rows + (kRows - 1) * (most < a.bt.n_seqs ? most : a.bt.n_seqs)) / kRows);
+    const uint64_t jobs = (uint64_t)p.tiles * a.kv.hkv;
+    uint64_t keys = max_kv_len;
+    if (a.window && keys > a.window + kRows / a.group) keys = a.window + kRows / a.group;
+    const uint64_t blocks = keys / kKeys + 1;
+    for (uint64_t n = 1; n == 1 || (n <= blocks / kPartBlocks && n <= LFM_ATTN_TILES && jobs * n <= LFM_ATTN_TILES && jobs * 8 <= LFM_ATTN_COUNTS - 2); ++n) {
+        const uint64_t cost = (jobs * n + sms - 1) / sms * ((blocks + n - 1) / n + kJobBlocks + (n > 1)) + (n > 1 ? n * head_dim / 128 : 0);
+        if (n == 1 || cost < p.cost) {
+            p.cost = cost;
+            p.parts = (uint32_t)n;
+        }
+    }
+    p.blocks = blocks;
+    return p;
 }
 
-cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, uint64_t above, int sm_count, uint32_t *count,
+cudaError_t lfm_launch_attn_tile(const AttnArgs &a, uint32_t head_dim, const TilePlan &plan, int sm_count, void *scratch,
                                  cudaStream_t s, bool pdl) {
-    const uint64_t tiles = lfm_attn_tiles(a, above), jobs = tiles * a.kv.hkv;
+    TilePlan p = plan;
+    const uint64_t jobs = (uint64_t)p.tiles * a.kv.hkv * p.parts;
     if (jobs == 0) return cudaSuccess;
     if (jobs > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    p.counts = static_cast<uint32_t *>(scratch);
+    p.part = reinterpret_cast<float *>(p.counts + LFM_ATTN_COUNTS);
     const dim3 grid((uint32_t)(jobs < (uint64_t)sm_count ? jobs : (uint64_t)sm_count));
-    return head_dim == 64 ? launch_tile<64>(a, above, (uint32_t)tiles, count, grid, s, pdl)
-                          : launch_tile<128>(a, above, (uint32_t)tiles, count, grid, s, pdl);
+    return head_dim == 64 ? launch_tile<64>(a, p, grid, s, pdl) : launch_tile<128>(a, p, grid, s, pdl);
 }
