@@ -218,7 +218,10 @@ def host_layer(cfg, kind, l):
 # ---------------------------------------------------------------------------
 
 def _cpu_forward(R, kind, L, x):
-    return R.moe_forward(L, x, capture=False)[0] if kind == "moe" else R.dense_forward(L, x)
+    from oracle.oracle import Reference
+    if kind != "moe":
+        return R.dense_forward(L, x)
+    return R.moe_forward(L, x, **({"capture": False} if isinstance(R, Reference) else {}))[0]
 
 
 def cpu_baseline(cfg, seconds=12.0, threads=0):
