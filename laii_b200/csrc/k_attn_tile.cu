@@ -172,7 +172,8 @@ __device__ __forceinline__ bool test(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 
-template <int D, bool kCap>
+/* kSplit: tiles in parts (an instance of its own: with the join's code in it the other one is 2% slower: prompt 132 us, 130). */
+template <int D, bool kCap, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan plan) {
     using C = Cfg<D>;
     uint32_t *const ticket = plan.counts + LFM_ATTN_COUNTS - 2;
@@ -212,7 +213,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
     __syncthreads();
     fence_after();
     lfm_pdl_wait();
-    lfm_pdl_launch_dependents();
     const uint32_t smem = lfm_smem_u32(sm);
     bool ok = true;
     /* job `it`, for all roles but the loader; false at the end */
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
             };
             /* a part: [value / 4][row] of 16 bytes, then the rows' m and sum */
             auto part_of = [&](uint32_t s) { return plan.part + ((size_t)jb.tile * plan.parts + s) * kRows * (D + 2); };
-            float *const mine = jb.parts > 1 ? part_of(jb.part) : nullptr;
+            float *const mine = kSplit && jb.parts > 1 ? part_of(jb.part) : nullptr;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t u[32];
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                 tie32(u);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
-                if (!mine) {
+                if (!kSplit || !mine) {
                     write(c, o, l > 0.0f ? 1.0f / l : 0.0f);
                 } else {
 #pragma unroll
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                                make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
                 }
             }
-            if (mine) {
+            if (kSplit && mine) {
                 /* the last warp to arrive with a part of these 32 rows joins them all, in their order */
                 __stcg(reinterpret_cast<float2 *>(mine + kRows * D) + r, make_float2(m, l));
                 __threadfence();
@@ -600,22 +600,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
             const uint32_t per = part ? D / 16 : D / 2, bytes = sub * per;
             const uint32_t to = C::kOffRaw + (part ? kKeys * (D / 2) : 0) + piece * bytes;
             uint32_t w = blockIdx.x;
-            const uint64_t found = lfm_find_tile(A.bt, G, kRows, plan.above, ~0ull, bars.tile);
-            const uint32_t tiles = (uint32_t)min((uint64_t)plan.tiles, found);
+            const uint32_t parts = kSplit ? plan.parts : 1;
+            /* parts are few rounds of the blocks: no ticket goes to a tile that is not there */
+            uint32_t tiles = plan.tiles;
+            if (kSplit) tiles = (uint32_t)min((uint64_t)tiles, lfm_find_tile(A.bt, G, kRows, plan.above, ~0ull, bars.tile));
             for (uint32_t it = 0; ok; ++it) {
                 /* the next job: the longest walks first (tiles from the last), all heads of one side by side */
                 Job jb;
                 jb.b = -1;
                 jb.n = 0;
-                for (; w < tiles * A.kv.hkv * plan.parts; w = gridDim.x + __shfl_sync(LFM_FULL_MASK, w, 0)) {
-                    const uint32_t tile = w / (A.kv.hkv * plan.parts);
+                for (; w < tiles * A.kv.hkv * parts; w = gridDim.x + __shfl_sync(LFM_FULL_MASK, w, 0)) {
+                    const uint32_t tile = w / (A.kv.hkv * parts);
                     lfm_find_tile(A.bt, G, kRows, plan.above, tiles - 1 - tile, bars.tile);
                     __syncwarp();
                     const int b = *(volatile int *)&bars.tile[0];
                     jb.row0 = (uint32_t)*(volatile int *)&bars.tile[1] * kRows;
                     jb.kvh = w % A.kv.hkv;
-                    jb.tile = tile * A.kv.hkv + jb.kvh;
-                    jb.part = w / A.kv.hkv % plan.parts;
+                    const uint32_t part = w / A.kv.hkv % parts;
                     __syncwarp();
                     if (lane == 0) w = atomicAdd(ticket, 1u); /* of the one after */
                     if (b < 0) continue;
@@ -631,12 +632,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                     lfm_visible(A, jb.n_q, jb.len, jb.row0, lo0, hi0);
                     lfm_visible(A, jb.n_q, jb.len, jb.row0 + jb.rows - 1, lo1, hi1);
                     jb.blk0 = lo0 / kKeys;
-                    const uint32_t all = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - jb.blk0) : 0;
-                    jb.parts = min(plan.parts, max(1u, all / kPartBlocks));
-                    if (jb.part >= jb.parts) continue;
-                    const uint32_t at = (uint32_t)((uint64_t)all * jb.part / jb.parts);
-                    jb.n = (uint32_t)((uint64_t)all * (jb.part + 1) / jb.parts) - at;
-                    jb.blk0 += at;
+                    jb.n = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - jb.blk0) : 0;
+                    if (kSplit) {
+                        jb.tile = tile * A.kv.hkv + jb.kvh;
+                        jb.part = part;
+                        jb.parts = min(parts, max(1u, jb.n / kPartBlocks));
+                        if (part >= jb.parts) continue;
+                        const uint32_t at = (uint32_t)((uint64_t)jb.n * part / jb.parts);
+                        jb.n = (uint32_t)((uint64_t)jb.n * (part + 1) / jb.parts) - at;
+                        jb.blk0 += at;
+                    }
                     jb.b = b;
                     break;
                 }
@@ -695,9 +700,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
 
 template <int D>
 cudaError_t launch_tile(const AttnArgs &a, const TilePlan &p, dim3 grid, cudaStream_t s, bool pdl) {
-    static size_t set[2][16];
-    auto fn = a.softcap > 0.0f ? k_attn_tile<D, true> : k_attn_tile<D, false>;
-    const cudaError_t e = lfm_smem_attr((const void *)fn, Cfg<D>::kSmem, set[a.softcap > 0.0f]);
+    static size_t set[4][16];
+    const bool cap = a.softcap > 0.0f, split = p.parts > 1;
+    auto fn = split ? (cap ? k_attn_tile<D, true, true> : k_attn_tile<D, false, true>)
+                    : (cap ? k_attn_tile<D, true, false> : k_attn_tile<D, false, false>);
+    const cudaError_t e = lfm_smem_attr((const void *)fn, Cfg<D>::kSmem, set[2 * split + cap]);
     return e != cudaSuccess ? e : lfm_launch_pdl(fn, grid, dim3(kThreads), Cfg<D>::kSmem, s, pdl, a, p);
 }
 
