@@ -107,15 +107,17 @@ class GpuAttn:
         self.moe = moe
         self.index = moe.device
         self.device = torch.device("cuda", moe.device)
-        self._lib = _native.load_gpu()
-
-    def _check(self, st: int):
-        if st != 0:
-            raise MoEError(st, self._lib.lfm_gpu_moe_last_error(self.moe._h).decode(errors="replace"))
+        self._lib = lib = _native.load_gpu()
+        # a small call is as long as its way through Python: looked up once
+        self._norm, self._read_q8, self._append = lib.lfm_gpu_add_rmsnorm, lib.lfm_gpu_q8k_read, lib.lfm_gpu_kv_append
+        self._read, self._attend = lib.lfm_gpu_kv_read, lib.lfm_gpu_attn_forward
 
     def _stream(self) -> int:
         # the address alone: building torch's Stream object takes as long as a launch
         return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def _fail(self, st: int):
+        raise MoEError(st, self._lib.lfm_gpu_moe_last_error(self.moe._h).decode(errors="replace"))
 
     def _rows(self, t: torch.Tensor, what: str, heads: Optional[int], dim: int, dtype) -> int:
         """Address of rows [tokens, heads, dim]."""
@@ -138,25 +140,35 @@ class GpuAttn:
         x fp32 [T, D]; x_out may be x (in place)."""
         dev = self.index
         xp = _dense(x, "x", torch.float32, dev, 2)
-        T, D = x.shape
-        dp, dt = None, 0
+        shape = T, D = x.shape
+        dp = wp = bp = qp = xb = qb = None
+        dt = bt = 0
         if delta is not None:
             dt = _type(delta.dtype, "delta")
             dp = _dense(delta, "delta", delta.dtype, dev, 2)
-            if delta.shape != x.shape:
+            if delta.shape != shape:
                 raise ValueError("delta must have the shape of x")
-        if weight is not None and weight.numel() != D:
-            raise ValueError(f"weight must have {D} values")
+        if weight is not None:
+            wp = _dense(weight, "weight", torch.float32, dev, 1)
+            if weight.shape[0] != D:
+                raise ValueError(f"weight must have {D} values")
         if x_out is None:
             x_out = torch.empty_like(x)
-        elif x_out.shape != x.shape:
-            raise ValueError("x_out must have the shape of x")
-        xb = x.new_empty((T, D), dtype=xb_dtype) if xb_dtype is not None else None
-        qb = x.new_empty((T, D // 256, Q8K_BYTES), dtype=torch.uint8) if q8 else None
-        self._check(self._lib.lfm_gpu_add_rmsnorm(
-            self.moe._h, xp, dp, dt, T, D, _dense(weight, "weight", torch.float32, dev, 1), eps,
-            _dense(x_out, "x_out", torch.float32, dev, 2), None if xb is None else xb.data_ptr(),
-            0 if xb is None else _type(xb_dtype, "xb_dtype"), None if qb is None else qb.data_ptr(), self._stream()))
+            op = x_out.data_ptr()
+        else:
+            op = _dense(x_out, "x_out", torch.float32, dev, 2)
+            if x_out.shape != shape:
+                raise ValueError("x_out must have the shape of x")
+        if xb_dtype is not None:
+            bt = _type(xb_dtype, "xb_dtype")
+            xb = x.new_empty(shape, dtype=xb_dtype)
+            bp = xb.data_ptr()
+        if q8:
+            qb = x.new_empty((T, D // 256, Q8K_BYTES), dtype=torch.uint8)
+            qp = qb.data_ptr()
+        st = self._norm(self.moe._h, xp, dp, dt, T, D, wp, eps, op, bp, bt, qp, self._stream())
+        if st:
+            self._fail(st)
         return x_out, xb, qb
 
     def read_q8(self, q8: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -166,8 +178,9 @@ class GpuAttn:
         if size != Q8K_BYTES:
             raise ValueError(f"q8 must be [T, D / 256, {Q8K_BYTES}]")
         out = q8.new_empty((T, n * 256), dtype=dtype)
-        self._check(self._lib.lfm_gpu_q8k_read(self.moe._h, p, T, n * 256, _type(dtype, "dtype"), out.data_ptr(),
-                                               self._stream()))
+        st = self._read_q8(self.moe._h, p, T, n * 256, _type(dtype, "dtype"), out.data_ptr(), self._stream())
+        if st:
+            self._fail(st)
         return out
 
     # -- the cache ----------------------------------------------------------
@@ -187,10 +200,12 @@ class GpuAttn:
             qs = q.stride(0) if T != 1 else heads * d  # the stride of one row says nothing
             if q_out is None:
                 q_out = q.new_empty(q.shape)
-            elif q_out.shape[0] < T:
-                raise ValueError("q_out must have the rows of q")
-            op = self._rows(q_out, "q_out", heads, d, dt)
-            os_ = q_out.stride(0) if q_out.shape[0] != 1 else heads * d
+                op, os_ = q_out.data_ptr(), heads * d
+            else:
+                if q_out.shape[0] < T:
+                    raise ValueError("q_out must have the rows of q")
+                op = self._rows(q_out, "q_out", heads, d, dt)
+                os_ = q_out.stride(0) if q_out.shape[0] != 1 else heads * d
         if k is not None:
             kp, vp = self._rows(k, "k", cache.n_kv_heads, d, dt), self._rows(v, "v", cache.n_kv_heads, d, dt)
             ks, vs = (k.stride(0), v.stride(0)) if T != 1 else (cache.n_kv_heads * d,) * 2
@@ -198,9 +213,10 @@ class GpuAttn:
                 raise ValueError("q, k and v must have the same number of tokens")
         if rope is not None and (rope.norm_dim - {d} or (rope.index >= 0 and rope.index != self.index)):
             raise ValueError(f"q_norm and k_norm must have {d} values, rotation and norms be on {self.device}")
-        self._check(self._lib.lfm_gpu_kv_append(
-            self.moe._h, cache._ref, batch.rows(T), None if rope is None else rope._ref, _type(dt, "q"), heads, qp, qs, op, os_,
-            kp, ks, vp, vs, self._stream()))
+        st = self._append(self.moe._h, cache._ref, batch.rows(T), None if rope is None else rope._ref, _type(dt, "q"), heads, qp,
+                          qs, op, os_, kp, ks, vp, vs, self._stream())
+        if st:
+            self._fail(st)
         return q_out
 
     def read(self, cache: KVPages, batch: KVBatch, n_tokens: int, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -208,8 +224,10 @@ class GpuAttn:
         self._same_device(cache, batch)
         kv = cache.pages.new_empty((2, n_tokens, cache.n_kv_heads, cache.head_dim), dtype=dtype)
         k, v = kv.unbind(0)
-        self._check(self._lib.lfm_gpu_kv_read(self.moe._h, cache._ref, batch.rows(n_tokens), _type(dtype, "dtype"),
-                                              k.data_ptr(), v.data_ptr(), self._stream()))
+        st = self._read(self.moe._h, cache._ref, batch.rows(n_tokens), _type(dtype, "dtype"), k.data_ptr(), v.data_ptr(),
+                        self._stream())
+        if st:
+            self._fail(st)
         return k, v
 
     # -- attention ------------------------------------------------------------
@@ -222,15 +240,20 @@ class GpuAttn:
         T, heads, _ = shape = q.shape
         if out is None:
             out = q.new_empty(shape)
-        elif out.shape[0] < T:
-            raise ValueError("out must have the rows of q")
-        op = self._rows(out, "out", heads, d, dt)
-        self._check(self._lib.lfm_gpu_attn_forward(
-            self.moe._h, cache._ref, batch.rows(T), heads, d ** -0.5 if scale is None else scale, causal, window, softcap,
-            _type(dt, "q"), qp, q.stride(0) if T != 1 else heads * d, op, out.stride(0) if out.shape[0] != 1 else heads * d,
-            self._stream()))
+            op, os_ = out.data_ptr(), heads * d
+        else:
+            if out.shape[0] < T:
+                raise ValueError("out must have the rows of q")
+            op = self._rows(out, "out", heads, d, dt)
+            os_ = out.stride(0) if out.shape[0] != 1 else heads * d
+        st = self._attend(self.moe._h, cache._ref, batch.rows(T), heads, d ** -0.5 if scale is None else scale, causal, window,
+                          softcap, _type(dt, "q"), qp, q.stride(0) if T != 1 else heads * d, op, os_, self._stream())
+        if st:
+            self._fail(st)
         return out
 
     def reserve(self):
         """Allocate attend's scratch now (needed before a stream capture)."""
-        self._check(self._lib.lfm_gpu_attn_reserve(self.moe._h))
+        st = self._lib.lfm_gpu_attn_reserve(self.moe._h)
+        if st:
+            self._fail(st)
