@@ -134,7 +134,7 @@ lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv_t *kv, 
                                       void *stream);
 
 /* Allocate the scratch in which lfm_gpu_attn_forward joins the parts of long
- * sequences (a fixed size per handle).  The first forward does it otherwise,
+ * sequences (79 MB per handle, whatever is asked later).  The first forward does it otherwise,
  * which a stream capture does not allow.  Calls on several streams are ordered
  * among each other where they share the scratch; replays of captured calls are
  * not: replay one graph at a time per handle. */

@@ -18,10 +18,21 @@
  *   - P: e^(z - m) in fp16 as the B fragment, transposed by movmatrix.  m only
  *     moves when a score passes it by 2^8, so p <= 256, and the sum is fp32.
  * A warp takes 4608-byte blocks of keys and values (64 keys of 64 values, 32 of
- * 128) through its own ring of bulk copies; the eight warps of a block split
- * the keys and are joined in shared memory, blocks that split a long sequence
- * through scratch: the last to finish joins the parts in their order (the same
- * bits on every run).
+ * 128) through its own ring of bulk copies.  All (tile of columns, kv head)
+ * units' blocks of keys lie in a row that is cut into equal parts, one for each
+ * block that the GPU holds at once, whatever the lengths; its four warps take
+ * the part's key blocks in turn and are joined in shared memory, the parts of a
+ * unit through scratch: the last to finish joins them in their order (the same
+ * bits on every run).  A block for each unit and a ring through its keys, which
+ * leaves the longest sequence to one SM, took 92 us where equal parts take 73
+ * (64 sequences of up to 8192 keys).
+ *
+ * Bound by instruction issue: a step of 16 keys is some 220 instructions of a
+ * warp, unpacking above all, for 1152 bytes.  32 / 8 heads, 64-value heads, 64
+ * tokens on ragged sequences of up to 8192 keys: 62 us, 187 MB read, 3.0 TB/s;
+ * issue 56%, HBM 34 to 47%.  128-value heads, two sequences of 131072 keys:
+ * 83 us, 302 MB, 3.6 TB/s.  One token on 1024 keys: 9.2 us, a chain of table, copy,
+ * products and join.  Eight tokens of each of 16 sequences of up to 8192 keys: 45 us.
  */
 #include <type_traits>
 
@@ -211,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
         }
         return v;
     };
-    uint64_t w = 0; /* this thread's sequence of the last 256 looked at */
+    uint64_t w = 0; /* this thread's sequence of the last kThreads looked at */
     {
         uint64_t sum = 0;
         uint32_t units = 0;
@@ -242,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
     /* blocks at work: a block of keys for each warp, or one for each unit where units are shorter */
     uint64_t n_cta = min((uint64_t)gridDim.x, max((total + kWarps - 1) / kWarps, (uint64_t)units));
     /* units that are all alike: cuts that fall between them, where that leaves few blocks idle.  A block that ends one
-     * unit and begins another loads q and joins twice */
+     * unit and begins another loads q and joins twice (256 rows on 2048 keys, 8 kv heads: 31 us, 21 so) */
     if (units && units <= n_cta && total % units == 0 && 4 * (n_cta / units * units) >= 3 * n_cta) n_cta = n_cta / units * units;
     if (blockIdx.x >= n_cta) return;
     uint64_t x = total * blockIdx.x / n_cta;
@@ -678,10 +689,13 @@ cudaError_t launch_rows(const AttnArgs &a, const RowsPlan &p, dim3 grid, cudaStr
 static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, uint64_t few, uint32_t max_kv_len,
                                         int sm_count, void *scratch, cudaStream_t s, bool pdl) {
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, G = a.group, keys = head_dim == 64 ? 64 : 32;
-    /* columns of a tile: what an average sequence fills, as far as registers go */
+    /* columns of a tile: what an average sequence fills, as far as registers go.  16 sequences of 8192 keys, 64-value
+     * heads, 8 / 16 / 32 columns: 4 rows 31, 38, 56 us; 12 rows 49, 42, 61; 24 rows 67, 67, 64; 64 rows 154, 117, 106.
+     * 128-value heads, 8 / 16: 4 rows 52, 66; 12 rows 88, 75; 64 rows 300, 226 */
     const uint64_t per = (T + B - 1) / B * G;
     const uint32_t nt = per <= 8 ? 1 : per <= 16 || head_dim == 128 ? 2 : 4;
-    /* blocks: as many as run at once, fewer where there are not enough blocks of keys by the hint */
+    /* blocks: as many as run at once (registers: more, with spills, ran slower), fewer where there are not enough
+     * blocks of keys by the hint */
     uint64_t grid = (uint64_t)sm_count * (head_dim * nt < 128 ? 4 : head_dim * nt == 128 ? 3 : 2);
     const uint64_t units = (B + T * G / (8 * nt)) * a.kv.hkv, work = units * ((max_kv_len + keys - 1) / keys + 1);
     const uint64_t most = work / kWarps > units ? work / kWarps : units;

@@ -22,9 +22,26 @@
  *             (p <= 256 in fp16); then the thread scales its row of O in TMEM
  * The blocks are persistent, one an SM, and take the tiles from a counter, the
  * longest first: loader and dequantisation run ahead into the next tile while
- * the softmax warps finish one.
+ * the softmax warps finish one.  Few tiles of long walks have their keys split
+ * into parts, tickets of their own, which leave O unscaled, m and the sum in
+ * scratch; for each 32 rows the last warp to arrive joins them in their order,
+ * the same bits on every run.
  * O in TMEM is scaled by 1 / sum at the end.  Rows that end early in a block
  * and slots that hold no token are masked in S; values of such slots are zero.
+ *
+ * Keys and values enter as fp16 products d * (code - 8), rounded once (2^-12
+ * relative, under the output's rounding and q's own); scores, m, the sum and O
+ * are fp32, p is fp16 <= 256.
+ *
+ * 32 / 8 heads.  4096 tokens from the beginning, 64-value heads: 130 us, 530
+ * TFLOP/s; 42 us of tensor work, 60 of exponentials (one a score, 16 a clock and
+ * SM).  2048 tokens behind 14336, 128-value heads: 540 us call after call, 580
+ * with other work between, 950 and 890 TFLOP/s; 314 of tensor work.  What is
+ * between is the hand-over from role to role for each block: tensor pipe 51%,
+ * exponential unit 51%, issue 50% for 128-value heads (25, 50, 45 for 64), and
+ * without the softmax's arithmetic the same barriers take 91 and 344 us.
+ * The few-row kernel's fragments in registers took 696 and 3469 us, a block's
+ * barriers for 128 keys at a time 141 and 646 when 64 took 138 and 595.  512 rows on 16384 keys: 50 us, in one part 245.
  */
 #include <type_traits>
 
@@ -35,7 +52,8 @@ namespace {
 constexpr int kM = 128, kRows = 2 * kM, kKeys = 64, kThreads = 512;
 constexpr uint32_t kChunkQ = kM * 16, kChunk = kKeys * 16; /* bytes between the 8-value chunks of a row */
 
-/* Key blocks that a part of a split tile has at least; what a tile costs beside its blocks, in blocks. */
+/* Key blocks that a part of a split tile has at least; what a tile costs beside its blocks, in blocks (32 blocks in 44
+ * us, 256 in 245: 1.1 us a block and 8 us). */
 constexpr uint32_t kPartBlocks = 8, kJobBlocks = 6;
 
 template <int D>
@@ -172,7 +190,8 @@ __device__ __forceinline__ bool test(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 
-/* kSplit: tiles in parts (an instance of its own: with the join's code in it the other one is 2% slower: prompt 132 us, 130). */
+/* kSplit: tiles in parts (an instance of its own: with the join's code in it the other one is 2% slower: prompt 132 us,
+ * 130). */
 template <int D, bool kCap, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan plan) {
     using C = Cfg<D>;
@@ -229,253 +248,259 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 152;"); /* 256 x 152 + 256 x 104 = 512 x 128 */
         const uint32_t h = warp >> 2, r = h * kM + (warp & 3) * 32 + lane, tmem = bars.tmem;
-      for (uint32_t it = 0; take(it); ++it) {
-        const Job &jb = bars.job[it & 1];
-        const uint32_t n = jb.n;
-        /* this thread's row of q or out */
-        auto row_at = [&](size_t stride) {
-            const uint32_t row = jb.row0 + r;
-            return (size_t)(jb.q0 + row / G) * stride + ((size_t)jb.kvh * G + row % G) * D;
-        };
-        if (n == 0) { /* no key for any row */
-            if (r < jb.rows) {
-                const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                const size_t at = row_at(A.out_stride);
-                for (int c = 0; c < D; c += 8) {
-                    if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + at + c, z);
-                    else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + at + c, z);
-                    else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + at + c, z);
-                }
-            }
-            drop(it);
-            continue;
-        }
-        {
-            /* values 8 v .. + 7 and 32 + 8 v .. + 7 of a span make chunks 2 v and 2 v + 1; the last job's products,
-             * waited for below, are done with the space */
-            const bool on = r < jb.rows;
-            const size_t at = on ? row_at(A.q_stride) : 0;
-            uint8_t *to = sm + h * C::kQ + (r % kM) * 16;
-            const bool neg = A.scale < 0.0f;
-            auto load = [&](const auto *q) { /* the type is told apart once, so the loads are under way together */
-#pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (on) {
-                        lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3), x);
-                        lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3) + 32, y);
-                    }
-                    lfm_fit_q(neg, x);
-                    lfm_fit_q(neg, y);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        *reinterpret_cast<uint4 *>(to + (2 * c + k) * kChunkQ) =
-                            make_uint4(lfm_pack2(x[4 * k], y[4 * k], __half()), lfm_pack2(x[4 * k + 1], y[4 * k + 1], __half()),
-                                       lfm_pack2(x[4 * k + 2], y[4 * k + 2], __half()), lfm_pack2(x[4 * k + 3], y[4 * k + 3], __half()));
-                }
+        for (uint32_t it = 0; take(it); ++it) {
+            const Job &jb = bars.job[it & 1];
+            const uint32_t n = jb.n;
+            /* this thread's row of q or out */
+            auto row_at = [&](size_t stride) {
+                const uint32_t row = jb.row0 + r;
+                return (size_t)(jb.q0 + row / G) * stride + ((size_t)jb.kvh * G + row % G) * D;
             };
-            if (A.type == 0) load(static_cast<const float *>(A.q));
-            else if (A.type == 1) load(static_cast<const __half *>(A.q));
-            else load(static_cast<const __nv_bfloat16 *>(A.q));
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) lfm_mbar_arrive(&bars.q_full[h]);
-        }
-        const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
-        const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
-        const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
-        /* what the row sees, in keys from the first block; the blocks [inside0, inside1) every row of the tile sees whole */
-        int lo = 0, hi = 0, inside0 = 0, inside1 = 0;
-        {
-            int64_t a = 0, e = 0, a_all = 0, e_all = 0, unused;
-            if (r < jb.rows) lfm_visible(A, jb.n_q, jb.len, jb.row0 + r, a, e);
-            if (h * kM < jb.rows) {
-                lfm_visible(A, jb.n_q, jb.len, jb.row0 + h * kM, unused, e_all);
-                lfm_visible(A, jb.n_q, jb.len, jb.row0 + min(jb.rows, (h + 1) * kM) - 1, a_all, unused);
+            if (n == 0) { /* no key for any row */
+                if (r < jb.rows) {
+                    const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    const size_t at = row_at(A.out_stride);
+                    for (int c = 0; c < D; c += 8) {
+                        if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + at + c, z);
+                        else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + at + c, z);
+                        else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + at + c, z);
+                    }
+                }
+                drop(it);
+                continue;
             }
-            const int64_t key0 = jb.blk0 * kKeys; /* positions are below 2^31 */
-            lo = (int)max((int64_t)0, a - key0);
-            hi = (int)max((int64_t)0, e - key0);
-            inside0 = (int)((max((int64_t)0, a_all - key0) + kKeys - 1) / kKeys);
-            inside1 = (int)(max((int64_t)0, e_all - key0) / kKeys);
-        }
-        const uint64_t sc2 = pk2(__float_as_uint(sc), __float_as_uint(sc));
-        /* O holds the products of block j.  A barrier's parity tells two phases apart: with the scores of block
-         * j + 1 the products of j - 2 are done (kBufs <= 6), so those of j and j - 1 take a barrier each, in turn */
-        auto products = [&](uint32_t j) {
-            return __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h][(base + j) & 1], ((base + j) >> 1) & 1, abort, A.err));
-        };
-        float m = LFM_NO_KEY;
-        uint64_t l2 = 0;
-        for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t q = 2 * (base + j) + h, buf = q % C::kBufs;
-            const uint32_t tS = tmem + buf * kColS + ((warp & 3) << 21);
-            ok = __all_sync(LFM_FULL_MASK, wait(&bars.s_full[buf], (q / C::kBufs) & 1, abort, A.err));
-            if (!ok) break;
-            fence_after();
-            const bool masked = (int)j < inside0 || (int)j >= inside1;
-            const int from = lo - (int)j * kKeys, to = hi - (int)j * kKeys;
-            uint32_t x[kKeys];
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            ld32(tS, x);
-            ld32(tS + 32, x + 32);
-            wait_ld();
-            tie32(x);
-            tie32(x + 32);
-            if (kCap) { /* tanh(x) = 1 - 2 / (1 + e^2x) */
+            {
+                /* values 8 v .. + 7 and 32 + 8 v .. + 7 of a span make chunks 2 v and 2 v + 1; the last job's products,
+                 * waited for below, are done with the space */
+                const bool on = r < jb.rows;
+                const size_t at = on ? row_at(A.q_stride) : 0;
+                uint8_t *to = sm + h * C::kQ + (r % kM) * 16;
+                const bool neg = A.scale < 0.0f;
+                auto load = [&](const auto *q) { /* the type is told apart once, so the loads are under way together */
 #pragma unroll
-                for (int i = 0; i < kKeys; ++i)
-                    x[i] = __float_as_uint(__fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(__uint_as_float(x[i]) * capz)), 1.0f));
-            }
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < kKeys; ++i)
-                    if (i < from || i >= to) x[i] = 0xFF800000u;
-            }
-#pragma unroll
-            for (int i = 0; i < kKeys; i += 8) {
-                max3(mx[0], x[i], x[i + 1]);
-                max3(mx[1], x[i + 2], x[i + 3]);
-                max3(mx[2], x[i + 4], x[i + 5]);
-                max3(mx[3], x[i + 6], x[i + 7]);
-            }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            if (__any_sync(LFM_FULL_MASK, __fmaf_rn(top, sc, -m) > 8.0f)) {
-                const float nm = fmaxf(m, top * sc), f = lfm_ex2(m - nm);
-                const uint64_t f2 = pk2(__float_as_uint(f), __float_as_uint(f));
-                m = nm;
-                l2 = mul2(l2, f2);
-                if (j) { /* the products of the block before are in O first */
-                    ok = products(j - 1);
-                    if (!ok) break;
-                    fence_after();
-#pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        ld32(tO + c, o);
-                        wait_ld();
-                        tie32(o);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const uint64_t x = mul2(pk2(o[i], o[i + 1]), f2);
-                            o[i] = (uint32_t)x;
-                            o[i + 1] = (uint32_t)(x >> 32);
+                    for (int c = 0; c < D / 16; ++c) {
+                        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                        if (on) {
+                            lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3), x);
+                            lfm_load<8>(q + at + 64 * (c >> 2) + 8 * (c & 3) + 32, y);
                         }
-                        st32(tO + c, o);
+                        lfm_fit_q(neg, x);
+                        lfm_fit_q(neg, y);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            *reinterpret_cast<uint4 *>(to + (2 * c + k) * kChunkQ) =
+                                make_uint4(lfm_pack2(x[4 * k], y[4 * k], __half()),
+                                           lfm_pack2(x[4 * k + 1], y[4 * k + 1], __half()),
+                                           lfm_pack2(x[4 * k + 2], y[4 * k + 2], __half()),
+                                           lfm_pack2(x[4 * k + 3], y[4 * k + 3], __half()));
                     }
-                }
-            }
-            const uint64_t nm2 = pk2(__float_as_uint(-m), __float_as_uint(-m));
-            uint64_t la = 0;
-            /* each operation on all before the next one: the exponentials' latency hides behind one another */
-#pragma unroll
-            for (int i = 0; i < kKeys; i += 2) {
-                const uint64_t z = fma2(pk2(x[i], x[i + 1]), sc2, nm2);
-                x[i] = (uint32_t)z;
-                x[i + 1] = (uint32_t)(z >> 32);
-            }
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[i]));
-#pragma unroll
-            for (int i = 0; i < kKeys; i += 2) {
-                if (i & 2) la = add2(la, pk2(x[i], x[i + 1]));
-                else l2 = add2(l2, pk2(x[i], x[i + 1]));
-                x[i / 2] = lfm_pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __half());
-            }
-            l2 = add2(l2, la);
-            st32(tS, x);
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) lfm_mbar_arrive(&bars.p_full[buf]);
-        }
-        /* the barrier of the last products may still be two of its phases back: the one before goes first */
-        if (ok && n > 1) ok = products(n - 2);
-        if (ok) ok = products(n - 1);
-        if (!ok) break;
-        {
-            fence_after();
-            const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
-            const bool on = r < jb.rows;
-            const size_t at = on ? row_at(A.out_stride) : 0;
-            /* columns 32 c ..: values 16 k .. + 15 of the span in the even ones, 32 + 16 k .. in the odd ones */
-            auto write = [&](int c, const float *o, float inv) {
-                if (!on) return;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = o[2 * (8 * (e & 1) + i) + (e >> 1)] * inv;
-                    const size_t to = at + 64 * (c >> 1) + 16 * (c & 1) + 8 * (e & 1) + 32 * (e >> 1);
-                    if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + to, v);
-                    else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + to, v);
-                    else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + to, v);
-                }
-            };
-            /* a part: [value / 4][row] of 16 bytes, then the rows' m and sum */
-            auto part_of = [&](uint32_t s) { return plan.part + ((size_t)jb.tile * plan.parts + s) * kRows * (D + 2); };
-            float *const mine = kSplit && jb.parts > 1 ? part_of(jb.part) : nullptr;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t u[32];
-                float o[32];
-                ld32(tO + 32 * c, u);
-                wait_ld();
-                tie32(u);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
-                if (!kSplit || !mine) {
-                    write(c, o, l > 0.0f ? 1.0f / l : 0.0f);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        __stcg(reinterpret_cast<float4 *>(mine) + (size_t)(8 * c + k) * kRows + r,
-                               make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
-                }
-            }
-            if (kSplit && mine) {
-                /* the last warp to arrive with a part of these 32 rows joins them all, in their order */
-                __stcg(reinterpret_cast<float2 *>(mine + kRows * D) + r, make_float2(m, l));
-                __threadfence();
+                };
+                if (A.type == 0) load(static_cast<const float *>(A.q));
+                else if (A.type == 1) load(static_cast<const __half *>(A.q));
+                else load(static_cast<const __nv_bfloat16 *>(A.q));
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                uint32_t *const arrived = plan.counts + jb.tile * 8 + warp;
-                uint32_t before = 0;
-                if (lane == 0) before = atomicAdd(arrived, 1u);
-                if (__shfl_sync(LFM_FULL_MASK, before, 0) + 1 == jb.parts) {
-                    __threadfence();
-                    if (lane == 0) *arrived = 0;
-                    auto ml = [&](uint32_t s) { return __ldcg(reinterpret_cast<const float2 *>(part_of(s) + kRows * D) + r); };
-                    float top = LFM_NO_KEY, sum = 0.0f;
-#pragma unroll 4
-                    for (uint32_t s = 0; s < jb.parts; ++s) top = fmaxf(top, ml(s).x);
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
+                if (lane == 0) lfm_mbar_arrive(&bars.q_full[h]);
+            }
+            const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
+            const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
+            const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
+            /* what the row sees, in keys from the first block; the blocks [inside0, inside1) every row of the tile sees
+             * whole */
+            int lo = 0, hi = 0, inside0 = 0, inside1 = 0;
+            {
+                int64_t a = 0, e = 0, a_all = 0, e_all = 0, unused;
+                if (r < jb.rows) lfm_visible(A, jb.n_q, jb.len, jb.row0 + r, a, e);
+                if (h * kM < jb.rows) {
+                    lfm_visible(A, jb.n_q, jb.len, jb.row0 + h * kM, unused, e_all);
+                    lfm_visible(A, jb.n_q, jb.len, jb.row0 + min(jb.rows, (h + 1) * kM) - 1, a_all, unused);
+                }
+                const int64_t key0 = jb.blk0 * kKeys; /* positions are below 2^31 */
+                lo = (int)max((int64_t)0, a - key0);
+                hi = (int)max((int64_t)0, e - key0);
+                inside0 = (int)((max((int64_t)0, a_all - key0) + kKeys - 1) / kKeys);
+                inside1 = (int)(max((int64_t)0, e_all - key0) / kKeys);
+            }
+            const uint64_t sc2 = pk2(__float_as_uint(sc), __float_as_uint(sc));
+            /* O holds the products of block j.  A barrier's parity tells two phases apart: with the scores of block
+             * j + 1 the products of j - 2 are done (kBufs <= 6), so those of j and j - 1 take a barrier each, in turn */
+            auto products = [&](uint32_t j) {
+                return __all_sync(LFM_FULL_MASK, wait(&bars.o_full[h][(base + j) & 1], ((base + j) >> 1) & 1, abort, A.err));
+            };
+            float m = LFM_NO_KEY;
+            uint64_t l2 = 0;
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t q = 2 * (base + j) + h, buf = q % C::kBufs;
+                const uint32_t tS = tmem + buf * kColS + ((warp & 3) << 21);
+                ok = __all_sync(LFM_FULL_MASK, wait(&bars.s_full[buf], (q / C::kBufs) & 1, abort, A.err));
+                if (!ok) break;
+                fence_after();
+                const bool masked = (int)j < inside0 || (int)j >= inside1;
+                const int from = lo - (int)j * kKeys, to = hi - (int)j * kKeys;
+                uint32_t x[kKeys];
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                ld32(tS, x);
+                ld32(tS + 32, x + 32);
+                wait_ld();
+                tie32(x);
+                tie32(x + 32);
+                if (kCap) { /* tanh(x) = 1 - 2 / (1 + e^2x) */
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0.0f;
-                        sum = 0.0f;
-#pragma unroll 2
-                        for (uint32_t s = 0; s < jb.parts; ++s) {
-                            const float2 x = ml(s);
-                            const float f = lfm_ex2(x.x - top);
-                            sum = __fmaf_rn(f, x.y, sum);
+                    for (int i = 0; i < kKeys; ++i)
+                        x[i] = __float_as_uint(__fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(__uint_as_float(x[i]) * capz)), 1.0f));
+                }
+                if (masked) {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                const float4 y = __ldcg(reinterpret_cast<const float4 *>(part_of(s)) + (size_t)(8 * c + k) * kRows + r);
-                                o[4 * k] = __fmaf_rn(f, y.x, o[4 * k]);
-                                o[4 * k + 1] = __fmaf_rn(f, y.y, o[4 * k + 1]);
-                                o[4 * k + 2] = __fmaf_rn(f, y.z, o[4 * k + 2]);
-                                o[4 * k + 3] = __fmaf_rn(f, y.w, o[4 * k + 3]);
+                    for (int i = 0; i < kKeys; ++i)
+                        if (i < from || i >= to) x[i] = 0xFF800000u;
+                }
+#pragma unroll
+                for (int i = 0; i < kKeys; i += 8) {
+                    max3(mx[0], x[i], x[i + 1]);
+                    max3(mx[1], x[i + 2], x[i + 3]);
+                    max3(mx[2], x[i + 4], x[i + 5]);
+                    max3(mx[3], x[i + 6], x[i + 7]);
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (__any_sync(LFM_FULL_MASK, __fmaf_rn(top, sc, -m) > 8.0f)) {
+                    const float nm = fmaxf(m, top * sc), f = lfm_ex2(m - nm);
+                    const uint64_t f2 = pk2(__float_as_uint(f), __float_as_uint(f));
+                    m = nm;
+                    l2 = mul2(l2, f2);
+                    if (j) { /* the products of the block before are in O first */
+                        ok = products(j - 1);
+                        if (!ok) break;
+                        fence_after();
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            ld32(tO + c, o);
+                            wait_ld();
+                            tie32(o);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const uint64_t x = mul2(pk2(o[i], o[i + 1]), f2);
+                                o[i] = (uint32_t)x;
+                                o[i + 1] = (uint32_t)(x >> 32);
                             }
+                            st32(tO + c, o);
                         }
-                        write(c, o, sum > 0.0f ? 1.0f / sum : 0.0f);
+                    }
+                }
+                const uint64_t nm2 = pk2(__float_as_uint(-m), __float_as_uint(-m));
+                uint64_t la = 0;
+                /* each operation on all before the next one: the exponentials' latency hides behind one another */
+#pragma unroll
+                for (int i = 0; i < kKeys; i += 2) {
+                    const uint64_t z = fma2(pk2(x[i], x[i + 1]), sc2, nm2);
+                    x[i] = (uint32_t)z;
+                    x[i + 1] = (uint32_t)(z >> 32);
+                }
+#pragma unroll
+                for (int i = 0; i < kKeys; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[i]));
+#pragma unroll
+                for (int i = 0; i < kKeys; i += 2) {
+                    if (i & 2) la = add2(la, pk2(x[i], x[i + 1]));
+                    else l2 = add2(l2, pk2(x[i], x[i + 1]));
+                    x[i / 2] = lfm_pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __half());
+                }
+                l2 = add2(l2, la);
+                st32(tS, x);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) lfm_mbar_arrive(&bars.p_full[buf]);
+            }
+            /* the barrier of the last products may still be two of its phases back: the one before goes first */
+            if (ok && n > 1) ok = products(n - 2);
+            if (ok) ok = products(n - 1);
+            if (!ok) break;
+            {
+                fence_after();
+                const float l = __uint_as_float((uint32_t)l2) + __uint_as_float((uint32_t)(l2 >> 32));
+                const bool on = r < jb.rows;
+                const size_t at = on ? row_at(A.out_stride) : 0;
+                /* columns 32 c ..: values 16 k .. + 15 of the span in the even ones, 32 + 16 k .. in the odd ones */
+                auto write = [&](int c, const float *o, float inv) {
+                    if (!on) return;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = o[2 * (8 * (e & 1) + i) + (e >> 1)] * inv;
+                        const size_t to = at + 64 * (c >> 1) + 16 * (c & 1) + 8 * (e & 1) + 32 * (e >> 1);
+                        if (A.type == 0) lfm_store<8>(static_cast<float *>(A.out) + to, v);
+                        else if (A.type == 1) lfm_store<8>(static_cast<__half *>(A.out) + to, v);
+                        else lfm_store<8>(static_cast<__nv_bfloat16 *>(A.out) + to, v);
+                    }
+                };
+                /* a part: [value / 4][row] of 16 bytes, then the rows' m and sum */
+                auto part_of = [&](uint32_t s) { return plan.part + ((size_t)jb.tile * plan.parts + s) * kRows * (D + 2); };
+                float *const mine = kSplit && jb.parts > 1 ? part_of(jb.part) : nullptr;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t u[32];
+                    float o[32];
+                    ld32(tO + 32 * c, u);
+                    wait_ld();
+                    tie32(u);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
+                    if (!kSplit || !mine) {
+                        write(c, o, l > 0.0f ? 1.0f / l : 0.0f);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            __stcg(reinterpret_cast<float4 *>(mine) + (size_t)(8 * c + k) * kRows + r,
+                                   make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+                    }
+                }
+                if (kSplit && mine) {
+                    /* the last warp to arrive with a part of these 32 rows joins them all, in their order */
+                    __stcg(reinterpret_cast<float2 *>(mine + kRows * D) + r, make_float2(m, l));
+                    __threadfence();
+                    __syncwarp();
+                    uint32_t *const arrived = plan.counts + jb.tile * 8 + warp;
+                    uint32_t before = 0;
+                    if (lane == 0) before = atomicAdd(arrived, 1u);
+                    if (__shfl_sync(LFM_FULL_MASK, before, 0) + 1 == jb.parts) {
+                        __threadfence();
+                        if (lane == 0) *arrived = 0;
+                        auto ml = [&](uint32_t s) {
+                            return __ldcg(reinterpret_cast<const float2 *>(part_of(s) + kRows * D) + r);
+                        };
+                        float top = LFM_NO_KEY, sum = 0.0f;
+#pragma unroll 4
+                        for (uint32_t s = 0; s < jb.parts; ++s) top = fmaxf(top, ml(s).x);
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            float o[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                            sum = 0.0f;
+#pragma unroll 2
+                            for (uint32_t s = 0; s < jb.parts; ++s) {
+                                const float2 x = ml(s);
+                                const float f = lfm_ex2(x.x - top);
+                                sum = __fmaf_rn(f, x.y, sum);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    const float4 y = __ldcg(reinterpret_cast<const float4 *>(part_of(s)) +
+                                                            (size_t)(8 * c + k) * kRows + r);
+                                    o[4 * k] = __fmaf_rn(f, y.x, o[4 * k]);
+                                    o[4 * k + 1] = __fmaf_rn(f, y.y, o[4 * k + 1]);
+                                    o[4 * k + 2] = __fmaf_rn(f, y.z, o[4 * k + 2]);
+                                    o[4 * k + 3] = __fmaf_rn(f, y.w, o[4 * k + 3]);
+                                }
+                            }
+                            write(c, o, sum > 0.0f ? 1.0f / sum : 0.0f);
+                        }
                     }
                 }
             }
+            base += n;
+            drop(it);
         }
-        base += n;
-        drop(it);
-      }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp < 12) {
@@ -483,46 +508,47 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
             const LfmNib nib;
             /* two threads a key: halves of its words */
             const uint32_t key = (warp & 1) * 32 + lane, half = (warp >> 1) & 1;
-            const uint32_t codes = key * (D / 2) + half * (D / 4), scales = kKeys * (D / 2) + key * (D / 16) + (D == 64 ? 0 : 4 * half);
-          for (uint32_t it = 0; take(it); ++it) {
-            const uint32_t n = bars.job[it & 1].n;
-            const int64_t len = bars.job[it & 1].len, blk0 = bars.job[it & 1].blk0 - base;
-            for (uint32_t u = 2 * base; u < 2 * (base + n); ++u) {
-                const uint32_t rs = u % C::kRaws, os = u % C::kOps;
-                bool w = wait(&bars.raw_full[rs], (u / C::kRaws) & 1, abort, A.err);
-                if (u >= (uint32_t)C::kOps) w = w && wait(&bars.op_empty[os], ((u / C::kOps) & 1) ^ 1, abort, A.err);
-                ok = __all_sync(LFM_FULL_MASK, w);
-                if (!ok) break;
-                const uint8_t *raw = sm + C::kOffRaw + rs * C::kRaw;
-                uint8_t *to = sm + C::kOffOp + os * C::kOp + key * 16 + half * (D / 16) * kChunk;
-                /* a slot that holds no token may hold anything: zero, for V */
-                const bool held = (blk0 + (u >> 1)) * kKeys + key < len;
-                const uint32_t d = held ? *reinterpret_cast<const uint32_t *>(raw + scales) : 0u;
+            const uint32_t codes = key * (D / 2) + half * (D / 4);
+            const uint32_t scales = kKeys * (D / 2) + key * (D / 16) + (D == 64 ? 0 : 4 * half);
+            for (uint32_t it = 0; take(it); ++it) {
+                const uint32_t n = bars.job[it & 1].n;
+                const int64_t len = bars.job[it & 1].len, blk0 = bars.job[it & 1].blk0 - base;
+                for (uint32_t u = 2 * base; u < 2 * (base + n); ++u) {
+                    const uint32_t rs = u % C::kRaws, os = u % C::kOps;
+                    bool w = wait(&bars.raw_full[rs], (u / C::kRaws) & 1, abort, A.err);
+                    if (u >= (uint32_t)C::kOps) w = w && wait(&bars.op_empty[os], ((u / C::kOps) & 1) ^ 1, abort, A.err);
+                    ok = __all_sync(LFM_FULL_MASK, w);
+                    if (!ok) break;
+                    const uint8_t *raw = sm + C::kOffRaw + rs * C::kRaw;
+                    uint8_t *to = sm + C::kOffOp + os * C::kOp + key * 16 + half * (D / 16) * kChunk;
+                    /* a slot that holds no token may hold anything: zero, for V */
+                    const bool held = (blk0 + (u >> 1)) * kKeys + key < len;
+                    const uint32_t d = held ? *reinterpret_cast<const uint32_t *>(raw + scales) : 0u;
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-                    const uint4 a = *reinterpret_cast<const uint4 *>(raw + codes + 16 * c);
-                    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+                    for (int c = 0; c < D / 64; ++c) {
+                        const uint4 a = *reinterpret_cast<const uint4 *>(raw + codes + 16 * c);
+                        const uint32_t x[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t y = x[k] >> 8;
-                        *reinterpret_cast<uint4 *>(to + (4 * c + k) * kChunk) =
-                            make_uint4(lfm_hmul2(lfm_hsub2(nib.lo(x[k]), LFM_NIB0_OFF), d),
-                                       lfm_hmul2(lfm_hsub2(nib.hi(x[k]), LFM_NIB1_OFF), d),
-                                       lfm_hmul2(lfm_hsub2(nib.lo(y), LFM_NIB0_OFF), d),
-                                       lfm_hmul2(lfm_hsub2(nib.hi(y), LFM_NIB1_OFF), d));
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t y = x[k] >> 8;
+                            *reinterpret_cast<uint4 *>(to + (4 * c + k) * kChunk) =
+                                make_uint4(lfm_hmul2(lfm_hsub2(nib.lo(x[k]), LFM_NIB0_OFF), d),
+                                           lfm_hmul2(lfm_hsub2(nib.hi(x[k]), LFM_NIB1_OFF), d),
+                                           lfm_hmul2(lfm_hsub2(nib.lo(y), LFM_NIB0_OFF), d),
+                                           lfm_hmul2(lfm_hsub2(nib.hi(y), LFM_NIB1_OFF), d));
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        lfm_mbar_arrive(&bars.op_full[os]);
+                        lfm_mbar_arrive(&bars.raw_empty[rs]);
                     }
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    lfm_mbar_arrive(&bars.op_full[os]);
-                    lfm_mbar_arrive(&bars.raw_empty[rs]);
-                }
+                if (!ok) break;
+                base += n;
+                drop(it);
             }
-            if (!ok) break;
-            base += n;
-            drop(it);
-          }
         } else if (warp == 12 || warp == 14) {
             /* A warp a tile: what one spends on barriers between its MMAs is the other's tensor time.  The whole warp
              * walks the loop and one thread issues: descriptors and TMEM addresses (base 0: all columns are ours) then
@@ -669,7 +695,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                         if (lane == 0) lfm_mbar_arrive_tx(&bars.raw_full[rs], all);
                         __syncwarp();
                         if (page)
-                            lfm_bulk_g2s_plain(sm + to + rs * C::kRaw, page + in + (k ? A.kv.half : 0), bytes, &bars.raw_full[rs]);
+                            lfm_bulk_g2s_plain(sm + to + rs * C::kRaw, page + in + (k ? A.kv.half : 0), bytes,
+                                               &bars.raw_full[rs]);
                     }
                     if (!ok) break;
                 }
@@ -718,10 +745,14 @@ TilePlan lfm_attn_tile_plan(const AttnArgs &a, uint32_t head_dim, uint64_t above
     p.tiles = (uint32_t)((rows + (kRows - 1) * (most < a.bt.n_seqs ? most : a.bt.n_seqs)) / kRows);
     const uint64_t jobs = (uint64_t)p.tiles * a.kv.hkv;
     uint64_t keys = max_kv_len;
-    if (a.window && keys > a.window + kRows / a.group) keys = a.window + kRows / a.group;
+    if (a.window) keys = keys < (uint64_t)a.window + kRows / a.group ? keys : (uint64_t)a.window + kRows / a.group;
     const uint64_t blocks = keys / kKeys + 1;
-    for (uint64_t n = 1; n == 1 || (n <= blocks / kPartBlocks && n <= LFM_ATTN_TILES && jobs * n <= LFM_ATTN_TILES && jobs * 8 <= LFM_ATTN_COUNTS - 2); ++n) {
-        const uint64_t cost = (jobs * n + sms - 1) / sms * ((blocks + n - 1) / n + kJobBlocks + (n > 1)) + (n > 1 ? n * head_dim / 128 : 0);
+    /* parts: as many as make the busiest SM's walk shortest.  One of more than a part pays for what it writes, and the
+     * last one joins n (a part of 128 values is as many bytes as a block takes time) */
+    const uint64_t bound = blocks / kPartBlocks < LFM_ATTN_TILES ? blocks / kPartBlocks : LFM_ATTN_TILES;
+    for (uint64_t n = 1; n == 1 || (n <= bound && jobs * n <= LFM_ATTN_TILES && jobs * 8 <= LFM_ATTN_COUNTS - 2); ++n) {
+        const uint64_t rounds = (jobs * n + sms - 1) / sms, walk = (blocks + n - 1) / n + kJobBlocks + (n > 1);
+        const uint64_t cost = rounds * walk + (n > 1 ? n * head_dim / 128 : 0);
         if (n == 1 || cost < p.cost) {
             p.cost = cost;
             p.parts = (uint32_t)n;

@@ -10,6 +10,14 @@
  * 32 lanes of one token by itself -- its sequence, position, angles and page
  * found once, a step's loads under way while the one before computes, no
  * block-wide barrier: one step for a few tokens (latency), more for prompts.
+ * d and the codes are formed in fp32 from the rounded fp16 d, so that reading
+ * back and attending see the d that the code was chosen for.
+ *
+ * Floor: the rows of q, k and v read, q and the codes written.  5307 tokens of
+ * 32 / 8 heads of 128 values, 116 MB: 30.0 us, 3.9 TB/s, read back 8.6 us.  By
+ * instruction issue (59%) and the loads' latency together: HBM stands at 30%.  A
+ * block of threads for each token, its steps between barriers: 74 us for both,
+ * 42 so.  64 tokens, 64-value heads: 3.1 us, a launch and a chain of loads.
  */
 #include "attn_device.cuh"
 
@@ -257,9 +265,11 @@ __global__ void __launch_bounds__(256) k_kv_read(ReadArgs A, uint32_t per_token)
     }
 }
 
-/* Steps a warp takes: one while that leaves the GPU unfilled (measured at 64 tokens: 4.4 us against 4.9 with eight), eight
- * beyond (4630 tokens of 48 heads of 128 values: see the kernel's comment). */
-constexpr uint64_t kManySteps = 148 * 64;
+/* Steps a warp takes: one where that leaves the GPU unfilled, eight beyond.  Tokens of 32 / 8 heads of 64 values, append
+ * and read back, one step / eight: 64 tokens 5.0 / 8.8 us, 512: 7.5 / 9.1, 1024: 10.6 / 9.9, 4096: 28.8 / 19.0; of 128
+ * values: 256: 7.4 / 11.0, 768: 12.5 / 12.0, 4096: 53.9 / 32.0.  The sides meet at 900 and 700 tokens, 11 and 17
+ * thousand steps; 96 warps an SM, 14 thousand, lie between. */
+constexpr uint64_t kManySteps = 148 * 96;
 
 template <class T, int D>
 cudaError_t launch_append(const AppendArgs &a, cudaStream_t s, bool pdl) {

@@ -8,7 +8,13 @@
  * 4 l .. 4 l + 3 and 128 + 4 l .. of its block in registers from the load to
  * the codes, so every tensor is touched once and the row's only exchange is
  * the sum of squares (warp shuffles, then the warps' sums in order: the same
- * result on every run).  Bound by HBM.
+ * result on every run).
+ *
+ * Floor: x, delta and the outputs once, 13.1 bytes a value with an fp32 delta:
+ * bound by HBM.  4096 rows of 2048 values, 110 MB, call after call (some of it
+ * then comes from L2): 16.1 us, 6.8 TB/s; the rows read back as bf16 values 5.7
+ * more.  1021 rows of 5120 with bf16 rows as well, 69 MB: 10.2 us.  64 rows of
+ * 2048: 2.0 us, a launch and a chain of loads, sum and maximum.
  */
 #include "attn_device.cuh"
 
