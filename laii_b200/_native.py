@@ -14,6 +14,7 @@ from . import build as _build
 
 _lock = threading.Lock()
 _gpu = None
+_attn_py = None
 _synth = None
 
 c_u32, c_i32, c_u64, c_f32, c_vp, c_int, c_sz = (ctypes.c_uint32, ctypes.c_int32, ctypes.c_uint64, ctypes.c_float,
@@ -144,6 +145,26 @@ def load_gpu(build_if_missing: bool = True):
                 raise RuntimeError(f"CUDA library missing: {_build.GPU_SO} (run python -m laii_b200.build)")
             _gpu = _bind(ctypes.CDLL(_build.GPU_SO), GPU_API + ATTN_API)
         return _gpu
+
+
+def load_attn_py(build_if_missing: bool = True):
+    """The Python module lfm_attn_py (csrc/lfm_attn_py.cpp) over the CUDA library."""
+    global _attn_py
+    load_gpu(build_if_missing)
+    with _lock:
+        if _attn_py is None:
+            if build_if_missing:
+                _build.build_attn_py()
+            if not os.path.exists(_build.ATTN_PY_SO):
+                raise RuntimeError(f"Python module missing: {_build.ATTN_PY_SO} (run python -m laii_b200.build)")
+            import importlib.util
+
+            import torch  # noqa: F401  the libraries that the module needs
+            spec = importlib.util.spec_from_file_location("lfm_attn_py", _build.ATTN_PY_SO)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _attn_py = module
+        return _attn_py
 
 
 def bind_synth(lib):

@@ -1,6 +1,7 @@
 """Build the native libraries in-tree (laii_b200/_lib/).
 
   liblfm_gpu_moe.so  CUDA kernels + C-ABI (include/lfm_gpu_moe.h, lfm_gpu_attn.h), sm_100a only
+  lfm_attn_py.so     Python module: the calls of lfm_gpu_attn.h on torch tensors (C++)
   liblfm_synth.so    host seeded-input generator (C)
 
 nvcc flags: -gencode arch=compute_100a,code=sm_100a; -fmad=false and
@@ -24,6 +25,7 @@ LIB = os.path.join(PKG, "_lib")
 BUILD = os.path.join(PKG, "_build")
 
 GPU_SO = os.path.join(LIB, "liblfm_gpu_moe.so")
+ATTN_PY_SO = os.path.join(LIB, "lfm_attn_py.so")
 SYNTH_SO = os.path.join(LIB, "liblfm_synth.so")
 
 CU_SOURCES = ["lfm_gpu_moe.cu", "k_route.cu", "k_gemv.cu", "k_layer.cu", "k_gemm.cu", "k_umma.cu", "k_expert.cu", "k_ep.cu", "k_q6k.cu", "k_synth.cu", "lfm_gguf.cpp",
@@ -128,9 +130,37 @@ def _build_gpu_locked(srcs, verbose_ptxas: bool) -> None:
     os.replace(tmp, GPU_SO)
 
 
+def build_attn_py(force: bool = False) -> str:
+    """After build_gpu, whose library the module is linked to."""
+    src = os.path.join(CSRC, "lfm_attn_py.cpp")
+    deps = [src, os.path.join(ROOT, "include", "lfm_gpu_moe.h"), os.path.join(ROOT, "include", "lfm_gpu_attn.h"),
+            os.path.abspath(__file__)]
+    if not (force or _stale(ATTN_PY_SO, deps)):
+        return ATTN_PY_SO
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    with _BuildLock():
+        if force or _stale(ATTN_PY_SO, deps):
+            tmp = f"{ATTN_PY_SO}.{os.getpid()}.tmp"
+            cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+            inc = [f"-I{d}" for d in (os.path.join(ROOT, "include"), cuda, sysconfig.get_paths()["include"])]
+            inc += [x for d in include_paths() for x in ("-isystem", d)]
+            libs = [x for d in library_paths() for x in (f"-L{d}", f"-Wl,-rpath,{d}")]
+            # the compiler that nvcc uses, not $CXX: exceptions pass between the module and torch, in one C++ runtime
+            _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc, src, "-o", tmp, f"-L{LIB}",
+                  "-l:" + os.path.basename(GPU_SO), "-Wl,-rpath,$ORIGIN", *libs, "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu",
+                  "-lc10_cuda", "-lc10"])
+            os.replace(tmp, ATTN_PY_SO)
+    return ATTN_PY_SO
+
+
 def build_all(force: bool = False) -> None:
     build_synth(force)
     build_gpu(force)
+    build_attn_py(force)
 
 
 if __name__ == "__main__":

@@ -56,3 +56,19 @@ def test_null_handle_is_an_error_not_a_crash():
     assert lib.lfm_gpu_kv_read(None, None, None, 0, None, None, None) == -1
     assert lib.lfm_gpu_attn_forward(None, None, None, 1, 1.0, 1, 0, 0.0, 0, None, 0, None, 0, None) == -1
     assert lib.lfm_gpu_attn_reserve(None) == -1
+
+
+def test_python_module_refuses_without_a_launch():
+    """Arguments that are not tensors of the device raise before the library is called."""
+    import torch
+    m = _native.load_attn_py()
+    x = torch.zeros(2, 256)
+    for x_ in (x, None, 3):
+        with pytest.raises(ValueError):
+            m.add_rmsnorm(0, 0, x_, None, None, 1e-5, None, -1, True)
+    with pytest.raises(ValueError):
+        m.read_q8(0, 0, x, 0)
+    with pytest.raises(TypeError):
+        m.add_rmsnorm(0, 0, None)
+    with pytest.raises(TypeError):
+        m.read_q8(0, "0", x, 0)

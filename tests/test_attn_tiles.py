@@ -140,3 +140,15 @@ def test_more_sequences_than_threads(lib, n, q):  # noqa: F811
     rows = [(0 if b % 11 == 5 else q, 0 if b % 7 == 3 else 1 + (b * 37) % 90) for b in range(n)]
     run(lib, rows, 16, 2, 4, 64, seed=3)
     run(lib, rows + [(330, 900)] + rows[:40], 16, 8, 4, 64, seed=4)
+
+
+def test_a_closed_handle_is_refused():
+    from laii_b200.attn import GpuAttn
+    from laii_b200.moe import GpuMoE
+    moe = GpuMoE(0)
+    attn = GpuAttn(moe)
+    moe.close()
+    with pytest.raises(ValueError):
+        attn.add_rmsnorm(torch.zeros(2, 256, device="cuda"), None, None)
+    with pytest.raises(ValueError):
+        attn.reserve()
