@@ -78,7 +78,9 @@ cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_k
                             cudaStream_t s, bool pdl);
 /* The tensor-core kernel for the sequences of more than `above` rows (token, head of a group). */
 struct TilePlan {
-    uint64_t above, blocks, cost;  /* key blocks of the longest walk by max_kv_len; blocks that the busiest SM walks */
+    uint64_t above;
+    uint64_t blocks;               /* of keys, in the longest walk by max_kv_len (what a row sees at most) */
+    uint64_t cost;                 /* blocks that the busiest SM walks */
     uint32_t tiles, parts;         /* tiles of rows of one kv head, at most; most parts of one */
     uint32_t *counts;              /* zero before and after */
     float *part;

@@ -689,15 +689,26 @@ cudaError_t launch_rows(const AttnArgs &a, const RowsPlan &p, dim3 grid, cudaStr
 static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, uint64_t few, uint32_t max_kv_len,
                                         int sm_count, void *scratch, cudaStream_t s, bool pdl) {
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, G = a.group, keys = head_dim == 64 ? 64 : 32;
-    /* columns of a tile: what an average sequence fills, as far as registers go.  16 sequences of 8192 keys, 64-value
-     * heads, 8 / 16 / 32 columns: 4 rows 31, 38, 56 us; 12 rows 49, 42, 61; 24 rows 67, 67, 64; 64 rows 154, 117, 106.
-     * 128-value heads, 8 / 16: 4 rows 52, 66; 12 rows 88, 75; 64 rows 300, 226 */
-    const uint64_t per = (T + B - 1) / B * G;
-    const uint32_t nt = per <= 8 ? 1 : per <= 16 || head_dim == 128 ? 2 : 4;
+    /* columns of a tile: what an average sequence fills, as far as registers go, but narrow ones where the work is little:
+     * more warps run at once, and each block has less to load, join and write.  By the keys that a warp would walk with
+     * tiles of 8, 16 or 12 warps an SM: up to 256, tiles of 8; up to 1024, of 16 if tiles of 32 are so few that their
+     * keys are split (otherwise each costs its loads and its join).  64-value heads, 8 kv heads, tiles of 8 / 16 / 32
+     * columns, rows of a sequence:
+     *   1 sequence of 2048 keys     32 rows 11.0, 12.6, 16.9 us
+     *   1 sequence of 16384 keys    16 rows 17.8, 23.6, 23.8;  32: 20.8, 22.0, 30.9;  64: 28.8, 25.3, 31.4
+     *   16 sequences of 1000 keys   32 rows 16.9, 23.4, 20.6;  64: 34.8, 33.6, 21.6
+     *   16 sequences of 8192 keys   4 rows 29, 37, 55;  12: 49, 39, 59;  24: 67, 65, 60;  64: 155, 116, 101
+     * 128-value heads, 8 / 16:
+     *   1 sequence of 16384 keys    16 rows 23.5, 31.1;  32: 30.2, 31.8;  64: 49.8, 40.6
+     *   16 sequences of 8192 keys   4 rows 50, 66;  12: 84, 68;  64: 292, 216 */
+    const uint64_t per = (T + B - 1) / B * G, span = ((uint64_t)max_kv_len + keys - 1) / keys;
+    const uint64_t walk = B * ((per + 7) / 8) * a.kv.hkv * span * keys / ((uint64_t)sm_count * (head_dim == 64 ? 16 : 12));
+    const bool split = B * ((per + 31) / 32) * a.kv.hkv < (uint64_t)sm_count / 2;
+    const uint32_t nt = per <= 8 || walk <= 256 ? 1 : per <= 16 || head_dim == 128 || (walk <= 1024 && split) ? 2 : 4;
     /* blocks: as many as run at once (registers: more, with spills, ran slower), fewer where there are not enough
      * blocks of keys by the hint */
     uint64_t grid = (uint64_t)sm_count * (head_dim * nt < 128 ? 4 : head_dim * nt == 128 ? 3 : 2);
-    const uint64_t units = (B + T * G / (8 * nt)) * a.kv.hkv, work = units * ((max_kv_len + keys - 1) / keys + 1);
+    const uint64_t units = (B + T * G / (8 * nt)) * a.kv.hkv, work = units * (span + 1);
     const uint64_t most = work / kWarps > units ? work / kWarps : units;
     if (grid > most) grid = most;
     if (grid > LFM_ATTN_BLOCKS) grid = LFM_ATTN_BLOCKS;
@@ -723,6 +734,8 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
  * In a batch for both, sequences of up to 64 rows (128-value heads: 32) are this kernel's. */
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
                             cudaStream_t s, bool pdl) {
+    /* what a row, or the rows of a tile, can see */
+    if (a.window && max_kv_len > (uint64_t)a.window + 256) max_kv_len = a.window + 256;
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group, few = B == 1 ? 0 : head_dim == 64 ? 64 : 32;
     const TilePlan p = lfm_attn_tile_plan(a, head_dim, few, max_kv_len, sm_count);
     const uint64_t here = (rows + 16 * B) / 32 * a.kv.hkv * (p.blocks + 12);   /* 12: a unit's cost beside its blocks */

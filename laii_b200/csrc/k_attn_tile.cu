@@ -744,9 +744,7 @@ TilePlan lfm_attn_tile_plan(const AttnArgs &a, uint32_t head_dim, uint64_t above
     p.above = above;
     p.tiles = (uint32_t)((rows + (kRows - 1) * (most < a.bt.n_seqs ? most : a.bt.n_seqs)) / kRows);
     const uint64_t jobs = (uint64_t)p.tiles * a.kv.hkv;
-    uint64_t keys = max_kv_len;
-    if (a.window) keys = keys < (uint64_t)a.window + kRows / a.group ? keys : (uint64_t)a.window + kRows / a.group;
-    const uint64_t blocks = keys / kKeys + 1;
+    const uint64_t blocks = max_kv_len / kKeys + 1;
     /* parts: as many as make the busiest SM's walk shortest.  One of more than a part pays for what it writes, and the
      * last one joins n (a part of 128 values is as many bytes as a block takes time) */
     const uint64_t bound = blocks / kPartBlocks < LFM_ATTN_TILES ? blocks / kPartBlocks : LFM_ATTN_TILES;
