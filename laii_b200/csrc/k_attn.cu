@@ -700,6 +700,7 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
      *   16 sequences of 8192 keys   4 rows 29, 37, 55;  12: 49, 39, 59;  24: 67, 65, 60;  64: 155, 116, 101
      * 128-value heads, 8 / 16:
      *   1 sequence of 16384 keys    16 rows 23.5, 31.1;  32: 30.2, 31.8;  64: 49.8, 40.6
+     *   16 sequences of 1000 keys   8 rows 15.4, 18.1;  16: 24.6, 19.8 (the wrong side)
      *   16 sequences of 8192 keys   4 rows 50, 66;  12: 84, 68;  64: 292, 216 */
     const uint64_t per = (T + B - 1) / B * G, span = ((uint64_t)max_kv_len + keys - 1) / keys;
     const uint64_t walk = B * ((per + 7) / 8) * a.kv.hkv * span * keys / ((uint64_t)sm_count * (head_dim == 64 ? 16 : 12));
@@ -730,7 +731,7 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
  *                              128-value heads  32 rows: 122, 136;  64: 225, 216;  128: 428, 213
  *   8 sequences of 4096 keys, 64-value heads    64 rows: 37, 43;  128: 55, 78;  256: 107, 72
  *   1 sequence of 16384 keys, 64-value heads    128 rows: 39, 48;  256: 59, 45;  512: 104, 50
- *   1 sequence of 2048 keys, 64-value heads     256 rows: 21, 23;  512: 26, 25;  1024: 33, 26
+ *   1 sequence of 2048 keys, 64-value heads     256 rows: 19, 23;  512: 26, 25;  1024: 33, 26
  * In a batch for both, sequences of up to 64 rows (128-value heads: 32) are this kernel's. */
 cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_kv_len, int sm_count, void *scratch,
                             cudaStream_t s, bool pdl) {
