@@ -442,10 +442,15 @@ lfm_gpu_status_t read_device_error(lfm_gpu_moe_t *h) {
     uint32_t e = 0;
     LFM_CUDA(h, cudaMemcpy(&e, h->dev_err, sizeof e, cudaMemcpyDeviceToHost));
     if (e == 0) return LFM_GPU_OK;
+    /* An abandoned forward can leave completion counters part-way: clear them.  The callers have waited for their own
+     * stream at most, and a memset returns before it has run, on a stream that others do not wait for: so nothing of the
+     * device's work is under way while they are cleared, and the clearing is over before the next call */
+    LFM_CUDA(h, cudaDeviceSynchronize());
+    LFM_CUDA(h, cudaMemcpy(&e, h->dev_err, sizeof e, cudaMemcpyDeviceToHost));
     LFM_CUDA(h, cudaMemset(h->dev_err, 0, sizeof(uint32_t)));
-    /* an abandoned forward can leave completion counters part-way: clear them */
     if (h->attn_scratch) LFM_CUDA(h, cudaMemset(h->attn_scratch, 0, LFM_ATTN_COUNTS * sizeof(uint32_t)));
     if (h->ws.base) LFM_CUDA(h, cudaMemset(h->ws.base, 0, h->ws.counters_bytes));
+    LFM_CUDA(h, cudaDeviceSynchronize());
     if (e & LFM_DEVERR_TIMEOUT) return fail(h, LFM_GPU_ERR_TIMEOUT, "device wait timed out (0x%x)", e);
     return fail(h, LFM_GPU_ERR_DEVICE_CHECK, "device bounds check tripped (0x%x)", e);
 }
