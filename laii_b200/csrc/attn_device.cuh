@@ -104,6 +104,16 @@ __device__ __forceinline__ bool lfm_sane(const BatchDev &bt, int64_t q0, int64_t
     return q0 >= 0 && n >= 0 && q0 + n <= (int64_t)bt.n_tokens;
 }
 
+/* Reports sequences whose rows are out of order or beyond the call's: the thread looks at sequences at, at + step, ... */
+__device__ __forceinline__ void lfm_check_batch(const BatchDev &bt, uint32_t at, uint32_t step, uint32_t *err) {
+    bool sane = true;
+    for (uint32_t b = at; b < bt.n_seqs; b += step) {
+        const int64_t q = bt.q_start[b];
+        sane &= lfm_sane(bt, q, (int64_t)bt.q_start[b + 1] - q);
+    }
+    if (!sane) atomicOr(err, LFM_DEVERR_PAGE);
+}
+
 /* One warp: the want-th tile of `per` rows (token, head of a group of G) over the sequences of more than `above` rows:
  * (sequence, tile) into out, or a sequence of -1.  Returns the tiles looked through: all where there is no such. */
 __device__ __forceinline__ uint64_t lfm_find_tile(const BatchDev &bt, uint32_t G, uint32_t per, uint64_t above, uint64_t want,
@@ -132,6 +142,7 @@ __device__ __forceinline__ uint64_t lfm_find_tile(const BatchDev &bt, uint32_t G
         if (__any_sync(LFM_FULL_MASK, here)) return before;
     }
     if (lane == 0) out[0] = -1;
+    __syncwarp(); /* before another call's writer */
     return before;
 }
 

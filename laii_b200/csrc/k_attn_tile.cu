@@ -707,6 +707,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                 ticket[0] = 0;
                 ticket[1] = 0;
             }
+        } else if (blockIdx.x == 0) { /* warp 15 has no other part; the loader passes such sequences over */
+            lfm_check_batch(A.bt, lane, 32, A.err);
         }
     }
     if (!ok) *abort = 1;

@@ -70,3 +70,32 @@ def test_an_error_read_by_a_forward_while_split_calls_run(lib):  # noqa: F811
         side.synchronize()
     lib.moe.sync()
     assert all(torch.equal(o, want) for o in outs)
+
+
+# ---- offsets that describe no batch --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("hkv,G,rows", [(1, 4, (1, 50)), (8, 4, (400, 400)), (8, 4, (200, 2100))], ids=["rows", "tiles", "split"])
+@pytest.mark.parametrize("start", [[0, 2 ** 31 - 1], [-1, 1], [1, 0], [0, 401]])
+def test_attend_reports_the_offsets_of_one_sequence(lib, hkv, G, rows, start):  # noqa: F811
+    c = Case([rows], 64, hkv, 64, seed=4)
+    c.batch._keep[0].copy_(torch.tensor(start, dtype=torch.int32))
+    buf = torch.full((c.T + 2, hkv * G, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    lib.attend(c.cache, c.batch, torch.randn(c.T, hkv * G, 64, generator=gen(1)).bfloat16().cuda(), out=buf[1:-1])
+    device_check(lib)
+    assert (buf == 5).all()
+
+
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("bad", [1, -1])
+def test_attend_reports_one_bad_sequence_of_several(lib, n, bad):  # noqa: F811
+    """Wherever it stands; the sequences before it are right."""
+    rows = [(90, 400)] * n
+    at = n - 1 if bad < 0 else 1
+    c = Case(rows, 64, 8, 64, seed=4)
+    c.batch._keep[0][at + 1:] = c.T + 1
+    q = torch.randn(c.T, 32, 64, generator=gen(1)).bfloat16()
+    out = lib.attend(c.cache, c.batch, q.cuda())
+    device_check(lib)
+    c.rows = rows[:at]
+    check_attend(c, q, out, "bf16", 0.125)
