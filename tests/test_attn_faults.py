@@ -99,3 +99,48 @@ def test_attend_reports_one_bad_sequence_of_several(lib, n, bad):  # noqa: F811
     device_check(lib)
     c.rows = rows[:at]
     check_attend(c, q, out, "bf16", 0.125)
+
+
+@pytest.mark.parametrize("n,start", [(4, [0, 10]), (4, [-2, 4]), (4, [3, 1]), (300, [0, 2 ** 31 - 1]), (600, [0, 601])])
+def test_append_and_read_report_offsets_and_leave_the_rows(lib, n, start):  # noqa: F811
+    """No token of an older place is written over, and nothing is read in its name."""
+    c = Case([(n, n + 40)], 16, 8, 64, fill=False)
+    c.batch._keep[0].copy_(torch.tensor(start, dtype=torch.int32))
+    k = torch.randn(n, 8, 64, generator=gen(1)).bfloat16().cuda()
+    q = torch.randn(n, 16, 64, generator=gen(2)).bfloat16().cuda()
+    before, out = c.cache.pages.clone(), torch.full_like(q, 3.0)
+    lib.append(c.cache, c.batch, q, k, k, q_out=out)
+    device_check(lib)
+    assert torch.equal(c.cache.pages, before) and (out == 3).all()
+    lib.read(c.cache, c.batch, n, torch.float32)
+    device_check(lib)
+
+
+@pytest.mark.parametrize("n", [3, 70, 600])
+def test_append_and_read_report_one_bad_sequence_of_several(lib, n):  # noqa: F811
+    c = Case([(1, 9)] * n, 16, 2, 64, fill=False)
+    c.batch._keep[0][n] = n + 1  # the last sequence: two rows of a call that has one for it
+    k = torch.randn(n, 2, 64, generator=gen(1)).bfloat16().cuda()
+    lib.append(c.cache, c.batch, None, k, k)
+    device_check(lib)
+    got, _ = lib.read(c.cache, c.batch, n, torch.float32)
+    device_check(lib)
+    from attn_ref import quantise
+    want = torch.stack([quantise(x)[0] for x in k[:n - 1].cpu().double()])
+    # without a norm or a rotation the codes are exact but for the fp32 quotient at a boundary
+    assert ((got[:n - 1].cpu().double() - want).abs() <= 1e-6).float().mean() > 0.999
+    last = int(c.table[n - 1, 0])
+    assert (c.cache.pages[last] == 255).all()
+
+
+def test_padding_rows_are_no_error(lib):  # noqa: F811
+    """Rows outside every sequence are padding: left alone, and nothing is reported."""
+    c = Case([(2, 20), (0, 5), (3, 30)], 16, 2, 64)
+    k = torch.randn(c.T + 6, 2, 64, generator=gen(1)).bfloat16().cuda()
+    q = torch.randn(c.T + 6, 4, 64, generator=gen(2)).bfloat16().cuda()
+    out = torch.full_like(q, 3.0)
+    lib.append(c.cache, c.batch, q, k, k, q_out=out)
+    lib.read(c.cache, c.batch, c.T + 6, torch.float32)
+    lib.attend(c.cache, c.batch, q)
+    lib.moe.sync()
+    assert torch.equal(out[:c.T], q[:c.T]) and (out[c.T:] == 3).all()
