@@ -22,9 +22,11 @@
  *    16-byte boundary (checked);
  *  - `type` is the GGML type of the 16- or 32-bit tensors: 0 (F32), 1 (F16)
  *    or 30 (BF16);
- *  - a bad page id, a position outside the page table or the rotation table is
- *    found on the device: the access is skipped and the next lfm_gpu_moe_sync
- *    returns LFM_GPU_ERR_DEVICE_CHECK.
+ *  - a bad page id, a position outside the page table or the rotation table,
+ *    offsets out of order or range and, for attention, a length that the page
+ *    table has no room for are found on the device: the access is skipped, the
+ *    sequence of bad offsets or length is passed over (its rows are left
+ *    alone), and the next lfm_gpu_moe_sync returns LFM_GPU_ERR_DEVICE_CHECK.
  */
 #ifndef LFM_GPU_ATTN_H
 #define LFM_GPU_ATTN_H

@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                     jb.q0 = A.bt.q_start[b];
                     jb.n_q = (int64_t)A.bt.q_start[b + 1] - jb.q0;
                     jb.len = A.bt.kv_len[b];
-                    if (jb.len < 0) {
+                    if (!lfm_sane_len(A.kv, A.bt, jb.len)) {
                         if (lane == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
                         continue;
                     }

@@ -144,3 +144,44 @@ def test_padding_rows_are_no_error(lib):  # noqa: F811
     lib.attend(c.cache, c.batch, q)
     lib.moe.sync()
     assert torch.equal(out[:c.T], q[:c.T]) and (out[c.T:] == 3).all()
+
+
+# ---- lengths that the page table has no room for -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [[(1, 100)], [(300, 400)], [(60, 2000), (300, 400)], [(1, 70), (1, 100)]],
+                         ids=["one", "tiles", "both", "batch"])
+@pytest.mark.parametrize("over", [1, 500, 2 ** 31 - 1])
+def test_attend_passes_over_a_length_beyond_the_table(lib, rows, over):  # noqa: F811
+    """The last sequence's length is past the table's span: reported, its rows left alone, the others right."""
+    c = Case(rows, 16, 8, 64, seed=4)
+    span = c.table.shape[1] * 16
+    c.batch._keep[1][-1] = min(span + over, 2 ** 31 - 1)
+    q = torch.randn(c.T, 32, 64, generator=gen(6)).bfloat16()
+    out = torch.full((c.T, 32, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    lib.attend(c.cache, c.batch, q.cuda(), out=out)
+    device_check(lib)
+    assert (out[c.starts[-2]:] == 5).all()
+    c.rows = rows[:-1]
+    check_attend(c, q, out, "bf16", 0.125)
+
+
+@pytest.mark.parametrize("rows", [[(1, 100), (0, 40)], [(300, 400), (0, 40)]])
+@pytest.mark.parametrize("n", [10 ** 6, -3])
+def test_the_length_of_a_sequence_without_rows_does_not_matter(lib, rows, n):  # noqa: F811
+    c = Case(rows, 16, 8, 64, seed=4)
+    c.batch._keep[1][1] = n
+    q = torch.randn(c.T, 32, 64, generator=gen(6)).bfloat16()
+    out = lib.attend(c.cache, c.batch, q.cuda())
+    lib.moe.sync()
+    c.rows = rows[:1]
+    check_attend(c, q, out, "bf16", 0.125)
+
+
+def test_a_length_that_fills_the_table_is_right(lib):  # noqa: F811
+    c = Case([(2, 128), (130, 256)], 16, 8, 64, seed=4)
+    assert c.table.shape[1] * 16 == 256
+    q = torch.randn(c.T, 32, 64, generator=gen(6)).bfloat16()
+    out = lib.attend(c.cache, c.batch, q.cuda())
+    lib.moe.sync()
+    check_attend(c, q, out, "bf16", 0.125)
