@@ -114,10 +114,8 @@ __device__ __forceinline__ void lfm_check_batch(const BatchDev &bt, uint32_t at,
     if (!sane) atomicOr(err, LFM_DEVERR_PAGE);
 }
 
-/* Tokens that the page table has room for; attention's walk over a sequence is bounded by that. */
-__device__ __forceinline__ bool lfm_sane_len(const KvDev &kv, const BatchDev &bt, int64_t len) {
-    return len >= 0 && len <= (int64_t)bt.table_stride << kv.page_shift;
-}
+/* A length that the page table has room for; attention's walk over a sequence is bounded by that. */
+__device__ __forceinline__ bool lfm_sane_len(const BatchDev &bt, int64_t len) { return (uint32_t)len <= bt.span; }
 
 /* One warp: the want-th tile of `per` rows (token, head of a group of G) over the sequences of more than `above` rows:
  * (sequence, tile) into out, or a sequence of -1.  Returns the tiles looked through: all where there is no such. */

@@ -23,7 +23,7 @@ struct KvDev {
 };
 
 struct BatchDev {
-    uint32_t n_seqs, n_tokens, table_stride;
+    uint32_t n_seqs, n_tokens, table_stride, span; /* span: tokens that a sequence's entries hold, below 2^31 */
     const int32_t *q_start, *kv_len, *page_table;
 };
 

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
         q.q0 = A.bt.q_start[b];
         q.n_q = (int64_t)A.bt.q_start[b + 1] - q.q0;
         q.len = A.bt.kv_len[b];
-        q.sane = lfm_sane(A.bt, q.q0, q.n_q) && (q.n_q == 0 || lfm_sane_len(A.kv, A.bt, q.len));
+        q.sane = lfm_sane(A.bt, q.q0, q.n_q) && (q.n_q == 0 || lfm_sane_len(A.bt, q.len));
         const uint64_t rows = q.sane ? (uint64_t)q.n_q * G : 0;
         if (rows == 0 || rows > P.most) return q;
         int64_t lo, hi, unused;

@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                     jb.q0 = A.bt.q_start[b];
                     jb.n_q = (int64_t)A.bt.q_start[b + 1] - jb.q0;
                     jb.len = A.bt.kv_len[b];
-                    if (!lfm_sane_len(A.kv, A.bt, jb.len)) {
+                    if (!lfm_sane_len(A.bt, jb.len)) {
                         if (lane == 0) atomicOr(A.err, LFM_DEVERR_PAGE);
                         continue;
                     }
@@ -707,10 +707,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                 ticket[0] = 0;
                 ticket[1] = 0;
             }
-        } else if (blockIdx.x == 0) { /* warp 15 has no other part; the loader passes such sequences over */
-            lfm_check_batch(A.bt, lane, 32, A.err);
         }
     }
+    /* the loader passes bad sequences over.  Warp 15, which has no other part, reports them, from behind the roles: beside
+     * them the check made prompts 2% slower */
+    if (blockIdx.x == 0 && warp == 15) lfm_check_batch(A.bt, lane, 32, A.err);
     if (!ok) *abort = 1;
     fence_before();
     __syncthreads();

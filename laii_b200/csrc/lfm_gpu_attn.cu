@@ -73,7 +73,7 @@ lfm_gpu_status_t view_cache(lfm_gpu_moe_t *h, const lfm_gpu_kv_t *kv, const lfm_
     k->head_bytes = page / kv->n_kv_heads;
     k->codes = kv->page_tokens * (kv->head_dim / 2);
     k->half = (uint32_t)(k->head_bytes / 2);
-    *b = BatchDev{bt->n_seqs, bt->n_tokens, bt->table_stride, bt->q_start, bt->kv_len, bt->page_table};
+    *b = BatchDev{bt->n_seqs, bt->n_tokens, bt->table_stride, bt->table_stride * kv->page_tokens, bt->q_start, bt->kv_len, bt->page_table};
     return LFM_GPU_OK;
 }
 
@@ -225,7 +225,7 @@ LFM_API lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv
     void *scratch = nullptr;
     st = lfm_host_scratch(h, s, &scratch);
     if (st != LFM_GPU_OK) return st;
-    const uint32_t span = batch->table_stride * kv->page_tokens;
+    const uint32_t span = a.bt.span;
     const uint32_t hint = batch->max_kv_len && batch->max_kv_len < span ? batch->max_kv_len : span;
     st = launch(h, hv, AK_ATTN, "attn_forward", s,
                 [&] { return lfm_launch_attn(a, kv->head_dim, hint, hv.sm_count, scratch, s, hv.pdl); });
