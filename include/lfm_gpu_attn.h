@@ -68,7 +68,8 @@ size_t lfm_gpu_kv_page_bytes(uint32_t page_tokens, uint32_t n_kv_heads, uint32_t
  * tokens last, so its row i is at position kv_len[b] - rows + i; token j lies
  * in page page_table[b * table_stride + j / page_tokens].  Rows outside every
  * sequence (padding) are left alone.  Entries past a sequence's last page are
- * not read. */
+ * not read, nor by attention with a window those of pages that end before the
+ * first token that a row of the sequence sees: such pages may be given back. */
 typedef struct {
     uint32_t n_seqs;
     uint32_t n_tokens;      /* rows of q (an upper bound of q_start[n_seqs])          */

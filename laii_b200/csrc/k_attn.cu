@@ -110,6 +110,13 @@ struct Seq {
     bool sane;
 };
 
+/* Words of a stage that no copy fills.  Not inlined: in the kernel it changes the key loop's registers (64 sequences:
+ * 62.0 -> 62.7 us; a test of each key pair beside the one for `held` 62.9). */
+__device__ __noinline__ void zero_shared(uint32_t to, uint32_t bytes) {
+    for (uint32_t i = 0; i < bytes; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + i), "r"(0u) : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); /* before a later copy into the stage */
+}
+
 /* A warp's copies of its blocks of keys first, first + kWarps, ... of a unit. */
 template <int D>
 struct Ring {
@@ -134,19 +141,24 @@ struct Ring {
         bytes = min(P, kK) * per;
         to = smem + (part & 2 ? Cfg<D>::kBytes / 2 : 0) + ((part & 1) ? kK * (D / 2) : 0) + j * bytes;
     }
-    __device__ __forceinline__ void unit(uint32_t b, uint32_t kvh, int64_t first_, uint32_t n_, int64_t end_) {
+    __device__ __forceinline__ void unit(uint32_t b, uint32_t kvh, int64_t first_, uint32_t n_, int64_t lo, int64_t end_) {
         row = bt.page_table + (size_t)b * bt.table_stride;
         from = kv.pages + (size_t)kvh * kv.head_bytes + (lane & 2 ? kv.half : 0) + (lane & 1 ? kv.codes : 0);
         first = first_;
         n = n_;
         end = end_;
-        next = lookup(0);
+        /* only a unit's first block begins below lo.  A page of it that ends there may be gone: it is not copied, and its
+         * slots' values get scales of zero (their scores are masked) */
+        bool gone = false;
+        next = lookup(0, [&](int64_t key) { return gone = key + min(kv.page_tokens, kK) <= lo; });
+        if (gone && (lane & 3) == 3) zero_shared(to, bytes);
     }
-    /* This lane's page in block i2 + lane / 16. */
-    __device__ __forceinline__ uint32_t lookup(uint32_t i2) {
+    /* This lane's page in block i2 + lane / 16, but for keys that no row sees. */
+    template <class Unseen>
+    __device__ __forceinline__ uint32_t lookup(uint32_t i2, Unseen &&unseen) {
         const uint32_t i = i2 + lane / 16, at = ((lane >> 2) & 3) * kv.page_tokens;
         const int64_t key = (first + (int64_t)i * kWarps) * kK + at;
-        if (i >= n || key >= end || (at && at >= kK)) return ~0u; /* nothing to copy */
+        if (i >= n || key >= end || (at && at >= kK) || unseen(key)) return ~0u; /* nothing to copy */
         const int64_t place = key >> kv.page_shift;
         uint32_t page = ~0u;
         if (place < (int64_t)bt.table_stride) page = (uint32_t)row[place];
@@ -157,7 +169,7 @@ struct Ring {
     __device__ __forceinline__ void issue(uint32_t i, uint32_t st) {
         if ((i & 1) == 0) {
             id = next;
-            next = lookup(i + 2);
+            next = lookup(i + 2, [](int64_t) { return false; });
         }
         const bool on = (lane >> 4) == (i & 1) && id < kv.n_pages;
         const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, on ? bytes : 0u);
@@ -328,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
         const int64_t mine = to - from - warp;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads(); /* s_lo, s_hi; the ring is free of an earlier unit's join, for the copies too */
-        rg.unit(b, kvh, from + warp, mine > 0 ? (uint32_t)((mine + kWarps - 1) / kWarps) : 0u, len);
+        rg.unit(b, kvh, from + warp, mine > 0 ? (uint32_t)((mine + kWarps - 1) / kWarps) : 0u, lo0, len);
 #pragma unroll
         for (uint32_t i = 0; i < kStages; ++i)
             if (i < rg.n) rg.issue(i, i);

@@ -72,9 +72,10 @@ constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32
 template <int D>
 constexpr uint32_t kIdescPV = (1u << 4) | ((uint32_t)(kM >> 4) << 24) | ((uint32_t)(D >> 3) << 17) | (1u << 16);
 
-/* 256 rows of a kv head: rows row0 .. of sequence b, key blocks blk0 .. + n; part `part` of `parts` of tile `tile`. */
+/* 256 rows of a kv head: rows row0 .. of sequence b, key blocks blk0 .. + n, of them the keys from lo on; part `part` of
+ * `parts` of tile `tile`. */
 struct Job {
-    int64_t q0, n_q, len, blk0;
+    int64_t q0, n_q, len, blk0, lo;
     uint32_t row0, rows, kvh, n, tile, part, parts;
     int b; /* -1: no more */
 };
@@ -512,7 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
             const uint32_t scales = kKeys * (D / 2) + key * (D / 16) + (D == 64 ? 0 : 4 * half);
             for (uint32_t it = 0; take(it); ++it) {
                 const uint32_t n = bars.job[it & 1].n;
-                const int64_t len = bars.job[it & 1].len, blk0 = bars.job[it & 1].blk0 - base;
+                /* slots that hold a token that a row sees, counted from the first block: from `lo` on, `held` of them */
+                const int64_t key0 = bars.job[it & 1].blk0 * kKeys;
+                const uint32_t lo = (uint32_t)max((int64_t)0, bars.job[it & 1].lo - key0), held = (uint32_t)(bars.job[it & 1].len - key0) - lo;
                 for (uint32_t u = 2 * base; u < 2 * (base + n); ++u) {
                     const uint32_t rs = u % C::kRaws, os = u % C::kOps;
                     bool w = wait(&bars.raw_full[rs], (u / C::kRaws) & 1, abort, A.err);
@@ -521,9 +524,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                     if (!ok) break;
                     const uint8_t *raw = sm + C::kOffRaw + rs * C::kRaw;
                     uint8_t *to = sm + C::kOffOp + os * C::kOp + key * 16 + half * (D / 16) * kChunk;
-                    /* a slot that holds no token may hold anything: zero, for V */
-                    const bool held = (blk0 + (u >> 1)) * kKeys + key < len;
-                    const uint32_t d = held ? *reinterpret_cast<const uint32_t *>(raw + scales) : 0u;
+                    /* a slot that holds no token, or none that a row sees, may hold anything: zero, for V */
+                    const uint32_t at = ((u >> 1) - base) * kKeys + key - lo;
+                    const uint32_t d = at < held ? *reinterpret_cast<const uint32_t *>(raw + scales) : 0u;
 #pragma unroll
                     for (int c = 0; c < D / 64; ++c) {
                         const uint4 a = *reinterpret_cast<const uint4 *>(raw + codes + 16 * c);
@@ -657,6 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                     int64_t lo0, hi0, lo1, hi1;
                     lfm_visible(A, jb.n_q, jb.len, jb.row0, lo0, hi0);
                     lfm_visible(A, jb.n_q, jb.len, jb.row0 + jb.rows - 1, lo1, hi1);
+                    jb.lo = lo0;
                     jb.blk0 = lo0 / kKeys;
                     jb.n = hi1 > lo0 ? (uint32_t)((hi1 + kKeys - 1) / kKeys - jb.blk0) : 0;
                     if (kSplit) {
@@ -682,8 +686,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                 const uint32_t n = jb.n;
                 for (uint32_t j = 0; j < n; ++j) {
                     const int64_t key = (jb.blk0 + j) * kKeys + (int64_t)piece * sub;
-                    const uint8_t *page = nullptr;
-                    if (piece * sub < kKeys && key < jb.len) page = lfm_page(A.kv, A.bt, jb.b, key, jb.kvh, A.err);
+                    const uint8_t *page = nullptr; /* one below the window may be gone */
+                    if (piece * sub < kKeys && key < jb.len && key + sub > jb.lo) page = lfm_page(A.kv, A.bt, jb.b, key, jb.kvh, A.err);
                     const uint32_t all = __reduce_add_sync(LFM_FULL_MASK, page ? bytes : 0u);
                     const uint32_t in = ((uint32_t)key & (P - 1)) * per + (part ? A.kv.codes : 0);
 #pragma unroll

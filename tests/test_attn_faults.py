@@ -185,3 +185,26 @@ def test_a_length_that_fills_the_table_is_right(lib):  # noqa: F811
     out = lib.attend(c.cache, c.batch, q.cuda())
     lib.moe.sync()
     check_attend(c, q, out, "bf16", 0.125)
+
+
+# ---- pages behind a sliding window ----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,hkv", [([(1, 333), (3, 261), (1, 129), (1, 17)], 2), ([(1, 5000), (1, 700)], 1), ([(8, 2000), (8, 900)], 2),
+                                      ([(300, 900), (70, 611)], 8), ([(200, 2100)], 8)], ids=["decode", "long", "verify", "tiles", "split"])
+@pytest.mark.parametrize("D,P", [(64, 16), (64, 32), (128, 16), (128, 64)])
+@pytest.mark.parametrize("window", [1, 33, 1100])
+@pytest.mark.parametrize("what", ["gone", "anything"])
+def test_pages_behind_the_window_may_be_given_back(lib, rows, hkv, D, P, window, what):  # noqa: F811
+    """Entries of pages that end before the first token that a row sees: -1, or a page of NaN scales."""
+    c = Case(rows, P, hkv, D, seed=D + P, spare=1)
+    t = c.table.clone()
+    used = set(int(i) for i in t[t >= 0])
+    spare = next(i for i in range(c.pages.shape[0]) if i not in used)   # all bytes 0xFF
+    for b, (q, n) in enumerate(rows):
+        t[b, : max(0, n - q + 1 - window) // P] = -1 if what == "gone" else spare
+    c.batch._keep[2].copy_(t)
+    q = torch.randn(c.T, 4 * hkv, D, generator=gen(9)).bfloat16()
+    out = lib.attend(c.cache, c.batch, q.cuda(), window=window)
+    lib.moe.sync()
+    check_attend(c, q, out, "bf16", D ** -0.5, window=window)
