@@ -124,7 +124,8 @@ lfm_gpu_status_t lfm_gpu_kv_read(lfm_gpu_moe_t *h, const lfm_gpu_kv_t *kv, const
                                  uint32_t type, void *k_out, void *v_out, void *stream);
 
 /* out = softmax(z) V per row and head, z = scale * q . k, or with softcap > 0
- * softcap * tanh(scale * q . k / softcap).  Head h reads kv head h / (n_heads /
+ * softcap * tanh(scale * q . k / softcap), to fp32 accuracy of the score for
+ * any cap.  Head h reads kv head h / (n_heads /
  * n_kv_heads).  causal != 0: the row at position p sees the keys j <= p, with
  * window > 0 only those with j > p - window; causal == 0: every key (window
  * must be 0).  A row that sees no key is 0.  q and out

@@ -191,6 +191,20 @@ __device__ __forceinline__ float lfm_rcp(float x) {
     return y;
 }
 
+/* tanh(x) for capped scores, e2 = 2 x / ln 2, as 1 - 2 / (1 + e^2x): within 2^-22 of the truth, so a score is off by
+ * softcap 2^-22.  That is well under what rounding the probabilities to fp16 costs up to LFM_PLAIN_CAP; beyond, where the
+ * error would grow with the cap, small arguments take the series x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 (relative error
+ * below 62 / 2835 4^-8 = 2^-21 up to 1/4), and the score is off by 2^-20 of itself whatever the cap. */
+#define LFM_PLAIN_CAP 128.0f
+__device__ __forceinline__ float lfm_tanh(float e2) { return __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(e2)), 1.0f); }
+__device__ __forceinline__ float lfm_tanh_any(float e2) {
+    const float x = e2 * 0.34657359f, y = x * x;
+    const float p = __fmaf_rn(y, __fmaf_rn(y, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f);
+    return fabsf(x) < 0.25f ? __fmaf_rn(x * y, p, x) : lfm_tanh(e2);
+}
+/* 2 / ln 2 times what takes a product to tanh's argument: finite, so that a product of zero stays one. */
+__device__ __forceinline__ float lfm_cap_scale(float scale, float softcap) { return fminf(fabsf(scale) * 2.88539008f / softcap, 3e38f); }
+
 #define LFM_NO_KEY -1e30f /* the running reference of a row that has seen no key */
 
 /* Eight values of q within fp16's finite range (NaN stays), negated for a negative scale. */

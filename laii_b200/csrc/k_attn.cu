@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
     uint32_t phases = 0; /* parity of each stage's next wait */
     lfm_pdl_wait();
     lfm_pdl_launch_dependents();
-    const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
+    const float sc = fmaxf((kCap ? A.softcap : fabsf(A.scale)) * 1.44269504f, 1e-30f); /* not 0: times -inf */
 
     /* ---- this block's share: all (tile, head) units' key blocks in a row, cut into equal parts ---- */
     auto sequence = [&](uint32_t b) {
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
         const uint32_t atk = rk * (D / 2) + 8 * t, atks = kKs + rk * (D / 16);
         const uint32_t atve = kV + ve * (D / 2) + 4 * g, atvo = kV + vo * (D / 2) + 4 * g;
         const uint32_t atvs = kV + kKs + (ve & ~1u) * (D / 16);
-        const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
+        const float capz = kCap ? lfm_cap_scale(A.scale, A.softcap) : 0.0f;
         constexpr int kPair = NT == 1 ? 2 : 1; /* steps of 16 keys whose scores are looked at together */
         const LfmNib nib;
         bool ok = true;
@@ -458,14 +458,17 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
                         }
                     }
                 }
-                if (kCap) { /* tanh(x) = 1 - 2 / (1 + e^2x) */
+                if (kCap) {
+                    auto cap = [&](auto &&tanh_of) {
 #pragma unroll
-                    for (int q = 0; q < kPair; ++q)
+                        for (int q = 0; q < kPair; ++q)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                z4[q][n][j] = __fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(z4[q][n][j] * capz)), 1.0f);
+                                for (int j = 0; j < 4; ++j) z4[q][n][j] = tanh_of(z4[q][n][j] * capz);
+                    };
+                    if (A.softcap <= LFM_PLAIN_CAP) cap([](float x) { return lfm_tanh(x); });
+                    else cap([](float x) { return lfm_tanh_any(x); });
                 }
                 if (!kWhole) {
 #pragma unroll

@@ -304,8 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                 if (lane == 0) lfm_mbar_arrive(&bars.q_full[h]);
             }
             const uint32_t tO = tmem + C::kColO + h * D + ((warp & 3) << 21);
-            const float sc = kCap ? A.softcap * 1.44269504f : fmaxf(fabsf(A.scale) * 1.44269504f, 1e-30f);
-            const float capz = kCap ? fabsf(A.scale) * 2.88539008f / A.softcap : 0.0f;
+            const float sc = fmaxf((kCap ? A.softcap : fabsf(A.scale)) * 1.44269504f, 1e-30f); /* not 0: times -inf */
+            const float capz = kCap ? lfm_cap_scale(A.scale, A.softcap) : 0.0f;
             /* what the row sees, in keys from the first block; the blocks [inside0, inside1) every row of the tile sees
              * whole */
             int lo = 0, hi = 0, inside0 = 0, inside1 = 0;
@@ -345,10 +345,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                 wait_ld();
                 tie32(x);
                 tie32(x + 32);
-                if (kCap) { /* tanh(x) = 1 - 2 / (1 + e^2x) */
+                if (kCap) {
+                    if (A.softcap <= LFM_PLAIN_CAP) {
 #pragma unroll
-                    for (int i = 0; i < kKeys; ++i)
-                        x[i] = __float_as_uint(__fmaf_rn(-2.0f, lfm_rcp(1.0f + lfm_ex2(__uint_as_float(x[i]) * capz)), 1.0f));
+                        for (int i = 0; i < kKeys; ++i) x[i] = __float_as_uint(lfm_tanh(__uint_as_float(x[i]) * capz));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i) x[i] = __float_as_uint(lfm_tanh_any(__uint_as_float(x[i]) * capz));
+                    }
                 }
                 if (masked) {
 #pragma unroll

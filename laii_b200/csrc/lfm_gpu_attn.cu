@@ -213,7 +213,8 @@ LFM_API lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv
     a.n_heads = n_heads;
     a.group = n_heads / kv->n_kv_heads;
     a.scale = scale;
-    a.softcap = softcap;
+    /* a product is at most 65504^2 head_dim: above this cap the argument of tanh is below 2^-12, and tanh itself in fp32 */
+    a.softcap = softcap > fabs((double)scale) * 4096.0 * 65504.0 * 65504.0 * kv->head_dim ? 0.0f : softcap;
     a.causal = causal != 0;
     a.window = window;
     a.type = type;

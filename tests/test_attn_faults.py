@@ -208,3 +208,43 @@ def test_pages_behind_the_window_may_be_given_back(lib, rows, hkv, D, P, window,
     out = lib.attend(c.cache, c.batch, q.cuda(), window=window)
     lib.moe.sync()
     check_attend(c, q, out, "bf16", D ** -0.5, window=window)
+
+
+# ---- caps far above and below the scores ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,hkv", [([(1, 300), (3, 150)], 2), ([(8, 700)], 2), ([(130, 400)], 8), ([(200, 2100)], 8)],
+                         ids=["decode", "verify", "tiles", "split"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [1e-39, 0.5, 100.0, 127.9, 300.0, 1e4, 1e6, 1e9, 1e30])
+def test_any_cap(lib, rows, hkv, D, cap):  # noqa: F811
+    """Under the bound of scores without a cap: a large one adds an error relative to a score, not to itself."""
+    import attn_ref as ref
+    c = Case(rows, 32, hkv, D, seed=D)
+    q = torch.randn(c.T, 4 * hkv, D, generator=gen(9)).bfloat16()
+    out = lib.attend(c.cache, c.batch, q.cuda(), scale=0.3, softcap=cap)
+    lib.moe.sync()
+    assert torch.isfinite(out).all()
+    for b, (n, _) in enumerate(rows):
+        a = slice(c.starts[b], c.starts[b] + n)
+        K, V = c.kv(b)
+        want, _ = ref.attend(q[a], K, V, 0.3, softcap=cap)
+        _, tol = ref.attend(q[a], K, V, 0.3)
+        # the bound's weights are those of uncapped scores: the capped ones are flatter, so by the largest value instead.
+        # A score is off by 2^-11 |q| |k| scale (q and the keys rounded; tanh's slope is at most one) and, up to a cap of
+        # 128, by 2^-22 of that; a probability by twice that, 2^-11 of itself and 2^-25 where fp16 goes subnormal
+        dz = torch.einsum("nhgd,jhd->nhgj", q[a].double().view(n, hkv, 4, D).abs(), K.abs()).amax(-1) * 0.3 * (2.0 ** -11 + 2.0 ** -19) + 128 * 2.0 ** -22
+        t = ((2.0 ** -10 + 2 * dz + 2.0 ** -17 + len(K) * 2.0 ** -25) * V.abs().amax()).reshape(n, -1, 1)
+        if cap >= 1e6:  # |z| / cap so small that the weights are those of the bound
+            t = torch.minimum(t, tol * 1.01 + 1e-9)
+        err = (out[a].cpu().double() - want).abs()
+        assert (err <= t + 2.0 ** -8 * want.abs()).all(), float((err / (t + 2.0 ** -8 * want.abs())).max())
+
+
+@pytest.mark.parametrize("rows,hkv", [([(1, 300)], 2), ([(130, 400)], 8)], ids=["rows", "tiles"])
+def test_a_cap_beyond_all_scores_is_none(lib, rows, hkv):  # noqa: F811
+    c = Case(rows, 32, hkv, 64, seed=1)
+    q = torch.randn(c.T, 4 * hkv, 64, generator=gen(9)).bfloat16().cuda()
+    plain = lib.attend(c.cache, c.batch, q)
+    assert torch.equal(lib.attend(c.cache, c.batch, q, softcap=1e37), plain)
+    lib.moe.sync()
