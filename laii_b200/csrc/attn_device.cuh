@@ -205,7 +205,13 @@ __device__ __forceinline__ float lfm_tanh_any(float e2) {
 /* 2 / ln 2 times what takes a product to tanh's argument: finite, so that a product of zero stays one. */
 __device__ __forceinline__ float lfm_cap_scale(float scale, float softcap) { return fminf(fabsf(scale) * 2.88539008f / softcap, 3e38f); }
 
-#define LFM_NO_KEY -1e30f /* the running reference of a row that has seen no key */
+/* The running reference m of a row, in powers of two: p = 2^(z - m) is held in fp16.  It is set LFM_REF_LOW below a score,
+ * so that keys far below a row's largest one keep their part of the product as they do of the sum (fp16 ends 2^-31 below
+ * the largest; set at the score itself it was 2^-24, and 131072 keys 17.4 nats below one lost 0.4% of the output), and
+ * moves when a score passes it by LFM_REF_MOVE: p <= 2^15, within fp16. */
+#define LFM_REF_LOW 7.0f
+#define LFM_REF_MOVE 15.0f
+#define LFM_NO_KEY -1e30f /* of a row that has seen no key */
 
 /* Eight values of q within fp16's finite range (NaN stays), negated for a negative scale. */
 __device__ __forceinline__ void lfm_fit_q(bool neg, float (&v)[8]) {

@@ -15,8 +15,9 @@
  *     multiplied into its 32-value partial sum in fp32: K enters exact;
  *   - V: offset subtracted and scale multiplied in fp16 pairs (the product is
  *     rounded to fp16: 2^-12 relative, under the output's rounding);
- *   - P: e^(z - m) in fp16 as the B fragment, transposed by movmatrix.  m only
- *     moves when a score passes it by 2^8, so p <= 256, and the sum is fp32.
+ *   - P: e^(z - m) in fp16 as the B fragment, transposed by movmatrix.  m lies
+ *     2^7 below a score and only moves when one passes it by 2^15, so p <= 2^15,
+ *     and the sum is fp32.
  * A warp takes 4608-byte blocks of keys and values (64 keys of 64 values, 32 of
  * 128) through its own ring of bulk copies.  All (tile of columns, kv head)
  * units' blocks of keys lie in a row that is cut into equal parts, one for each
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
                         float x = fmaxf(z4[0][n][e], z4[0][n][2 + e]);
                         if (kPair == 2) x = fmaxf(x, fmaxf(z4[kPair - 1][n][e], z4[kPair - 1][n][2 + e]));
                         top[n][e] = x;
-                        grow |= __fmaf_rn(x, sc, -m[n][e]) > 8.0f;
+                        grow |= __fmaf_rn(x, sc, -m[n][e]) > LFM_REF_MOVE;
                     }
                 if (__any_sync(LFM_FULL_MASK, grow)) {
 #pragma unroll
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, D * NT < 128 ? 4 : D * NT == 128 ? 3
                             float x = top[n][e];
 #pragma unroll
                             for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(LFM_FULL_MASK, x, k));
-                            const float nm = fmaxf(m[n][e], x * sc), f = lfm_ex2(m[n][e] - nm);
+                            const float nm = fmaxf(m[n][e], __fmaf_rn(x, sc, -LFM_REF_LOW)), f = lfm_ex2(m[n][e] - nm);
                             m[n][e] = nm;
                             l[n][e] *= f;
 #pragma unroll

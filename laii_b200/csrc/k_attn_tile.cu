@@ -18,8 +18,9 @@
  *             128), taken in turn by (key block, tile), so the scores of a
  *             tile's next block are there when its softmax ends
  *   2 x 4 warps  softmax, a thread a row: no exchange between threads.  The
- *             running reference m only moves when a score passes it by 2^8
- *             (p <= 256 in fp16); then the thread scales its row of O in TMEM
+ *             running reference m lies 2^7 below a score and only moves when one
+ *             passes it by 2^15 (p <= 2^15 in fp16); then the thread scales its
+ *             row of O in TMEM
  * The blocks are persistent, one an SM, and take the tiles from a counter, the
  * longest first: loader and dequantisation run ahead into the next tile while
  * the softmax warps finish one.  Few tiles of long walks have their keys split
@@ -31,7 +32,7 @@
  *
  * Keys and values enter as fp16 products d * (code - 8), rounded once (2^-12
  * relative, under the output's rounding and q's own); scores, m, the sum and O
- * are fp32, p is fp16 <= 256.
+ * are fp32, p is fp16 <= 2^15.
  *
  * 32 / 8 heads.  4096 tokens from the beginning, 64-value heads: 130 us, 530
  * TFLOP/s; 42 us of tensor work, 60 of exponentials (one a score, 16 a clock and
@@ -367,8 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_tile(AttnArgs A, TilePlan 
                     max3(mx[3], x[i + 6], x[i + 7]);
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if (__any_sync(LFM_FULL_MASK, __fmaf_rn(top, sc, -m) > 8.0f)) {
-                    const float nm = fmaxf(m, top * sc), f = lfm_ex2(m - nm);
+                if (__any_sync(LFM_FULL_MASK, __fmaf_rn(top, sc, -m) > LFM_REF_MOVE)) {
+                    const float nm = fmaxf(m, __fmaf_rn(top, sc, -LFM_REF_LOW)), f = lfm_ex2(m - nm);
                     const uint64_t f2 = pk2(__float_as_uint(f), __float_as_uint(f));
                     m = nm;
                     l2 = mul2(l2, f2);

@@ -248,3 +248,51 @@ def test_a_cap_beyond_all_scores_is_none(lib, rows, hkv):  # noqa: F811
     plain = lib.attend(c.cache, c.batch, q)
     assert torch.equal(lib.attend(c.cache, c.batch, q, softcap=1e37), plain)
     lib.moe.sync()
+
+
+# ---- one key far above all others -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,hkv,G", [((1, 6000), 1, 4), ((8, 6000), 1, 4), ((64, 20000), 8, 4), ((1200, 6000), 8, 4)],
+                         ids=["decode", "verify", "split", "tiles"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nats", [10.0, 17.5, 20.0])
+def test_keys_far_below_one_keep_their_part(lib, rows, hkv, G, D, nats):  # noqa: F811
+    """The first key scores `nats` and has a value of 0, all others score 0 and have 1: row i sees n = i of them and is
+    n e^-nats / (1 + n e^-nats).  q, keys and values are exact.  A probability is off by 2^-11 of itself (fp16) and 2^-20
+    (its exponent, 25 at most, in fp32), or by 2^-32 of the largest where fp16 goes subnormal, 2^-25 of a reference 2^7
+    below the largest score."""
+    n, length = rows
+    c = Case([(length, length)], 64, hkv, D, fill=False)
+    k = torch.zeros(length, hkv, D)
+    v = torch.ones(length, hkv, D)
+    k[0], v[0] = 1.0, 0.0
+    lib.append(c.cache, c.batch, None, k.cuda(), v.cuda())
+    c.batch._keep[0][1] = n
+    q = torch.ones(n, hkv * G, D, device="cuda")
+    scale = nats / D
+    out = lib.attend(c.cache, c.batch, q, scale=scale).cpu().double()
+    lib.moe.sync()
+    seen = torch.arange(length - n, length, dtype=torch.float64)[:, None, None]
+    part = seen * torch.exp(torch.tensor(-nats, dtype=torch.float64))
+    want = part / (1 + part)
+    assert ((out - want).abs() <= want * (2.0 ** -10 + 2.0 ** -19) + seen * 2.0 ** -32).all(), float(((out - want).abs() / want).max())
+
+
+@pytest.mark.parametrize("rows,hkv", [([(1, 900)], 2), ([(8, 900)], 2), ([(300, 900)], 8), ([(200, 2100)], 8)],
+                         ids=["decode", "verify", "tiles", "split"])
+@pytest.mark.parametrize("scale", [0.02, 0.6, -3.0, 40.0])
+def test_scores_that_climb(lib, rows, hkv, scale):  # noqa: F811
+    """Keys in the order of their scores, so that the reference moves late and often: no probability leaves fp16."""
+    c = Case(rows, 16, hkv, 64, seed=5)
+    import attn_ref as ref
+    kc, ks, _, _ = ref.split_page(c.pages, 16, hkv, 64)
+    p = c.pages.view(c.pages.shape[0], hkv, -1)
+    for i, page in enumerate(c.table[0]):   # scales that grow from key to key
+        at = (torch.arange(16) + 16 * i + 1.0) / rows[0][1]
+        p[int(page), :, 512:576] = (0.1 * at)[:, None].expand(16, 2).half().contiguous().view(torch.uint8).reshape(-1)
+    c.cache.pages.copy_(c.pages)
+    q = torch.randn(c.T, 4 * hkv, 64, generator=gen(3)).bfloat16()
+    out = lib.attend(c.cache, c.batch, q.cuda(), scale=scale)
+    lib.moe.sync()
+    check_attend(c, q, out, "bf16", scale)
