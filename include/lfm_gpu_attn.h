@@ -124,14 +124,15 @@ lfm_gpu_status_t lfm_gpu_kv_read(lfm_gpu_moe_t *h, const lfm_gpu_kv_t *kv, const
                                  uint32_t type, void *k_out, void *v_out, void *stream);
 
 /* out = softmax(z) V per row and head, z = scale * q . k, or with softcap > 0
- * softcap * tanh(scale * q . k / softcap), to fp32 accuracy of the score for
- * any cap.  Head h reads kv head h / (n_heads /
- * n_kv_heads).  causal != 0: the row at position p sees the keys j <= p, with
- * window > 0 only those with j > p - window; causal == 0: every key (window
- * must be 0).  A row that sees no key is 0.  q and out
- * [n_tokens][n_heads][head_dim] of `type`, strides in elements.  q is rounded
- * to fp16 (saturated) for the tensor cores, products and sums are fp32, the
- * probabilities fp16. */
+ * softcap * tanh(scale * q . k / softcap), within 2^-20 of the score or 2^-15
+ * for any cap.  Head h reads kv head h / (n_heads / n_kv_heads).  causal != 0:
+ * the row at position p sees the keys j <= p, with window > 0 only those with
+ * j > p - window; causal == 0: every key (window must be 0).  A row that sees
+ * no key is 0, one whose q holds a NaN is NaN.  q and out
+ * [n_tokens][n_heads][head_dim] of `type`, strides in elements.  For the tensor
+ * cores q is rounded to fp16 whatever its type (beyond its range +-65504, below
+ * 2^-14 to multiples of 2^-24), the cache's values and the probabilities too;
+ * products and sums are fp32. */
 lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv_t *kv, const lfm_gpu_kv_batch_t *batch,
                                       uint32_t n_heads, float scale, int causal, uint32_t window, float softcap,
                                       uint32_t type, const void *q, size_t q_stride, void *out, size_t out_stride,
@@ -139,9 +140,11 @@ lfm_gpu_status_t lfm_gpu_attn_forward(lfm_gpu_moe_t *h, const lfm_gpu_kv_t *kv, 
 
 /* Allocate the scratch in which lfm_gpu_attn_forward joins the parts of long
  * sequences (79 MB per handle, whatever is asked later).  The first forward does it otherwise,
- * which a stream capture does not allow.  Calls on several streams are ordered
- * among each other where they share the scratch; replays of captured calls are
- * not: replay one graph at a time per handle. */
+ * which a stream capture does not allow.  Calls on several streams (per-thread
+ * default streams of several threads among them) are ordered among each other
+ * where they share the scratch.  Captured calls are not: keep those of one
+ * capture on one stream, or order them, and replay one graph at a time per
+ * handle, with no call beside it. */
 lfm_gpu_status_t lfm_gpu_attn_reserve(lfm_gpu_moe_t *h);
 
 #ifdef __cplusplus

@@ -123,7 +123,7 @@ struct lfm_gpu_moe {
     EpP2P ep;
     void *attn_scratch = nullptr;      /* parts of split sequences (k_attn.cu)           */
     cudaEvent_t attn_done = nullptr;   /* behind the last work on it                     */
-    cudaStream_t attn_stream = nullptr;
+    unsigned long long attn_stream = 0; /* that work's stream by its id: a handle's value may come to name another stream */
     bool attn_used = false;
 };
 
@@ -492,7 +492,11 @@ lfm_gpu_status_t lfm_host_scratch(lfm_gpu_moe_t *h, cudaStream_t s, void **out) 
         if (e != cudaSuccess) { cudaFree(p); return cuda_fail(h, e, "attention scratch memset"); }
         h->attn_scratch = p;
     }
-    if (h->attn_used && s != h->attn_stream && !capturing(s)) LFM_CUDA(h, cudaStreamWaitEvent(s, h->attn_done, 0));
+    if (h->attn_used && !capturing(s)) {
+        unsigned long long id = 0;
+        LFM_CUDA(h, cudaStreamGetId(s, &id));
+        if (id != h->attn_stream) LFM_CUDA(h, cudaStreamWaitEvent(s, h->attn_done, 0));
+    }
     *out = h->attn_scratch;
     return LFM_GPU_OK;
 }
@@ -500,7 +504,7 @@ lfm_gpu_status_t lfm_host_scratch(lfm_gpu_moe_t *h, cudaStream_t s, void **out) 
 lfm_gpu_status_t lfm_host_scratch_used(lfm_gpu_moe_t *h, cudaStream_t s) {
     if (capturing(s)) return LFM_GPU_OK; /* replays are ordered by their caller */
     LFM_CUDA(h, cudaEventRecord(h->attn_done, s));
-    h->attn_stream = s;
+    LFM_CUDA(h, cudaStreamGetId(s, &h->attn_stream));
     h->attn_used = true;
     return LFM_GPU_OK;
 }

@@ -296,3 +296,64 @@ def test_scores_that_climb(lib, rows, hkv, scale):  # noqa: F811
     out = lib.attend(c.cache, c.batch, q.cuda(), scale=scale)
     lib.moe.sync()
     check_attend(c, q, out, "bf16", scale)
+
+
+# ---- one handle, streams that share a name --------------------------------------------------------------------------
+
+
+def test_per_thread_default_streams_take_turns(lib):  # noqa: F811
+    """Two threads' default streams have one handle value (cudaStreamPerThread): a call of the second waits for the work
+    that the first's has on the scratch."""
+    import ctypes
+    import threading
+    c = Case([(1, 20000)], 64, 1, 64, seed=6)
+    q = torch.randn(1, 4, 64, generator=gen(8)).bfloat16().cuda()
+    want = lib.attend(c.cache, c.batch, q)
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    done = [torch.cuda.Event() for _ in range(2)]
+    c.batch.rows(1)
+    torch.cuda.synchronize()
+
+    def work(i, spin):
+        s = torch.cuda.ExternalStream(2)  # cudaStreamPerThread
+        with torch.cuda.stream(s):
+            if spin:
+                torch.cuda._sleep(200_000_000)  # some 0.1 s of clocks
+            st = lib._lib.lfm_gpu_attn_forward(lib.moe._h, ctypes.byref(c.cache._c), ctypes.byref(c.batch._c), 4, 0.125, 1, 0, 0.0,
+                                               30, q.data_ptr(), 256, outs[i].data_ptr(), 256, ctypes.c_void_p(2))
+            done[i].record()
+        status.append(st)
+
+    status = []
+    for i, spin in enumerate((True, False)):
+        t = threading.Thread(target=work, args=(i, spin))
+        t.start()
+        t.join()
+    done[1].synchronize()
+    assert done[0].query()  # the first thread's work is over too
+    torch.cuda.synchronize()
+    lib.moe.sync()
+    assert status == [0, 0] and all(torch.equal(o, want) for o in outs)
+
+
+def test_a_stream_made_after_another_was_destroyed_waits(lib):  # noqa: F811
+    """Whatever value the new stream's handle has."""
+    import ctypes
+    cudart = torch.cuda.cudart()
+    c = Case([(1, 20000)], 64, 1, 64, seed=6)
+    q = torch.randn(1, 4, 64, generator=gen(8)).bfloat16().cuda()
+    want = lib.attend(c.cache, c.batch, q)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        box = ctypes.c_size_t()
+        err = cudart.cudaStreamCreate(ctypes.addressof(box))
+        assert int(err) == 0
+        s = torch.cuda.ExternalStream(box.value)
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(2_000_000)
+            outs.append(lib.attend(c.cache, c.batch, q))
+        assert int(cudart.cudaStreamDestroy(box.value)) == 0   # with its work under way
+    torch.cuda.synchronize()
+    lib.moe.sync()
+    assert all(torch.equal(o, want) for o in outs)
