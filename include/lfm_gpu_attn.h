@@ -98,9 +98,11 @@ typedef struct {
  * * weight;  xb = n as xb_type, q8 = n as block_q8_K [T][D / 256] (292 bytes
  * each, 4-byte aligned).  x and x_out fp32 [T][D] (may be the same memory),
  * delta of delta_type, weight fp32 [D] (NULL: ones); x_out, xb and q8 may each
- * be NULL.  D a multiple of 256, at most 8192.  The batched, stand-alone
- * counterpart of lfm2_rmsnorm_quantize_q8_K (tools/lfm2_decode_1x4.c:93-196)
- * with the residual's addition in front; its sums run in another order. */
+ * be NULL.  D a multiple of 256, at most 8192.  A block of q8 with a NaN or an
+ * infinity in it has that scale and codes of 0: its values read as NaN.  The
+ * batched, stand-alone counterpart of lfm2_rmsnorm_quantize_q8_K
+ * (tools/lfm2_decode_1x4.c:93-196) with the residual's addition in front; its
+ * sums run in another order. */
 lfm_gpu_status_t lfm_gpu_add_rmsnorm(lfm_gpu_moe_t *h, const float *x, const void *delta, uint32_t delta_type,
                                      uint32_t T, uint32_t D, const float *weight, float eps, float *x_out, void *xb,
                                      uint32_t xb_type, void *q8, void *stream);

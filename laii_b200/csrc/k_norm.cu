@@ -91,10 +91,12 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const float *x, const void
         else store_row(static_cast<__nv_bfloat16 *>(xb) + at, v);
     }
     if (!q8) return;
-    float m = 0.0f;
+    /* magnitudes as integers, where NaN is above infinity above the rest: a block that holds one gets the scale NaN, so
+     * that its values read as such (codes alone cannot say it) */
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
-    m = lfm_warp_max(m);
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    const float m = __uint_as_float(__reduce_max_sync(LFM_FULL_MASK, top));
     const float sc = m != 0.0f ? 127.0f / m : 0.0f;
     int a[4], b[4];
 #pragma unroll

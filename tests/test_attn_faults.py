@@ -357,3 +357,61 @@ def test_a_stream_made_after_another_was_destroyed_waits(lib):  # noqa: F811
     torch.cuda.synchronize()
     lib.moe.sync()
     assert all(torch.equal(o, want) for o in outs)
+
+
+# ---- NaN and infinities ---------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D", [256, 1024])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_add_rmsnorm_keeps_what_is_not_finite(lib, D, value):  # noqa: F811
+    """A NaN spreads over its row, an infinity leaves a NaN in its place (its row's norm is infinite): the Q8_K values say
+    so as the other outputs do, and the other rows are as without it."""
+    x = torch.randn(5, D, generator=gen(1))
+    w = 1 + 0.1 * torch.randn(D, generator=gen(2))
+    _, xb0, q0 = lib.add_rmsnorm(x.cuda(), None, w.cuda(), xb_dtype=torch.float32)
+    x[2, 7] = value
+    xo, xb, q8 = lib.add_rmsnorm(x.cuda(), None, w.cuda(), xb_dtype=torch.float32)
+    lib.moe.sync()
+    assert torch.equal(xo.cpu().nan_to_num(7.0), x.nan_to_num(7.0)) and xb[2, 7].isnan()
+    v = lib.read_q8(q8, torch.float32)
+    blocks = xb[2].view(-1, 256).isnan().any(1)
+    assert blocks[0] and torch.equal(v[2].view(-1, 256).isnan().all(1), blocks)
+    assert not v[2].view(-1, 256)[~blocks].isnan().any()
+    others = [0, 1, 3, 4]
+    assert torch.equal(xb[others], xb0[others]) and torch.equal(q8[others], q0[others])
+
+
+def test_add_rmsnorm_infinite_weight(lib):  # noqa: F811
+    x = torch.randn(2, 512, generator=gen(1)).cuda()
+    w = torch.ones(512)
+    w[300] = float("inf")
+    q8 = lib.add_rmsnorm(x, None, w.cuda())[2]
+    v = lib.read_q8(q8, torch.float32)
+    assert torch.isfinite(v[:, :256]).all() and not torch.isfinite(v[:, 256:]).any()
+    assert torch.equal(q8[:, 0], lib.add_rmsnorm(x, None, None)[2][:, 0])
+
+
+@pytest.mark.parametrize("rows,hkv", [([(1, 300), (1, 90)], 2), ([(8, 700)], 2), ([(130, 400)], 8), ([(200, 2100)], 8), ([(400, 900)], 8)],
+                         ids=["decode", "verify", "tiles", "split", "more"])
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=20.0), dict(window=50)], ids=["plain", "cap", "window"])
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+def test_attend_nan_and_infinite_q(lib, rows, hkv, kw, name):  # noqa: F811
+    """A NaN makes its own row NaN, infinities stand for +-65504; every other row is the same, bit for bit."""
+    from test_attn_ops import DTYPES
+    c = Case(rows, 32, hkv, 64, seed=3)
+    H = 4 * hkv
+    q = torch.randn(c.T, H, 64, generator=gen(9)).to(DTYPES[name])
+    big = torch.tensor(65504.0).to(DTYPES[name])
+    q[c.T - 1, 1, 3], q[0, H - 2, 60] = big, -big
+    want = lib.attend(c.cache, c.batch, q.cuda(), **kw)
+    assert torch.isfinite(want).all()
+    q[c.T - 1, 1, 3], q[0, H - 2, 60] = float("inf"), float("-inf")
+    nan = (c.T // 2, 2)
+    q[nan[0], nan[1], 11] = float("nan")
+    out = lib.attend(c.cache, c.batch, q.cuda(), **kw)
+    lib.moe.sync()
+    assert out[nan].isnan().all()
+    keep = torch.ones(c.T, H, dtype=torch.bool, device="cuda")
+    keep[nan] = False
+    assert torch.equal(out[keep], want[keep])
