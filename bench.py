@@ -29,8 +29,12 @@ Printed JSON (one line, rank 0):
              same input rows: ids, Q8_K, weights, rel-L2 and max-abs; a miss
              makes the run exit non-zero;
   cpu_baseline  the reference's own CPU path on this host's cores (rank 0, N=1).
+             Where oracle/_ref is not built, the oracle's scalar port stands in
+             ("kind": "port").
 --impl reference times the reference's CPU path (oracle/_ref, built from the
-reference sources) on the same workload and prints the same config.
+reference sources) on the same workload and prints the same config.  Where it is
+not built the line says "unavailable" and why; its value is then a sample of the
+oracle's scalar port ("kind": "port") and no figure of the reference.
 """
 from __future__ import annotations
 
@@ -235,9 +239,11 @@ def cpu_baseline(cfg, seconds=12.0, threads=0):
     if os.path.exists(REF_SO):
         R = Reference(threads)
         kind_s, cores, label = "reference", R.n_threads, f"{R.isa}; {R.cpu}"
+        what, call = "the reference", "one lfm2_forward_moe_ffn_1x4 per token"
     else:
         R = Oracle()
-        kind_s, cores, label = "port", 1, "scalar oracle port"
+        kind_s, cores, label = "port", 1, "the reference's library is not built here"
+        what, call = "the oracle's scalar port, one thread", "not the reference"
     per_tok = {}
     T = min(cfg["T"], 8)
     for kind in kinds:
@@ -252,7 +258,7 @@ def cpu_baseline(cfg, seconds=12.0, threads=0):
     t_tok = cfg["layers"] * per_tok["moe"] + cfg.get("dense", 0) * per_tok.get("dense", 0.0)
     n_layers = cfg["layers"] + cfg.get("dense", 0)
     return {"value": 1.0 / t_tok, "unit": "tok/s", "cores": cores, "kind": kind_s,
-            "sample": f"per-token time of the reference ({T}-token calls, one lfm2_forward_moe_ffn_1x4 per token) on "
+            "sample": f"per-token time of {what} ({T}-token calls, {call}) on "
                       f"one MoE layer ({per_tok['moe'] * 1e6:.0f} us)"
                       + (f" and one dense layer ({per_tok['dense'] * 1e6:.0f} us)" if "dense" in per_tok else "")
                       + (f", extrapolated to the {n_layers}-layer stack" if n_layers > 1 else "")
@@ -263,20 +269,23 @@ def run_reference(args, cfg_id, cfg):
     """--impl reference: the reference's own CPU path (oracle/_ref) on the same workload.  A step is
     the config's whole stack over its T tokens, one lfm2_forward_moe_ffn_1x4 call per token and
     layer (dense layers: lfm2_forward_ffn_fused_1x4's path); all host threads but one (the reference
-    pool's default).  Inputs come from the oracle's own build of the seeded generator."""
+    pool's default).  Inputs come from the oracle's own build of the seeded generator.  Without the
+reference's library there is nothing to time, and the line says so."""
     ws, rank, _ = dist_setup()
     if rank != 0:
         return
     from laii_b200 import synth
-    from oracle.oracle import GEN_SO, REF_SO, Oracle, Reference
+    from oracle.oracle import GEN_SO, REF_SO, Reference
     if os.path.exists(GEN_SO):
         synth.use_generator_library(GEN_SO)
-    if os.path.exists(REF_SO):
-        R = Reference(0)
-        kind, cores, label = "reference", R.n_threads, f"{R.isa}; {R.cpu}"
-    else:
-        R = Oracle()
-        kind, cores, label = "port", 1, "scalar oracle port"
+    if not os.path.exists(REF_SO):
+        port = cpu_baseline(cfg, seconds=min(2.0, args.cpu_seconds))
+        print(json.dumps({"impl": "reference", "unavailable": "the reference's CPU library (oracle/_ref/libref_moe.so) is not "
+                          "built: its sources are not here; value is a sample of the oracle's scalar port",
+                          "config": workload(cfg_id, cfg), **port}), flush=True)
+        return
+    R = Reference(0)
+    kind, cores, label = "reference", R.n_threads, f"{R.isa}; {R.cpu}"
     layers = stack_layers(cfg)
     host = [(k, host_layer(cfg, k, l)) for k, l in layers]
     T = cfg["T"]
