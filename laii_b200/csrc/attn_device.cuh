@@ -107,9 +107,10 @@ __device__ __forceinline__ bool lfm_sane(const BatchDev &bt, int64_t q0, int64_t
 /* Reports sequences whose rows are out of order or beyond the call's: the thread looks at sequences at, at + step, ... */
 __device__ __forceinline__ void lfm_check_batch(const BatchDev &bt, uint32_t at, uint32_t step, uint32_t *err) {
     bool sane = true;
+#pragma unroll 1
     for (uint32_t b = at; b < bt.n_seqs; b += step) {
-        const int64_t q = bt.q_start[b];
-        sane &= lfm_sane(bt, q, (int64_t)bt.q_start[b + 1] - q);
+        const uint32_t q = (uint32_t)bt.q_start[b], end = (uint32_t)bt.q_start[b + 1]; /* negative: above n_tokens */
+        sane &= q <= end && end <= bt.n_tokens;
     }
     if (!sane) atomicOr(err, LFM_DEVERR_PAGE);
 }

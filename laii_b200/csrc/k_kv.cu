@@ -149,7 +149,7 @@ __device__ __forceinline__ int locate(const BatchDev &bt, uint32_t tok, int64_t 
             q1 = bt.q_start[b + 1];
             len = bt.kv_len[b];
         }
-        const uint32_t who = __ballot_sync(LFM_FULL_MASK, q0 <= (int64_t)tok && (int64_t)tok < q1 && lfm_sane(bt, q0, q1 - q0));
+        const uint32_t who = __ballot_sync(LFM_FULL_MASK, q0 >= 0 && q0 <= (int64_t)tok && (int64_t)tok < q1 && q1 <= (int64_t)bt.n_tokens);
         if (who) {
             const int src = __ffs(who) - 1;
             pos = __shfl_sync(LFM_FULL_MASK, len - (q1 - q0) + ((int64_t)tok - q0), src);
@@ -164,12 +164,10 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(AppendArgs A, uint32_t per
     constexpr uint32_t kL = D / 8, kHeads = 32 / kL; /* lanes of a head, heads of a step */
     lfm_pdl_wait();
     lfm_pdl_launch_dependents();
+    if (blockIdx.x == 0) lfm_check_batch(A.bt, threadIdx.x, blockDim.x, A.err);
     const uint32_t task = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, sub = lane % kL;
     const uint32_t tok = task / per_token, own = lane / kL;
-    if (tok >= A.bt.n_tokens) {
-        if (blockIdx.x == gridDim.x - 1) lfm_check_batch(A.bt, threadIdx.x, blockDim.x, A.err); /* a block behind the tokens' */
-        return;
-    }
+    if (tok >= A.bt.n_tokens) return;
     /* a step is all q, all k or all v */
     const uint32_t hkv = A.k ? A.kv.hkv : 0, nq = (A.n_heads + kHeads - 1) / kHeads, nk = (hkv + kHeads - 1) / kHeads;
     const uint32_t first = task % per_token * steps, end = min(nq + 2 * nk, first + steps);
@@ -233,12 +231,10 @@ __global__ void __launch_bounds__(256) k_kv_read(ReadArgs A, uint32_t per_token)
     constexpr uint32_t kL = D / 8, kHeads = 32 / kL;
     lfm_pdl_wait();
     lfm_pdl_launch_dependents();
+    if (blockIdx.x == 0) lfm_check_batch(A.bt, threadIdx.x, blockDim.x, A.err);
     const uint32_t task = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, sub = lane % kL;
     const uint32_t tok = task / per_token, first = task % per_token * kPass * kHeads + lane / kL;
-    if (tok >= A.bt.n_tokens) {
-        if (blockIdx.x == gridDim.x - 1) lfm_check_batch(A.bt, threadIdx.x, blockDim.x, A.err); /* a block behind the tokens' */
-        return;
-    }
+    if (tok >= A.bt.n_tokens) return;
     int64_t pos = 0;
     const int b = locate(A.bt, tok, pos);
     if (b < 0) return;
@@ -283,7 +279,7 @@ cudaError_t launch_append(const AppendArgs &a, cudaStream_t s, bool pdl) {
     constexpr uint32_t kHeads = 256 / D;
     const uint32_t steps = (a.n_heads + kHeads - 1) / kHeads + (a.k ? 2 * ((a.kv.hkv + kHeads - 1) / kHeads) : 0);
     const uint32_t pass = (uint64_t)steps * a.bt.n_tokens > kManySteps ? 8 : 1, per = (steps + pass - 1) / pass;
-    const uint64_t blocks = ((uint64_t)per * a.bt.n_tokens + 7) / 8 + 1; /* the last looks the offsets over */
+    const uint64_t blocks = ((uint64_t)per * a.bt.n_tokens + 7) / 8;
     if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
     return lfm_launch_pdl(k_kv_append<T, D>, dim3((uint32_t)blocks), dim3(256), 0, s, pdl, a, per, pass);
 }
@@ -291,7 +287,7 @@ template <class T, int D>
 cudaError_t launch_read(const ReadArgs &a, cudaStream_t s, bool pdl) {
     const uint32_t steps = (2 * a.kv.hkv * (D / 8) + 31) / 32;
     const uint32_t pass = (uint64_t)steps * a.bt.n_tokens > kManySteps ? 8 : 1, per = (steps + pass - 1) / pass;
-    const uint64_t blocks = ((uint64_t)per * a.bt.n_tokens + 7) / 8 + 1; /* the last looks the offsets over */
+    const uint64_t blocks = ((uint64_t)per * a.bt.n_tokens + 7) / 8;
     if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
     return lfm_launch_pdl(pass == 8 ? k_kv_read<T, D, 8> : k_kv_read<T, D, 1>, dim3((uint32_t)blocks), dim3(256), 0, s, pdl, a, per);
 }
