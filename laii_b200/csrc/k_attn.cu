@@ -28,12 +28,17 @@
  * leaves the longest sequence to one SM, took 92 us where equal parts take 73
  * (64 sequences of up to 8192 keys).
  *
- * Bound by instruction issue: a step of 16 keys is some 220 instructions of a
- * warp, unpacking above all, for 1152 bytes.  32 / 8 heads, 64-value heads, 64
- * tokens on ragged sequences of up to 8192 keys: 62 us, 187 MB read, 3.0 TB/s;
- * issue 56%, HBM 34 to 47%.  128-value heads, two sequences of 131072 keys:
- * 83 us, 302 MB, 3.6 TB/s.  One token on 1024 keys: 9.2 us, a chain of table, copy,
- * products and join.  Eight tokens of each of 16 sequences of up to 8192 keys: 45 us.
+ * Where the time goes: 32 / 8 heads of 64 values, 64 tokens on ragged sequences
+ * of up to 8192 keys take 62 us for 186 MB, 3.0 TB/s (46% of a copy's rate).  No
+ * pipe is full: issue 57%, tensor pipe 17%.  A step of 16 keys is some 220
+ * instructions of a warp, unpacking above all, for 1152 bytes, in one chain of
+ * dependent ones, and an SM holds 16 warps: of the 6.1 cycles between a warp's
+ * instructions 1.4 pass in the fixed latency of the one before, 1.0 until its
+ * turn, 0.7 for a busy arithmetic pipe, 0.7 for memory, 0.6 at the join's barriers
+ * and fences.  128-value heads, two sequences of 131072 keys: 83 us, 302 MB, 3.6
+ * TB/s (56%), the same picture.  One token on 1024 keys: 9.0 us, a chain of table,
+ * copy, products and join.  72 tokens of 16 sequences (2 to 7 each) of up to 8192
+ * keys: 46 us, two warps a scheduler with wide tiles half empty, issue 27%.
  */
 #include <type_traits>
 
@@ -722,8 +727,8 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
     const uint64_t walk = B * ((per + 7) / 8) * a.kv.hkv * span * keys / ((uint64_t)sm_count * (head_dim == 64 ? 16 : 12));
     const bool split = B * ((per + 31) / 32) * a.kv.hkv < (uint64_t)sm_count / 2;
     const uint32_t nt = per <= 8 || walk <= 256 ? 1 : per <= 16 || head_dim == 128 || (walk <= 1024 && split) ? 2 : 4;
-    /* blocks: as many as run at once (registers: more, with spills, ran slower), fewer where there are not enough
-     * blocks of keys by the hint */
+    /* blocks: as many as run at once by their registers (some instances spill 20 to 136 bytes at that; more blocks, with
+     * fewer registers and more spills, ran slower), fewer where there are not enough blocks of keys by the hint */
     uint64_t grid = (uint64_t)sm_count * (head_dim * nt < 128 ? 4 : head_dim * nt == 128 ? 3 : 2);
     const uint64_t units = (B + T * G / (8 * nt)) * a.kv.hkv, work = units * (span + 1);
     const uint64_t most = work / kWarps > units ? work / kWarps : units;
@@ -739,9 +744,9 @@ static cudaError_t lfm_launch_attn_rows(const AttnArgs &a, uint32_t head_dim, ui
 }
 
 /* Which kernel takes a sequence.  Per SM, 32 rows against 64 keys take this file's kernel 0.44 us (64-value heads;
- * 128: 0.98), and 256 rows, however few of them there are, the tile kernel 1.1 us (1.15).  This one spreads any work
- * over all SMs, the tile kernel whole rounds of tiles or of their parts; a call for both pays for two launches.  So
- * both sides are estimated, in blocks of keys, and the shorter taken.  Measured, 32 / 8 heads, rows of a sequence
+ * 128: 0.98), and 256 rows, however few of them there are, the tile kernel 0.99 us (1.18): about 2 to 5 and 6 to 7.
+ * This one spreads any work over all SMs, the tile kernel whole rounds of tiles or of their parts; a call for both pays
+ * for two launches.  So both sides are estimated, in blocks of keys, and the shorter taken.  Measured, 32 / 8 heads, rows of a sequence
  * (token, head of the group), this kernel and the other:
  *   32 sequences of 4096 keys, 64-value heads   64 rows: 110 us, 115;  128: 201, 174;  256: 376, 140
  *                              128-value heads  32 rows: 122, 136;  64: 225, 216;  128: 428, 213
@@ -755,7 +760,7 @@ cudaError_t lfm_launch_attn(const AttnArgs &a, uint32_t head_dim, uint32_t max_k
     if (a.window && max_kv_len > (uint64_t)a.window + 256) max_kv_len = a.window + 256;
     const uint64_t T = a.bt.n_tokens, B = a.bt.n_seqs, rows = T * a.group, few = B == 1 ? 0 : head_dim == 64 ? 64 : 32;
     const TilePlan p = lfm_attn_tile_plan(a, head_dim, few, max_kv_len, sm_count);
-    const uint64_t here = (rows + 16 * B) / 32 * a.kv.hkv * (p.blocks + 12);   /* 12: a unit's cost beside its blocks */
+    const uint64_t here = (rows + 16 * B) / 32 * a.kv.hkv * (p.blocks + 12);   /* 12: a unit's cost beside its blocks, by the pairs above */
     const uint64_t there = (p.cost + (B == 1 ? 3 : 10)) * (uint64_t)sm_count;  /* 10: the second launch */
     /* sequences of few rows by their average, and of no odd one that could be long: a step of single tokens (64
      * sequences of 8192 keys: 86 us, 92 with an idle launch of the other kernel), a batch to verify (16 sequences of

@@ -34,13 +34,17 @@
  * relative, under the output's rounding and q's own); scores, m, the sum and O
  * are fp32, p is fp16 <= 2^15.
  *
- * 32 / 8 heads.  4096 tokens from the beginning, 64-value heads: 130 us, 530
+ * 32 / 8 heads.  4096 tokens from the beginning, 64-value heads: 128 us, 537
  * TFLOP/s; 42 us of tensor work, 60 of exponentials (one a score, 16 a clock and
- * SM).  2048 tokens behind 14336, 128-value heads: 540 us call after call, 580
- * with other work between, 950 and 890 TFLOP/s; 314 of tensor work.  What is
- * between is the hand-over from role to role for each block: tensor pipe 51%,
- * exponential unit 51%, issue 50% for 128-value heads (25, 50, 45 for 64), and
- * without the softmax's arithmetic the same barriers take 91 and 344 us.
+ * SM).  2048 tokens behind 14336, 128-value heads: 525 us call after call, 560 to
+ * 575 with other work between, some 900 TFLOP/s; 314 of tensor work.  12 ragged
+ * chunks, 3891 tokens in all, window 1024, capped: 128 us, 53 of them the three
+ * operations of the exponential unit for each score.  No pipe is full: for the
+ * prompt tensor 25%, exponential unit 51%, issue 46% (chunk: 51, 51, 50; capped:
+ * 11, 68, 38).  Of the 8.3 cycles between a warp's instructions 2.1 wait for tensor
+ * memory and barriers, 2.1 for the instruction before (capped: 3.4 and 2.2 of 10):
+ * the hand-over from role to role for each block, with two softmax warps a
+ * scheduler.  Without the softmax's arithmetic the same barriers take 91 and 344 us.
  * The few-row kernel's fragments in registers took 696 and 3469 us, a block's
  * barriers for 128 keys at a time 141 and 646 when 64 took 138 and 595.  512 rows on 16384 keys: 50 us, in one part 245.
  */
@@ -53,8 +57,9 @@ namespace {
 constexpr int kM = 128, kRows = 2 * kM, kKeys = 64, kThreads = 512;
 constexpr uint32_t kChunkQ = kM * 16, kChunk = kKeys * 16; /* bytes between the 8-value chunks of a row */
 
-/* Key blocks that a part of a split tile has at least; what a tile costs beside its blocks, in blocks (32 blocks in 44
- * us, 256 in 245: 1.1 us a block and 8 us). */
+/* Key blocks that a part of a split tile has at least; what a tile costs beside its blocks, in blocks.  64-value heads,
+ * one tile an SM of 8, 32, 128 key blocks: 17.5, 43.0, 136 us, each further one 12.9, 38.4, 132: 0.99 us a block and 5 us;
+ * 128-value heads 24.3, 52.7, 164 and 20.0, 48.3, 161: 1.18 us and 10.5, nine blocks. */
 constexpr uint32_t kPartBlocks = 8, kJobBlocks = 6;
 
 template <int D>

@@ -14,10 +14,13 @@
  * back and attending see the d that the code was chosen for.
  *
  * Floor: the rows of q, k and v read, q and the codes written.  5307 tokens of
- * 32 / 8 heads of 128 values, 116 MB: 30.0 us, 3.9 TB/s, read back 8.6 us.  By
- * instruction issue (59%) and the loads' latency together: HBM stands at 30%.  A
- * block of threads for each token, its steps between barriers: 74 us for both,
- * 42 so.  64 tokens, 64-value heads: 3.1 us, a launch and a chain of loads.
+ * 32 / 8 heads of 128 values, 116 MB: 30.1 us, 3.9 TB/s, read back (28 MB, 4.3 us
+ * at a copy's rate) 8.8 us.  Neither pipe is full (issue 62%, HBM 30%): with 24
+ * warps an SM and two loads of each under way, of the 9.1 cycles between a warp's
+ * instructions 3.2 wait for memory, 1.6 for the instruction before, 1.6 for their
+ * turn; the reading kernel is one such chain a warp.  A block of threads for each
+ * token, its steps between barriers: 74 us for both, 42 so.  64 tokens, 64-value
+ * heads: 3.1 us, a launch and a chain of loads.
  */
 #include "attn_device.cuh"
 

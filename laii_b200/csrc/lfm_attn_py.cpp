@@ -6,7 +6,7 @@
  * stream in one step.  A small call is as long as its way to the launch: through
  * ctypes, with the checks and allocations in Python, a row norm of 64 rows with
  * its read-back took 17.3 us for 3.3 us on the device; two launches alone take
- * 5.  So: 8.6 us.
+ * 5.  So: 8 to 9 us.
  * Functions return their outputs, or the status as an int where it is not 0.
  */
 #include <torch/csrc/Exceptions.h>
